@@ -455,6 +455,77 @@ int mivos_resize_bicubic(const float *x, float *out, int planes, int h, int w, i
 int mivos_onehot_nearest(const uint8_t *label_map, const uint8_t *labels, int n_labels, float *out, int h, int w, int H,
                          int W, int64_t out_pstride, int64_t out_rstride, int pad_top, int pad_left, void *stream);
 
+/* ---- token memory: rotary positions over several axes, norm + rotary of queries and keys, a memory bank held in 4 bits ----
+ * Operators of a transformer over video tokens next to the space-time memory: tokens carry a (time, height, width) position, queries and
+ * keys of every head are normed and turned, keys and values are kept in a bank of 4-bit blocks that attention reads and that is brought
+ * back to a budget by dropping the slots that received the least attention. */
+
+typedef enum { MIVOS_F32 = 0, MIVOS_F16 = 1, MIVOS_BF16 = 2 } mivos_dtype;
+
+/* One operand (queries or keys) of the rotary entries: element (b, n, h, c) of x at x + b*xb + n*xn + h*xh + c (strides in ELEMENTS, the
+ * channel stride is 1), g likewise; y is dense [batch][tokens][heads][dim].  heads = 0: absent (rows[1] only). */
+typedef struct {
+  const void *x;       /* forward: the input.  norm_rotary_grad: the forward input                        */
+  const void *g;       /* norm_rotary_grad: gradient of the forward output; else NULL                     */
+  void *y;             /* forward: the output.  norm_rotary_grad: gradient of x                           */
+  const float *weight; /* [dim], norm only                                                                */
+  int64_t xb, xn, xh, gb, gn, gh;
+  int32_t heads;       /* at most 4096                                                                    */
+  int32_t reserved;
+} mivos_rotary_rows;
+typedef struct {
+  mivos_rotary_rows rows[2];      /* queries, keys                                                        */
+  const int32_t *positions;       /* position of token (b, n) on axis a at b*pb + n*pn + a*pa             */
+  const uint64_t *freq;           /* [pairs] turns a position in units of 2^-64 (round(f / (2 pi) * 2^64)) */
+  const int32_t *axis;            /* [pairs] the axis pair i turns with                                   */
+  void *workspace;                /* norm_rotary_grad                                                     */
+  int64_t pb, pn, pa, workspace_bytes;
+  int32_t batch, tokens, dim, pairs; /* dim 2..512, 2*pairs <= dim; channels behind the pairs are not turned */
+  int32_t dtype;                  /* mivos_dtype of x, g, y                                               */
+  int32_t interleaved;            /* pair i = channels (2i, 2i+1); 0: (i, i + pairs)                      */
+  int32_t inverse;                /* turn by minus the angle: the gradient of the rotation                */
+  float eps;                      /* >= 0: x / sqrt(mean(x^2) + eps) * weight first; < 0: no norm         */
+} mivos_rotary;
+int mivos_rotary_axes(const mivos_rotary *d, void *stream);
+int64_t mivos_norm_rotary_grad_workspace_bytes(int dim);
+/* dx of both operands, and the gradients of the two norm weights (fp32 [dim], written, summed over all rows in a fixed order). */
+int mivos_norm_rotary_grad(const mivos_rotary *d, float *dq_weight, float *dk_weight, void *stream);
+
+/* The bank: dense [batch][heads][slots][...] buffers.  A row of D channels is D/2 bytes of codes (even channel in the low half; sign, two
+ * exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) and D/32 scale bytes (value = code * 2^(byte - 127); append writes 7..252,
+ * the smallest power of two with max |x| <= 6 * 2^e, and 255 for a block that holds an infinity or a NaN, which stands for NaN).
+ * Slots [0, lens[b]) of stream b are filled; the others are never interpreted. */
+typedef struct {
+  uint8_t *key_codes, *key_scales, *value_codes, *value_scales;   /* 16-byte aligned                      */
+  float *weight;       /* [batch][heads][slots] softmax weight the slot has received                      */
+  int32_t *lens;       /* [batch]                                                                         */
+  int32_t *status;     /* [1 + batch], zeroed by the owner once: word 0 bit 0 is raised when appended tokens did not fit; the others are
+                          counters of the append kernel (zero between calls)                              */
+  int64_t slots;       /* at most 2^30                                                                    */
+  int32_t batch, heads, key_dim, value_dim;                       /* dims: multiples of 32 up to 1024     */
+} mivos_bank4;
+/* keys [batch][tokens][heads][key_dim], values [...][value_dim] (strides as above): token t < count[b] (NULL: all) of stream b goes to slot
+ * at[b] + t, its weight becomes 0, lens[b] = at[b] + count[b].  at may be bank->lens itself (append behind what is there).  Tokens whose
+ * slot is outside the bank are dropped and raise status bit 0. */
+int mivos_bank4_append(const mivos_bank4 *bank, const void *keys, int64_t kb, int64_t kt, int64_t kh, const void *values, int64_t vb, int64_t vt,
+                       int64_t vh, int dtype, const int32_t *at, const int32_t *count, int tokens, void *stream);
+/* What slots [first[b], first[b] + count) (first NULL: 0) stand for: dense [batch][heads][count][key_dim] / [value_dim], fp32 or bf16 (both
+ * exact); 0 for slots outside [0, lens[b]). */
+int mivos_bank4_values(const mivos_bank4 *bank, const int32_t *first, int64_t count, void *key_out, void *value_out, int dtype, void *stream);
+/* q (b, t, j, c) at b*qb + t*qt + j*qh + c, q_heads a multiple of bank->heads (bank head j / (q_heads / heads)); out dense
+ * [batch][tokens][q_heads][value_dim] = softmax over the visible slots of scale * q . k, times v.  Visible: all filled slots; causal: token t
+ * of count[b] (NULL: tokens) sees slots < lens[b] - count[b] + t + 1 (the tokens are the newest ones, already appended).  Tokens >= count[b]
+ * and rows that see nothing give 0.  weigh: weight[b][h][s] += the softmax weights of the stream's rows on slot s.  key_dim 64, 128 or 256,
+ * value_dim a multiple of 64, at most 2^20 rows (tokens x q_heads / heads). */
+int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int q_heads, int tokens, int weigh);
+int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t qb, int64_t qt, int64_t qh, int dtype, int q_heads, int tokens, const int32_t *count,
+                     float scale, int causal, int weigh, void *out, void *workspace, int64_t workspace_bytes, void *stream);
+/* Keeps `keep` slots of every (stream, head): the first `first`, the last `recent` and, of the others, those with the largest weight (equal
+ * weights: the lowest slots; NaN counts as the least), in their order, in bank `out` (other buffers, slots >= keep) with their weights;
+ * out->lens[b] = min(lens[b], keep).  slots_out [batch][heads][keep]: the slots they came from, -1 behind them.  Rows of `out` behind its new
+ * length are left as they were. */
+int mivos_bank4_evict(const mivos_bank4 *bank, const mivos_bank4 *out, int64_t keep, int64_t first, int64_t recent, int32_t *slots_out, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

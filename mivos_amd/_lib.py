@@ -43,6 +43,25 @@ class FusionNetDesc(C.Structure):
                 ("workspace_bytes", i64)]
 
 
+class RotaryRows(C.Structure):
+    """mivos_rotary_rows"""
+    _fields_ = [("x", vp), ("g", vp), ("y", vp), ("weight", vp), ("xb", i64), ("xn", i64), ("xh", i64), ("gb", i64), ("gn", i64), ("gh", i64),
+                ("heads", i32), ("reserved", i32)]
+
+
+class RotaryDesc(C.Structure):
+    """mivos_rotary"""
+    _fields_ = [("rows", RotaryRows * 2), ("positions", vp), ("freq", vp), ("axis", vp), ("workspace", vp), ("pb", i64), ("pn", i64), ("pa", i64),
+                ("workspace_bytes", i64), ("batch", i32), ("tokens", i32), ("dim", i32), ("pairs", i32), ("dtype", i32), ("interleaved", i32),
+                ("inverse", i32), ("eps", f32)]
+
+
+class Bank4Desc(C.Structure):
+    """mivos_bank4"""
+    _fields_ = [("key_codes", vp), ("key_scales", vp), ("value_codes", vp), ("value_scales", vp), ("weight", vp), ("lens", vp), ("status", vp),
+                ("slots", i64), ("batch", i32), ("heads", i32), ("key_dim", i32), ("value_dim", i32)]
+
+
 # name -> (restype, argtypes); every symbol include/mivos_hip.h declares
 PROTOTYPES = {
     "mivos_version": (C.c_int, []),
@@ -111,6 +130,14 @@ PROTOTYPES = {
     "mivos_ingest_u8": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, i64, i64, i64, C.c_int, C.c_int, C.POINTER(f32), C.POINTER(f32), vp]),
     "mivos_resize_bicubic": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, i64, i64, C.c_int, C.c_int, vp]),
     "mivos_onehot_nearest": (C.c_int, [vp, vp, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int, i64, i64, C.c_int, C.c_int, vp]),
+    "mivos_rotary_axes": (C.c_int, [C.POINTER(RotaryDesc), vp]),
+    "mivos_norm_rotary_grad_workspace_bytes": (i64, [C.c_int]),
+    "mivos_norm_rotary_grad": (C.c_int, [C.POINTER(RotaryDesc), vp, vp, vp]),
+    "mivos_bank4_append": (C.c_int, [C.POINTER(Bank4Desc), vp, i64, i64, i64, vp, i64, i64, i64, C.c_int, vp, vp, C.c_int, vp]),
+    "mivos_bank4_values": (C.c_int, [C.POINTER(Bank4Desc), vp, i64, vp, vp, C.c_int, vp]),
+    "mivos_bank4_read_workspace_bytes": (i64, [C.POINTER(Bank4Desc), C.c_int, C.c_int, C.c_int]),
+    "mivos_bank4_read": (C.c_int, [C.POINTER(Bank4Desc), vp, i64, i64, i64, C.c_int, C.c_int, C.c_int, vp, f32, C.c_int, C.c_int, vp, vp, i64, vp]),
+    "mivos_bank4_evict": (C.c_int, [C.POINTER(Bank4Desc), C.POINTER(Bank4Desc), i64, i64, i64, vp, vp]),
     "mivos_interleave_planes": (C.c_int, [C.POINTER(InterleaveDesc), vp, C.c_int, i64, vp]),
 }
 

@@ -1,0 +1,409 @@
+// Rotary positions with several axes (time, height, width), alone or behind the norm of each head's query / key, and their gradients.
+//
+//   n = w * x * (mean(x^2) + eps)^(-1/2)                      (norm; w per channel, shared by the heads)          or n = x
+//   y[u] = n[u] cos a_i - n[v] sin a_i,  y[v] = n[v] cos a_i + n[u] sin a_i        a_i = position[axis_i] * f_i,   pair i = channels (u, v)
+// with pairs (2i, 2i + 1) or (i, i + pairs); channels behind the pairs keep n.  Backward: g = the rotation by -a of dy,
+//   dx = r (w g - x r^2 mean(w g x)),  r = (mean(x^2) + eps)^(-1/2),      dw = sum over the rows of g x r.
+//
+// The angle.  A position times a frequency is needed modulo a turn only, so the frequency is kept as a 64-bit fraction of a turn and the
+// product taken modulo 2^64: exact to 2^-33 turns for every 32-bit position (an fp32 product is off by 0.004 radian at position 70 000).
+// Sine and cosine are Taylor polynomials on an eighth of a turn to either side (error < 2^-24), once a token and pair: a workgroup puts them in LDS
+// and all heads of its tokens read them there.
+//
+// Bound: bytes.  Every row is read once and written once (backward: x and dy once, dx once); a row of 16 * U channels is held by
+// 2^ceil(log2 U) neighbouring lanes, 16 channels a lane, so the mean is log2 lane exchanges and nothing is staged.
+#include "bank4.h"
+
+namespace mivos {
+
+struct RotaryRows {
+  const void *x, *g;
+  void *y;
+  const float *weight;
+  int64_t xb, xn, xh, gb, gn, gh;
+  int heads;
+};
+struct RotaryArgs {
+  RotaryRows rows[2];
+  const int32_t *pos;
+  int64_t pb, pn, pa;
+  const uint64_t *freq;
+  const int32_t *axis;
+  float *partial;                     // backward: [workgroup][2][dim]
+  int batch, tokens, dim, pairs, interleaved, norm, tile, n_tiles;
+  float eps, sign;
+};
+
+// sine and cosine of pos * freq turns (freq in 2^-64 turns)
+__device__ __forceinline__ void turn_sincos(int32_t pos, uint64_t freq, float sign, float &s, float &c) {
+  const uint32_t turn = (uint32_t)(((uint64_t)(int64_t)pos * freq) >> 32);
+  const uint32_t quarter = (turn + 0x20000000u) >> 30;
+  const float x = (float)(int32_t)(turn - (quarter << 30)) * 1.4629180792671596e-9f;      // 2 pi / 2^32: [-pi/4, pi/4)
+  const float z = x * x;
+  const float sx = x * (1.f + z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880)))));
+  const float cx = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
+  float sn = quarter & 1 ? cx : sx, cs = quarter & 1 ? sx : cx;
+  if (quarter & 2) sn = -sn;
+  if ((quarter + 1) & 2) cs = -cs;
+  s = sign * sn;
+  c = cs;
+}
+
+// ------------------------------------------------------------------------------------------ any width, any alignment: one wave a row
+// Lane l holds channels l, l + 64, ...; dim <= 512.
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void rotary_any_kernel(RotaryArgs a) {
+  __shared__ float dw[4][2][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_token = a.rows[0].heads + a.rows[1].heads;
+  const int64_t total = (int64_t)a.batch * a.tokens * per_token;
+  float acc[2][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[0][j] = acc[1][j] = 0.f;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < total; row += (int64_t)gridDim.x * 4) {
+    const int64_t bn = row / per_token;
+    int h = (int)(row - bn * per_token);
+    const int b = (int)(bn / a.tokens), n = (int)(bn - (int64_t)b * a.tokens), which = h >= a.rows[0].heads;
+    if (which) h -= a.rows[0].heads;
+    const RotaryRows &R = a.rows[which];
+    const T *x = (const T *)R.x + b * R.xb + n * R.xn + h * R.xh;
+    const T *g = GRAD ? (const T *)R.g + b * R.gb + n * R.gn + h * R.gh : x;
+    float xs[8], ps[8], sn[8], cs[8], ss = 0.f;      // own channel of the rotated operand, its partner's, and the turn
+    const T *rot = GRAD ? g : x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = lane + 64 * j;
+      xs[j] = ps[j] = sn[j] = 0.f;
+      cs[j] = 1.f;
+      if (c >= a.dim) continue;
+      xs[j] = (float)rot[c];
+      if (c < 2 * a.pairs) {
+        const int i = a.interleaved ? c >> 1 : c < a.pairs ? c : c - a.pairs;
+        const bool second = a.interleaved ? c & 1 : c >= a.pairs;
+        const int partner = a.interleaved ? c ^ 1 : second ? c - a.pairs : c + a.pairs;
+        ps[j] = (float)rot[partner];
+        if (a.norm && !GRAD) { ps[j] *= R.weight[partner]; }
+        turn_sincos(a.pos[b * a.pb + n * a.pn + a.axis[i] * a.pa], a.freq[i], second ? a.sign : -a.sign, sn[j], cs[j]);
+      }
+      ss += xs[j] * xs[j];
+    }
+    float r = 1.f;
+    if (a.norm && !GRAD) {
+      for (int d = 1; d < 64; d <<= 1) ss += __shfl_xor(ss, d);
+      r = 1.f / sqrtf(ss / a.dim + a.eps);
+    }
+    T *y = (T *)R.y + ((int64_t)bn * R.heads + h) * a.dim;
+    if constexpr (!GRAD) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = lane + 64 * j;
+        if (c < a.dim) y[c] = (T)(r * ((a.norm ? xs[j] * R.weight[c] : xs[j]) * cs[j] + ps[j] * sn[j]));
+      }
+    } else {
+      float xx[8], gw[8], dot = 0.f;
+      ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = lane + 64 * j;
+        xx[j] = gw[j] = 0.f;
+        if (c >= a.dim) continue;
+        xx[j] = (float)x[c];
+        xs[j] = xs[j] * cs[j] + ps[j] * sn[j];       // g
+        gw[j] = xs[j] * R.weight[c];
+        ss += xx[j] * xx[j];
+        dot += gw[j] * xx[j];
+      }
+      for (int d = 1; d < 64; d <<= 1) { ss += __shfl_xor(ss, d); dot += __shfl_xor(dot, d); }
+      r = 1.f / sqrtf(ss / a.dim + a.eps);
+      const float k = r * r * dot / a.dim;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = lane + 64 * j;
+        if (c < a.dim) y[c] = (T)(r * (gw[j] - xx[j] * k));
+        if (which) acc[1][j] += xs[j] * xx[j] * r;
+        else acc[0][j] += xs[j] * xx[j] * r;
+      }
+    }
+  }
+  if constexpr (GRAD) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { dw[wave][0][lane + 64 * j] = acc[0][j]; dw[wave][1][lane + 64 * j] = acc[1][j]; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * a.dim; i += 256) {
+      const int w = i / a.dim, c = i - w * a.dim;
+      a.partial[(int64_t)blockIdx.x * 2 * a.dim + i] = dw[0][w][c] + dw[1][w][c] + dw[2][w][c] + dw[3][w][c];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ 16 channels a lane
+// A lane's unit: 8 pairs (two runs of 8 channels `pairs` apart, or 16 neighbours), or 16 channels behind the pairs.
+template <bool INTER>
+__device__ __forceinline__ void unit_channels(int u, int pairs, int &c0, int &c1, bool &rot) {
+  rot = 8 * u < pairs;
+  if (rot && !INTER) { c0 = 8 * u; c1 = pairs + 8 * u; }
+  else { c0 = 16 * u; c1 = 16 * u + 8; }
+}
+// rotates the unit (lo, hi) by the table's angles
+template <bool INTER>
+__device__ __forceinline__ void unit_turn(f32x8 &lo, f32x8 &hi, const f32x2 *cs) {
+  f32x8 ol, oh;
+  if constexpr (INTER) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 e = cs[j], f = cs[4 + j];
+      ol[2 * j] = lo[2 * j] * e.x - lo[2 * j + 1] * e.y;
+      ol[2 * j + 1] = lo[2 * j + 1] * e.x + lo[2 * j] * e.y;
+      oh[2 * j] = hi[2 * j] * f.x - hi[2 * j + 1] * f.y;
+      oh[2 * j + 1] = hi[2 * j + 1] * f.x + hi[2 * j] * f.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const f32x2 e = cs[j];
+      ol[j] = lo[j] * e.x - hi[j] * e.y;
+      oh[j] = hi[j] * e.x + lo[j] * e.y;
+    }
+  }
+  lo = ol;
+  hi = oh;
+}
+
+template <typename T, bool INTER, bool NORM, bool GRAD>
+__global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a, int lanes /* a row, a power of two */) {
+  extern __shared__ __align__(16) f32x2 table[];     // [tile][pairs] (cos, sin); backward: the weight gradients afterwards
+  const int tid = threadIdx.x, units = a.dim / 16, slots = 256 / lanes, u = tid & (lanes - 1);
+  int c0, c1;
+  bool rot;
+  unit_channels<INTER>(u, a.pairs, c0, c1, rot);
+  const bool live = u < units;
+  f32x8 acc[2][2], w[2][2];
+  if constexpr (NORM || GRAD) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (live && a.rows[k].heads) {
+        w[k][0] = load8(a.rows[k].weight + c0, false);
+        w[k][1] = load8(a.rows[k].weight + c1, false);
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[k][0][j] = acc[k][1][j] = 0.f;
+
+  for (int tile = blockIdx.x; tile < a.n_tiles; tile += gridDim.x) {
+    const int64_t first = (int64_t)tile * a.tile, all = (int64_t)a.batch * a.tokens;
+    const int n_tok = (int)(all - first < a.tile ? all - first : a.tile);
+    __syncthreads();
+    for (int e = tid; e < n_tok * a.pairs; e += 256) {
+      const int t = e / a.pairs, i = e - t * a.pairs;
+      const int b = (int)((first + t) / a.tokens), n = (int)(first + t - (int64_t)b * a.tokens);
+      float s, c;
+      turn_sincos(a.pos[b * a.pb + n * a.pn + a.axis[i] * a.pa], a.freq[i], a.sign, s, c);
+      table[t * a.pairs + i] = f32x2{c, s};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const RotaryRows &R = a.rows[k];
+      const int n_rows = n_tok * R.heads;
+      for (int row = tid / lanes; row < n_rows; row += slots) {
+        const int t = row / R.heads, h = row - t * R.heads;
+        const int b = (int)((first + t) / a.tokens), n = (int)(first + t - (int64_t)b * a.tokens);
+        f32x8 lo, hi, xl, xh;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lo[j] = hi[j] = xl[j] = xh[j] = 0.f;
+        if (live) {
+          const T *x = (const T *)R.x + b * R.xb + n * R.xn + h * R.xh;
+          if constexpr (GRAD) {
+            const T *g = (const T *)R.g + b * R.gb + n * R.gn + h * R.gh;
+            xl = load8(x + c0, true);
+            xh = load8(x + c1, true);
+            lo = load8(g + c0, true);
+            hi = load8(g + c1, true);
+          } else {
+            lo = load8(x + c0, true);
+            hi = load8(x + c1, true);
+          }
+        }
+        if constexpr (NORM) {
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss += lo[j] * lo[j] + hi[j] * hi[j];
+          for (int d = 1; d < lanes; d <<= 1) ss += __shfl_xor(ss, d);
+          const float r = 1.f / sqrtf(ss / a.dim + a.eps);
+          lo *= r * w[k][0];
+          hi *= r * w[k][1];
+        }
+        if (rot && live) unit_turn<INTER>(lo, hi, table + t * a.pairs + 8 * u);
+        if constexpr (GRAD) {
+          const f32x8 gl = lo * w[k][0], gh = hi * w[k][1];
+          float ss = 0.f, dot = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            ss += xl[j] * xl[j] + xh[j] * xh[j];
+            dot += live ? gl[j] * xl[j] + gh[j] * xh[j] : 0.f;
+          }
+          for (int d = 1; d < lanes; d <<= 1) { ss += __shfl_xor(ss, d); dot += __shfl_xor(dot, d); }
+          const float r = 1.f / sqrtf(ss / a.dim + a.eps), q = r * r * dot / a.dim;
+          acc[k][0] += lo * xl * r;
+          acc[k][1] += hi * xh * r;
+          lo = r * (gl - xl * q);
+          hi = r * (gh - xh * q);
+        }
+        if (live) {
+          T *y = (T *)R.y + ((first + t) * R.heads + h) * a.dim;
+          store8(y + c0, lo);
+          store8(y + c1, hi);
+        }
+      }
+    }
+  }
+  if constexpr (GRAD) {                               // the workgroup's share of both weight gradients, its row slots in order
+    float *dw = reinterpret_cast<float *>(table);     // [slots][16 * lanes]
+    for (int k = 0; k < 2; ++k) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        dw[tid * 16 + j] = k ? acc[1][0][j] : acc[0][0][j];
+        dw[tid * 16 + 8 + j] = k ? acc[1][1][j] : acc[0][1][j];
+      }
+      __syncthreads();
+      for (int i = tid; i < units * 16; i += 256) {
+        int d0, d1;
+        bool r2;
+        unit_channels<INTER>(i / 16, a.pairs, d0, d1, r2);
+        const int c = (i & 8 ? d1 : d0) + (i & 7);
+        float sum = 0.f;
+        for (int s = 0; s < slots; ++s) sum += dw[s * 16 * lanes + i];
+        a.partial[((int64_t)blockIdx.x * 2 + k) * a.dim + c] = sum;
+      }
+    }
+  }
+}
+
+// dw[k][c] = the workgroups' shares in order: 16 columns a workgroup, 16 runs of workgroups each
+__global__ __launch_bounds__(256) void rotary_weight_sum_kernel(const float *__restrict__ partial, int groups, int dim, float *dq, float *dk) {
+  __shared__ float part[16][17];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4, width = 2 * dim;
+  const int per = (groups + 15) / 16, g1 = (run + 1) * per < groups ? (run + 1) * per : groups;
+  float sum = 0.f;
+  if (col < width)
+    for (int g = run * per; g < g1; ++g) sum += partial[(int64_t)g * width + col];
+  part[run][threadIdx.x & 15] = sum;
+  __syncthreads();
+  if (run == 0 && col < width) {
+    float t = 0.f;
+    for (int r = 0; r < 16; ++r) t += part[r][threadIdx.x];
+    float *out = col < dim ? dq : dk;
+    if (out) out[col < dim ? col : col - dim] = t;
+  }
+}
+
+constexpr int ROTARY_GRAD_GROUPS = 1024;   // workgroups of a backward launch (4 a CU); their shares are 2 * dim floats each
+
+struct RotaryPlan {
+  bool rows;            // 16 channels a lane (else one wave a row)
+  int lanes, grid;
+  size_t lds;
+};
+
+static int rotary_plan(const mivos_rotary *d, RotaryArgs *a, RotaryPlan *p, bool grad) {
+  const int es = dtype_bytes(d->dtype);
+  uintptr_t bits = 0;
+  for (int k = 0; k < 2; ++k) {
+    const mivos_rotary_rows &r = d->rows[k];
+    a->rows[k] = RotaryRows{r.x, r.g, r.y, r.weight, r.xb, r.xn, r.xh, r.gb, r.gn, r.gh, r.heads};
+    if (!r.heads) continue;
+    bits |= (uintptr_t)r.x | (uintptr_t)r.y | (uintptr_t)((r.xb | r.xn | r.xh) * es);
+    if (grad) bits |= (uintptr_t)r.g | (uintptr_t)((r.gb | r.gn | r.gh) * es);
+  }
+  a->pos = d->positions; a->pb = d->pb; a->pn = d->pn; a->pa = d->pa;
+  a->freq = d->freq; a->axis = d->axis; a->partial = (float *)d->workspace;
+  a->batch = d->batch; a->tokens = d->tokens; a->dim = d->dim; a->pairs = d->pairs; a->interleaved = d->interleaved;
+  a->norm = grad || d->eps >= 0.f; a->eps = d->eps; a->sign = d->inverse ? -1.f : 1.f;
+  const int64_t all = (int64_t)d->batch * d->tokens;
+  p->rows = (bits & 15) == 0 && d->dim % 16 == 0 && d->pairs % 8 == 0 && d->dim <= 512;
+  if (p->rows) {
+    p->lanes = 1;
+    while (p->lanes < d->dim / 16) p->lanes *= 2;
+    int64_t tile = all / 1024;                            // tokens a workgroup: enough workgroups first, then more heads on one table
+    tile = tile < 1 ? 1 : tile > 16 ? 16 : tile;
+    a->tile = (int)tile;
+    a->n_tiles = (int)((all + tile - 1) / tile);
+    p->lds = (size_t)tile * d->pairs * 8;
+    if (grad && p->lds < 256 * 16 * 4) p->lds = 256 * 16 * 4;
+    p->grid = a->n_tiles;
+    if (grad && p->grid > ROTARY_GRAD_GROUPS) p->grid = ROTARY_GRAD_GROUPS;
+    else if (p->grid > (1 << 20)) p->grid = 1 << 20;
+  } else {
+    const int64_t rows = all * (d->rows[0].heads + d->rows[1].heads);
+    const int64_t most = grad ? ROTARY_GRAD_GROUPS : 256 * 64;
+    p->grid = (int)((rows + 3) / 4 < most ? (rows + 3) / 4 : most);
+  }
+  return MIVOS_OK;
+}
+
+static int rotary_check(const mivos_rotary *d, bool grad, const char *what) {
+  if (!d || !dtype_ok(d->dtype) || d->batch < 0 || d->tokens < 0 || d->dim < 2 || d->dim > 512 || d->pairs < 1 || 2 * d->pairs > d->dim || !d->freq || !d->axis)
+    return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: bad shape (rows of 2 to 512 channels, at most half as many pairs)", what);
+  if ((int64_t)d->batch * d->tokens > (1ll << 30)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: too many tokens", what);
+  if ((int64_t)d->batch * d->tokens == 0) return MIVOS_OK;
+  if (!d->positions) return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: null positions", what);
+  for (int k = 0; k < 2; ++k) {
+    const mivos_rotary_rows &r = d->rows[k];
+    if (r.heads < 0 || r.heads > 4096 || (k == 0 && r.heads == 0)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: %d heads", what, r.heads);
+    if (r.heads && (!r.x || !r.y || (grad && !r.g) || ((grad || d->eps >= 0.f) && !r.weight))) return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: null rows", what);
+  }
+  return MIVOS_OK;
+}
+
+template <typename T, bool GRAD>
+static void rotary_launch(const RotaryArgs &a, const RotaryPlan &p, hipStream_t s) {
+  if (!p.rows) { rotary_any_kernel<T, GRAD><<<p.grid, 256, 0, s>>>(a); return; }
+  if constexpr (GRAD) {
+    if (a.interleaved) rotary_rows_kernel<T, true, false, true><<<p.grid, 256, p.lds, s>>>(a, p.lanes);
+    else rotary_rows_kernel<T, false, false, true><<<p.grid, 256, p.lds, s>>>(a, p.lanes);
+  } else if (a.norm) {
+    if (a.interleaved) rotary_rows_kernel<T, true, true, false><<<p.grid, 256, p.lds, s>>>(a, p.lanes);
+    else rotary_rows_kernel<T, false, true, false><<<p.grid, 256, p.lds, s>>>(a, p.lanes);
+  } else {
+    if (a.interleaved) rotary_rows_kernel<T, true, false, false><<<p.grid, 256, p.lds, s>>>(a, p.lanes);
+    else rotary_rows_kernel<T, false, false, false><<<p.grid, 256, p.lds, s>>>(a, p.lanes);
+  }
+}
+
+}  // namespace mivos
+
+using namespace mivos;
+
+extern "C" int mivos_rotary_axes(const mivos_rotary *d, void *stream) {
+  if (int rc = rotary_check(d, false, "rotary_axes")) return rc;
+  if ((int64_t)d->batch * d->tokens == 0) return MIVOS_OK;
+  RotaryArgs a{};
+  RotaryPlan p{};
+  rotary_plan(d, &a, &p, false);
+  hipStream_t s = (hipStream_t)stream;
+  if (d->dtype == MIVOS_F32) rotary_launch<float, false>(a, p, s);
+  else if (d->dtype == MIVOS_F16) rotary_launch<_Float16, false>(a, p, s);
+  else rotary_launch<__bf16, false>(a, p, s);
+  return check_launch("rotary_axes");
+}
+
+extern "C" int64_t mivos_norm_rotary_grad_workspace_bytes(int dim) { return (int64_t)ROTARY_GRAD_GROUPS * 2 * dim * 4; }
+
+extern "C" int mivos_norm_rotary_grad(const mivos_rotary *d, float *dq_weight, float *dk_weight, void *stream) {
+  if (int rc = rotary_check(d, true, "norm_rotary_grad")) return rc;
+  if (d->eps < 0.f || !dq_weight || (d->rows[1].heads && !dk_weight)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "norm_rotary_grad: bad argument");
+  hipStream_t s = (hipStream_t)stream;
+  RotaryArgs a{};
+  RotaryPlan p{};
+  if ((int64_t)d->batch * d->tokens) {
+    if (!d->workspace || d->workspace_bytes < mivos_norm_rotary_grad_workspace_bytes(d->dim)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "norm_rotary_grad: workspace");
+    rotary_plan(d, &a, &p, true);
+    if (d->dtype == MIVOS_F32) rotary_launch<float, true>(a, p, s);
+    else if (d->dtype == MIVOS_F16) rotary_launch<_Float16, true>(a, p, s);
+    else rotary_launch<__bf16, true>(a, p, s);
+  }
+  rotary_weight_sum_kernel<<<cdiv(2 * d->dim, 16), 256, 0, s>>>(a.partial, p.grid, d->dim, dq_weight, dk_weight);
+  return check_launch("norm_rotary_grad");
+}

@@ -11,7 +11,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import ConvDesc, FusionNetDesc, InterleaveDesc, MivosHipError, check
+from ._lib import Bank4Desc, ConvDesc, FusionNetDesc, InterleaveDesc, MivosHipError, RotaryDesc, check
 
 _checked_devices = set()
 # "f16x3": error-compensated fp16 MFMA convolutions (3 products per term, fp32-class accuracy, 5.3x the
@@ -1041,3 +1041,311 @@ def interleave(planes, n, p, c_out, device):
     out = torch.empty((n, p, c_out), dtype=torch.float32, device=device)
     check(_lib.load().mivos_interleave_planes(C.byref(d), out.data_ptr(), n, p, _stream()))
     return out
+
+
+# ---- token memory: rotary positions over several axes, norm + rotary of queries and keys, a memory bank in 4 bits ----
+# The operators of a transformer over video tokens beside the space-time memory above: tokens have a (time, height, width) position, the
+# bank keeps keys and values in 4 bits, `bank4_read` is its attention, `bank4_evict` brings it back to a budget.  fp32, fp16 and bf16
+# operands; no autograd graph is recorded, the gradients are calls of their own (as with the fusion training operators above).
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # mivos_dtype
+
+
+def _same_device(ref, *tensors):
+    for t in tensors:
+        if t is not None and t.device != ref.device:
+            raise MivosHipError(f"operands live on {ref.device} and {t.device}")
+
+
+def _dtype_code(t):
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise MivosHipError(f"expected float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _head_rows(t, name, shape=None):
+    """[B, N, heads, channels] with dense channels (any other strides); checks the shape."""
+    if t.dim() != 4 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise MivosHipError(f"{name}: expected {'[batch, tokens, heads, channels]' if shape is None else list(shape)}, got {list(t.shape)}")
+    if t.stride(3) != 1 and t.shape[3] > 1 and t.numel():
+        raise MivosHipError(f"{name}: the channel stride must be 1")
+    return t
+
+
+def _int32_vector(t, n, name):
+    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise MivosHipError(f"{name}: expected a dense int32 [{n}] tensor, got {t.dtype} {list(t.shape)}")
+    return t
+
+
+class RotaryAxes:
+    """Plan of a rotary position with several axes: `sections[a]` channel pairs turn with axis a (time, height, width, ...), the channels
+    behind the pairs are not turned.  Pair j of a section of n has the frequency base^(-j / n); shared=True: one ladder over all pairs,
+    base^(-i / sum(sections)).  interleaved=True pairs neighbouring channels, else channel i goes with i + sum(sections).  The device
+    table keeps every frequency as a 64-bit fraction of a turn, so angles are exact for every int32 position."""
+    __slots__ = ("head_dim", "sections", "pairs", "interleaved", "freq", "axis")
+
+    def __init__(self, head_dim, sections, base=10000.0, shared=False, interleaved=False, device="cuda"):
+        import decimal
+        sections = tuple(int(n) for n in sections)
+        pairs = sum(sections)
+        if not sections or min(sections) < 0 or pairs < 1 or 2 * pairs > head_dim or head_dim > 512:
+            raise MivosHipError(f"RotaryAxes: sections {sections} (channel pairs an axis) do not fit heads of {head_dim} channels (at most 512)")
+        if not 0 < base < float("inf"):
+            raise MivosHipError(f"RotaryAxes: base {base}")
+        self.head_dim, self.sections, self.pairs, self.interleaved = int(head_dim), sections, pairs, bool(interleaved)
+        with decimal.localcontext() as ctx:
+            ctx.prec = 60
+            D = decimal.Decimal
+            two_pi = 2 * D("3.14159265358979323846264338327950288419716939937510582097494459")
+            steps = [(D(i) / pairs if shared else D(j) / n, a) for i, (a, n, j) in enumerate((a, n, j) for a, n in enumerate(sections) for j in range(n))]
+            turns = [int((D(float(base)) ** -e / two_pi * 2 ** 64).to_integral_value()) % 2 ** 64 for e, _ in steps]
+        self.freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
+        self.axis = torch.tensor([a for _, a in steps], dtype=torch.int32, device=device)
+        if self.freq.is_cuda:
+            with torch.cuda.device(self.freq.device):
+                publish_constants()
+
+
+def _rotary_desc(q, k, positions, plan, inverse, eps):
+    _head_rows(q, "q")
+    b, n, _, d = q.shape
+    if d != plan.head_dim:
+        raise MivosHipError(f"q has heads of {d} channels, the plan {plan.head_dim}")
+    if k is not None:
+        _head_rows(k, "k", (b, n, k.shape[2] if k.dim() == 4 else -1, d))
+        if k.dtype != q.dtype:
+            raise MivosHipError(f"q is {q.dtype}, k is {k.dtype}")
+    if positions.dtype != torch.int32 or tuple(positions.shape) != (b, n, len(plan.sections)):
+        raise MivosHipError(f"positions: expected int32 {[b, n, len(plan.sections)]}, got {positions.dtype} {list(positions.shape)}")
+    code = _dtype_code(q)
+    _same_device(q, k, positions, plan.freq)
+    _ensure_device(q)
+    desc = RotaryDesc()
+    desc.positions, desc.freq, desc.axis = positions.data_ptr(), plan.freq.data_ptr(), plan.axis.data_ptr()
+    desc.pb, desc.pn, desc.pa = positions.stride()
+    desc.batch, desc.tokens, desc.dim, desc.pairs = b, n, d, plan.pairs
+    desc.dtype, desc.interleaved, desc.inverse, desc.eps = code, plan.interleaved, inverse, eps
+    return desc
+
+
+def _rotary_rows(row, x, g=None, weight=None):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    row.x, row.y, row.heads = x.data_ptr(), y.data_ptr(), x.shape[2]
+    row.xb, row.xn, row.xh = x.stride()[:3]
+    if g is not None:
+        row.g = g.data_ptr()
+        row.gb, row.gn, row.gh = g.stride()[:3]
+    if weight is not None:
+        row.weight = weight.data_ptr()
+    return y
+
+
+def _norm_weight(w, ref, name):
+    if w is None or w.dtype != torch.float32 or tuple(w.shape) != (ref.shape[3],) or not w.is_contiguous():
+        raise MivosHipError(f"{name}: expected a dense float32 [{ref.shape[3]}] tensor")
+    _same_device(ref, w)
+    return w
+
+
+def _rotary(q, k, positions, plan, inverse, eps, q_weight=None, k_weight=None):
+    desc = _rotary_desc(q, k, positions, plan, inverse, eps)
+    yq = _rotary_rows(desc.rows[0], q, None, q_weight)
+    yk = None if k is None else _rotary_rows(desc.rows[1], k, None, k_weight)
+    check(_lib.load().mivos_rotary_axes(desc, _stream()))
+    return yq, yk
+
+
+def rotary_axes(q, k, positions, plan):
+    """q [B, N, Hq, D], k [B, N, Hk, D] or None (dense channels, other strides free: slices of a joint projection are fine), positions int32
+    [B, N, axes] -> (q, k) turned by their positions (RotaryAxes), dense, in the input's type."""
+    return _rotary(q, k, positions, plan, 0, -1.0)
+
+
+def rotary_axes_grad(dq, dk, positions, plan):
+    """Gradients of `rotary_axes`: the turn by minus the angle."""
+    return _rotary(dq, dk, positions, plan, 1, -1.0)
+
+
+def norm_rotary(q, k, q_weight, k_weight, positions, plan, eps=1e-6):
+    """The norm of every head's query / key, x / sqrt(mean(x^2) + eps) * weight (fp32 [D], shared by the heads), and `rotary_axes`, in one
+    pass over the rows (fp32 inside, one rounding at the end)."""
+    if not eps >= 0:
+        raise MivosHipError(f"norm_rotary: eps {eps}")
+    _norm_weight(q_weight, _head_rows(q, "q"), "q_weight")
+    if k is not None:
+        _norm_weight(k_weight, _head_rows(k, "k"), "k_weight")
+    return _rotary(q, k, positions, plan, 0, float(eps), q_weight, k_weight)
+
+
+def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, plan, eps=1e-6):
+    """dq, dk: gradients of norm_rotary's outputs; q, k: its inputs -> (gradient of q, of k, of q_weight, of k_weight); the weights'
+    gradients are fp32 sums over all tokens and heads in a fixed order."""
+    if not eps >= 0:
+        raise MivosHipError(f"norm_rotary_grad: eps {eps}")
+    _norm_weight(q_weight, _head_rows(q, "q"), "q_weight")
+    _head_rows(dq, "dq", q.shape)
+    if (dk is None) != (k is None):
+        raise MivosHipError("norm_rotary_grad: dk goes with k")
+    if k is not None:
+        _norm_weight(k_weight, _head_rows(k, "k"), "k_weight")
+        _head_rows(dk, "dk", k.shape)
+    for g in (dq, dk):
+        if g is not None and g.dtype != q.dtype:
+            raise MivosHipError(f"q is {q.dtype}, its gradient {g.dtype}")
+    desc = _rotary_desc(q, k, positions, plan, 1, float(eps))
+    _same_device(q, dq, dk)
+    lib = _lib.load()
+    ws = torch.empty(lib.mivos_norm_rotary_grad_workspace_bytes(q.shape[3]), dtype=torch.uint8, device=q.device)
+    desc.workspace, desc.workspace_bytes = ws.data_ptr(), ws.numel()
+    gq = _rotary_rows(desc.rows[0], q, dq, q_weight)
+    gk = None if k is None else _rotary_rows(desc.rows[1], k, dk, k_weight)
+    wq = torch.empty_like(q_weight)
+    wk = None if k is None else torch.empty_like(k_weight)
+    check(lib.mivos_norm_rotary_grad(desc, wq.data_ptr(), None if wk is None else wk.data_ptr(), _stream()))
+    return gq, gk, wq, wk
+
+
+class Bank4:
+    """A memory bank in 4 bits: per (stream, head, slot) a key row and a value row of blocks of 32 channels, one power-of-two scale a block
+    (`mivos_bank4` in include/mivos_hip.h has the format: 17 bytes for 32 channels), the attention weight the slot has received, and the
+    streams' lengths.  `Bank4.empty` allocates one; the constructor takes the buffers of one (dense tensors, any of which the program may
+    keep and read): codes uint8 [B, H, S, D / 2], scales uint8 [B, H, S, D / 32], weight fp32 [B, H, S], lens int32 [B].  Calls on one bank
+    belong to one stream at a time."""
+    __slots__ = ("key_codes", "key_scales", "value_codes", "value_scales", "weight", "lens", "status", "batch", "heads", "slots", "key_dim",
+                 "value_dim", "_desc", "_storages")
+
+    def __init__(self, key_codes, key_scales, value_codes, value_scales, weight, lens):
+        if key_codes.dim() != 4 or value_codes.dim() != 4:
+            raise MivosHipError("Bank4: codes are [batch, heads, slots, channels / 2]")
+        b, h, s, _ = key_codes.shape
+        dk, dv = 2 * key_codes.shape[3], 2 * value_codes.shape[3]
+        for name, d in (("key", dk), ("value", dv)):
+            if d < 32 or d > 1024 or d % 32:
+                raise MivosHipError(f"Bank4: {name} rows of {d} channels (a multiple of 32, at most 1024)")
+        if not (1 <= b * h <= 65535 and 1 <= s <= 1 << 30):
+            raise MivosHipError(f"Bank4: {b} streams x {h} heads x {s} slots")
+        for t, shape, dtype in ((key_codes, (b, h, s, dk // 2), torch.uint8), (key_scales, (b, h, s, dk // 32), torch.uint8),
+                                (value_codes, (b, h, s, dv // 2), torch.uint8), (value_scales, (b, h, s, dv // 32), torch.uint8),
+                                (weight, (b, h, s), torch.float32), (lens, (b,), torch.int32)):
+            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+                raise MivosHipError(f"Bank4: expected a dense {dtype} {list(shape)} buffer, got {t.dtype} {list(t.shape)}")
+            if dtype == torch.uint8 and t.data_ptr() % 16:
+                raise MivosHipError("Bank4: codes and scales must be 16-byte aligned")
+        _same_device(key_codes, key_scales, value_codes, value_scales, weight, lens)
+        self.key_codes, self.key_scales, self.value_codes, self.value_scales, self.weight, self.lens = key_codes, key_scales, value_codes, value_scales, weight, lens
+        self.batch, self.heads, self.slots, self.key_dim, self.value_dim = b, h, s, dk, dv
+        self.status = torch.zeros(1 + b, dtype=torch.int32, device=lens.device)
+        buffers = (key_codes, key_scales, value_codes, value_scales, weight, lens, self.status)
+        self._desc = Bank4Desc(*(t.data_ptr() for t in buffers), s, b, h, dk, dv)
+        self._storages = frozenset(t.untyped_storage().data_ptr() for t in buffers)
+        if len(self._storages) != len(buffers):
+            raise MivosHipError("Bank4: the buffers share memory")
+
+    @classmethod
+    def empty(cls, batch, heads, slots, key_dim, value_dim, device="cuda"):
+        """An empty bank (lens = 0)."""
+        if min(batch, heads, slots) < 1 or key_dim % 32 or value_dim % 32:
+            raise MivosHipError(f"Bank4: {batch} streams x {heads} heads x {slots} slots of {key_dim} / {value_dim} channels")
+        u8 = lambda n: torch.empty((batch, heads, slots, n), dtype=torch.uint8, device=device)  # noqa: E731
+        return cls(u8(key_dim // 2), u8(key_dim // 32), u8(value_dim // 2), u8(value_dim // 32),
+                   torch.zeros((batch, heads, slots), dtype=torch.float32, device=device), torch.zeros(batch, dtype=torch.int32, device=device))
+
+    def check_room(self):
+        """Raise MivosHipError if tokens were dropped because their slot lay outside the bank since the last check (waits for the GPU)."""
+        if int(self.status[0].item()):
+            self.status[0].zero_()
+            raise MivosHipError(f"Bank4: appended tokens did not fit the {self.slots} slots")
+
+
+def _overlap(a, b):
+    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
+def bank4_append(bank, keys, values, at=None, count=None):
+    """keys [B, T, H, Dk], values [B, T, H, Dv] (one type; dense channels) quantised into slots [at[b], at[b] + count[b]) of the bank (at None:
+    behind what is there; count None: all T); their weight becomes 0 and bank.lens[b] = at[b] + count[b].  Tokens beyond the bank's last slot
+    are dropped and remembered (Bank4.check_room)."""
+    _head_rows(keys, "keys", (bank.batch, keys.shape[1] if keys.dim() == 4 else -1, bank.heads, bank.key_dim))
+    _head_rows(values, "values", (bank.batch, keys.shape[1], bank.heads, bank.value_dim))
+    if keys.dtype != values.dtype:
+        raise MivosHipError(f"keys are {keys.dtype}, values {values.dtype}")
+    code = _dtype_code(keys)
+    if at is None:
+        at = bank.lens
+    else:
+        _int32_vector(at, bank.batch, "at")
+        if at.data_ptr() != bank.lens.data_ptr() and _overlap(at, bank.lens):
+            raise MivosHipError("at overlaps the bank's lengths")
+    if count is not None and _overlap(_int32_vector(count, bank.batch, "count"), bank.lens):
+        raise MivosHipError("count overlaps the bank's lengths")
+    _same_device(bank.lens, keys, values, at, count)
+    _ensure_device(keys)
+    ks, vs = keys.stride(), values.stride()
+    check(_lib.load().mivos_bank4_append(bank._desc, keys.data_ptr(), ks[0], ks[1], ks[2], values.data_ptr(), vs[0], vs[1], vs[2], code, at.data_ptr(),
+                                         None if count is None else count.data_ptr(), keys.shape[1], _stream()))
+
+
+def bank4_values(bank, first=None, count=None, dtype=torch.bfloat16):
+    """What slots [first[b], first[b] + count) of every stream (first None: 0; count None: all slots) stand for -> keys [B, H, count, Dk], values
+    [B, H, count, Dv], bf16 or fp32 (both exact: e.g. for `memory_read`, which takes fp32 rows); 0 behind a stream's length."""
+    count = bank.slots if count is None else int(count)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise MivosHipError(f"bank4_values: float32 or bfloat16, got {dtype}")
+    if not 0 <= count <= bank.slots:
+        raise MivosHipError(f"bank4_values: {count} of {bank.slots} slots")
+    if first is not None:
+        _int32_vector(first, bank.batch, "first")
+    _same_device(bank.lens, first)
+    _ensure_device(bank.lens)
+    keys = torch.empty((bank.batch, bank.heads, count, bank.key_dim), dtype=dtype, device=bank.lens.device)
+    values = torch.empty((bank.batch, bank.heads, count, bank.value_dim), dtype=dtype, device=bank.lens.device)
+    check(_lib.load().mivos_bank4_values(bank._desc, None if first is None else first.data_ptr(), count, keys.data_ptr(), values.data_ptr(), _DTYPES[dtype],
+                                         _stream()))
+    return keys, values
+
+
+def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False):
+    """queries [B, T, Hq, Dk], Hq a multiple of the bank's heads -> [B, T, Hq, Dv] in the queries' type: softmax attention of every token over
+    the stream's filled slots (scale None: Dk^-0.5).  causal=True: the T tokens are the newest of the bank (appended before), token t sees the
+    slots up to its own.  count int32 [B]: valid tokens of a padded batch; the others, and tokens that see no slot, give 0.  weigh=True also
+    adds the softmax weights every slot receives from the stream's tokens and its head's queries to bank.weight, for bank4_evict."""
+    _head_rows(queries, "queries", (bank.batch, queries.shape[1] if queries.dim() == 4 else -1, queries.shape[2] if queries.dim() == 4 else -1, bank.key_dim))
+    b, t, hq, d = queries.shape
+    if hq < 1 or hq % bank.heads:
+        raise MivosHipError(f"{hq} query heads over {bank.heads} bank heads")
+    code = _dtype_code(queries)
+    if count is not None:
+        _int32_vector(count, b, "count")
+    _same_device(bank.lens, queries, count)
+    lib = _lib.load()
+    need = lib.mivos_bank4_read_workspace_bytes(bank._desc, hq, t, weigh)
+    if need < 0:
+        check(int(need))
+    _ensure_device(queries)
+    out = torch.empty((b, t, hq, bank.value_dim), dtype=queries.dtype, device=queries.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=queries.device) if need else None
+    qs = queries.stride()
+    check(lib.mivos_bank4_read(bank._desc, queries.data_ptr(), qs[0], qs[1], qs[2], code, hq, t, None if count is None else count.data_ptr(),
+                               d ** -0.5 if scale is None else float(scale), causal, weigh, out.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                               _stream()))
+    return out
+
+
+def bank4_evict(bank, keep, out, first=0, recent=0):
+    """Brings every stream down to `keep` slots: the first `first` (the frames a user marked), the last `recent`, and of the others those with
+    the largest bank.weight (equal: the lowest slots), in their order, moved into bank `out` (same streams, heads and channels, at least `keep`
+    slots, other memory) with their weights; out.lens = min(bank.lens, keep), rows of `out` behind that stay as they were.  Returns the slots
+    they came from, int32 [B, H, keep] (-1 behind out.lens).  Two banks used in turn keep a stream within its budget."""
+    if (out.batch, out.heads, out.key_dim, out.value_dim) != (bank.batch, bank.heads, bank.key_dim, bank.value_dim):
+        raise MivosHipError("bank4_evict: the two banks differ in streams, heads or channels")
+    if bank._storages & out._storages:
+        raise MivosHipError("bank4_evict: the two banks share memory")
+    if not 1 <= keep <= out.slots or first < 0 or recent < 0 or first + recent > keep:
+        raise MivosHipError(f"bank4_evict: keep {keep} of {out.slots} slots, first {first}, recent {recent}")
+    _same_device(bank.lens, out.lens)
+    _ensure_device(bank.lens)
+    slots = torch.empty((bank.batch, bank.heads, keep), dtype=torch.int32, device=bank.lens.device)
+    check(_lib.load().mivos_bank4_evict(bank._desc, out._desc, keep, first, recent, slots.data_ptr(), _stream()))
+    return slots
