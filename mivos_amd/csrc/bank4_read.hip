@@ -16,6 +16,7 @@
 namespace mivos {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int BLOCK_ROWS_MIN = 65;   // rows a bank head from which the 128-row kernel runs
 
 struct ReadArgs {
   const uint8_t *kc, *ks, *vc, *vs;
@@ -24,10 +25,11 @@ struct ReadArgs {
   const void *q;
   void *out;
   int64_t qb, qt, qh;
-  float *part_o, *part_ml, *logits;
+  float *part_o, *part_ml, *logits, *lse;
   int64_t slots, logit_stride;
   int batch, heads, group, tokens, rows, value_dim, nsplit, causal, weigh, q_vec;
-  float scale_log2;       // scale * log2(e): the softmax runs in powers of two
+  float scale_log2;       // scale * log2(e): the softmax runs in powers of two; bank4_block / weigh: |scale|, its sign goes to the queries
+  float q_sign;
 };
 
 __device__ __forceinline__ int64_t read_len(const ReadArgs &a, int b) {
@@ -111,18 +113,44 @@ __global__ __launch_bounds__(256) void bank4_rows_kernel(ReadArgs a) {
   __bf16 *vt = reinterpret_cast<__bf16 *>(lds) + wave * 32 * VPAD;
   const int vs_row = a.value_dim / 32;
 
+  // a step's codes and scales, fetched a step ahead: 64 slots x (DK + DVC) / 2 bytes a wave stay in flight while the last step is computed
+  struct Step {
+    uint32_t kc[4][KSTEPS], ks[4][(KSTEPS + 7) / 8];
+    u32x4 vc[DVC / 32];
+    uint32_t vs[DVC / 32];
+  } now, next;
+  auto fetch = [&](Step &f, int64_t base) {
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      const int64_t slot = base + kt * 16 + col, row = row_base + (slot < a.slots ? slot : a.slots - 1);
+      const uint8_t *codes = a.kc + row * (DK / 2) + grp * (CPL / 2), *sc = a.ks + row * (DK / 32) + grp * CPL / 32;
+      if constexpr (KSTEPS == 2) *reinterpret_cast<u32x2 *>(f.kc[kt]) = *reinterpret_cast<const u32x2 *>(codes);
+      else
+#pragma unroll
+        for (int i = 0; i < KSTEPS / 4; ++i) *reinterpret_cast<u32x4 *>(f.kc[kt] + 4 * i) = reinterpret_cast<const u32x4 *>(codes)[i];
+#pragma unroll
+      for (int i = 0; i < (KSTEPS + 7) / 8; ++i) f.ks[kt][i] = KSTEPS == 8 ? *reinterpret_cast<const uint16_t *>(sc) : sc[i];
+    }
+#pragma unroll
+    for (int i = 0; i < DVC / 32; ++i) {       // 64 rows x DVC / 32 blocks of 16 bytes over 64 lanes
+      const int e = i * 64 + lane;
+      const int64_t slot = base + e / (DVC / 32), row = row_base + (slot < a.slots ? slot : a.slots - 1);
+      f.vc[i] = *reinterpret_cast<const u32x4 *>(a.vc + row * (a.value_dim / 2) + chunk * (DVC / 2) + e % (DVC / 32) * 16);
+      f.vs[i] = a.vs[row * vs_row + chunk * (DVC / 32) + e % (DVC / 32)];
+    }
+  };
+  if (s0 + wave * 64 < s1) fetch(next, s0 + wave * 64);
   for (int64_t base = s0 + wave * 64; base < s1; base += 256) {
+    now = next;
+    if (base + 256 < s1) fetch(next, base + 256);
     // ---- logits of 64 slots
     f32x4 x[4];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      const int64_t slot = base + kt * 16 + col, row = row_base + (slot < a.slots ? slot : a.slots - 1);
-      const uint32_t *codes = reinterpret_cast<const uint32_t *>(a.kc + row * (DK / 2) + grp * (CPL / 2));
-      const uint8_t *sc = a.ks + row * (DK / 32) + grp * CPL / 32;
       x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KSTEPS; ++i) {
-        const bf16x8 kf = bank4_unpack8(codes[i], bank4_scale(sc[i * 8 / 32]));
+        const bf16x8 kf = bank4_unpack8(now.kc[kt][i], bank4_scale(KSTEPS == 8 ? (now.ks[kt][0] >> (i / 4 * 8)) & 255 : now.ks[kt][0]));
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][p], x[kt], 0, 0, 0);
       }
@@ -159,12 +187,11 @@ __global__ __launch_bounds__(256) void bank4_rows_kernel(ReadArgs a) {
       split8<PARTS>(p, pf);
       wave_lds_fence();
 #pragma unroll
-      for (int i = 0; i < DVC / 64; ++i) {       // 32 rows x DVC / 32 blocks of 16 bytes over 64 lanes
+      for (int i = 0; i < DVC / 64; ++i) {
         const int e = i * 64 + lane, vr = e / (DVC / 32), blk = e % (DVC / 32);
-        const int64_t slot = base + half * 32 + vr, row = row_base + (slot < a.slots ? slot : a.slots - 1);
-        u32x4 codes = *reinterpret_cast<const u32x4 *>(a.vc + row * (a.value_dim / 2) + chunk * (DVC / 2) + blk * 16);
-        uint32_t byte = a.vs[row * vs_row + chunk * (DVC / 32) + blk];
-        if (slot >= s1) { codes = u32x4{0u, 0u, 0u, 0u}; byte = 127; }      // never-written memory may stand for NaN
+        u32x4 codes = now.vc[half * (DVC / 64) + i];
+        uint32_t byte = now.vs[half * (DVC / 64) + i];
+        if (base + half * 32 + vr >= s1) { codes = u32x4{0u, 0u, 0u, 0u}; byte = 127; }      // never-written memory may stand for NaN
         const float sc = bank4_scale(byte);
 #pragma unroll
         for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(vt + vr * VPAD + blk * 32 + j * 8) = bank4_unpack8(codes[j], sc);
@@ -214,72 +241,466 @@ __global__ __launch_bounds__(256) void bank4_rows_kernel(ReadArgs a) {
   }
 }
 
-// Joins the slices of a row (first `out_blocks` workgroups, one wave a row) and adds the rows' weights to the slots (the others,
-// 1024 slots each, the rows in order: the sum does not depend on timing).
-template <int PARTS>
+// ------------------------------------------------------------------------------------------ many rows: 128 a workgroup
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// K rows of a tile in a lane's registers: 32x32 products take row l % 32, channels i * 64 + (l / 32) * 32 .. + 31 of it.
+template <int DK>
+struct KeyRow {
+  static constexpr int KI = DK / 64;
+  u32x4 codes[KI];
+  uint32_t scales[(KI + 1) / 2];        // byte 2 (i % 2) of word i / 2: the scale of the lane's block i
+  __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *ks, int64_t row, int half) {
+#pragma unroll
+    for (int i = 0; i < KI; ++i) codes[i] = *reinterpret_cast<const u32x4 *>(kc + row * (DK / 2) + i * 32 + half * 16);
+    if constexpr (KI == 1) scales[0] = ks[row * 2 + half];
+    else
+#pragma unroll
+      for (int i = 0; i < KI / 2; ++i) scales[i] = reinterpret_cast<const uint32_t *>(ks + row * (DK / 32))[i] >> (8 * half);
+  }
+  __device__ __forceinline__ float scale(int i) const { return bank4_scale((scales[i / 2] >> (16 * (i & 1))) & 255); }
+};
+
+// Queries of a lane (column l % 32).  bf16 queries are held as two 8-bit floats a channel, each with a power-of-two scale a block of 32
+// channels - high four bits and the rest: the 8 bits of a bf16 number, exact down to 2^-22 of the block's largest - and multiply the
+// bank's codes and scales as they are (the block-scaled product takes 4-bit codes beside 8-bit floats).  fp16 and fp32 queries are 2 / 3 bf16 numbers and
+// multiply widened keys.
+template <int DK, int PARTS>
+struct QueryCols {
+  bf16x8 f[DK / 16][PARTS];
+  template <typename T>
+  __device__ __forceinline__ void load(const T *row, int half, bool live, bool vec, float sign) {
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        f32x8 x = load8(row + i * 64 + half * 32 + u * 8, vec);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = live ? x[j] * sign : 0.f;
+        split8<PARTS>(x, f[i * 4 + u]);
+      }
+  }
+  __device__ __forceinline__ f32x16 dot(const KeyRow<DK> &k) const {       // [32 keys][32 queries]
+    f32x16 c;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) {
+      const float sc = k.scale(i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bf16x8 kf = bank4_unpack8(k.codes[i][u], sc);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, f[i * 4 + u][p], c, 0, 0, 0);
+      }
+    }
+    return c;
+  }
+};
+
+template <int DK>
+struct QueryCols<DK, 1> {
+  i32x8 hi[DK / 64], lo[DK / 64];
+  int scale[DK / 64];                   // byte 0 / 1: the scale of hi / lo of block i * 64 + half * 32
+  __device__ __forceinline__ void load(const __bf16 *row, int half, bool live, bool vec, float sign) {
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) {
+      // an 8-bit operand's lane holds channels half * 16 .. + 15 of both blocks of the 64
+      float x[2][16], top[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const f32x8 x0 = load8(row + i * 64 + b * 32 + half * 16, vec), x1 = load8(row + i * 64 + b * 32 + half * 16 + 8, vec);
+        top[b] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          x[b][j] = live ? (j < 8 ? x0[j & 7] : x1[j & 7]) * sign : 0.f;
+          const float m = __builtin_fabsf(x[b][j]);
+          top[b] = m < INFINITY ? fmaxf(top[b], m) : INFINITY;
+        }
+        top[b] = fmaxf(top[b], __shfl_xor(top[b], 32));
+      }
+      int e[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {     // the block's largest in [128, 256); an infinity or NaN makes the block NaN
+        e[b] = (int)(__float_as_uint(top[b]) >> 23) - 127 - 7;
+        e[b] = e[b] < -110 ? -110 : e[b];
+        const float down = top[b] < INFINITY ? __uint_as_float((uint32_t)(127 - e[b]) << 23) : NAN;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          int h = 0, l = 0;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float y0 = x[b][w * 4 + j * 2] * down, y1 = x[b][w * 4 + j * 2 + 1] * down;
+            const int pair = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
+            const float r0 = (y0 - __builtin_amdgcn_cvt_f32_fp8(pair, 0)) * 32.f, r1 = (y1 - __builtin_amdgcn_cvt_f32_fp8(pair, 1)) * 32.f;
+            h |= (pair & 0xffff) << (16 * j);
+            l |= (__builtin_amdgcn_cvt_pk_fp8_f32(r0, r1, 0, false) & 0xffff) << (16 * j);
+          }
+          hi[i][b * 4 + w] = h;
+          lo[i][b * 4 + w] = l;
+        }
+      }
+      const int mine = 127 + (half ? e[1] : e[0]);
+      scale[i] = mine | (mine - 5) << 8;
+    }
+  }
+  __device__ __forceinline__ f32x16 dot(const KeyRow<DK> &k) const {
+    f32x16 c;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) {
+      const i32x8 kf = {(int)k.codes[i].x, (int)k.codes[i].y, (int)k.codes[i].z, (int)k.codes[i].w, 0, 0, 0, 0};
+      const int ks = (int)k.scales[i / 2];
+      if (i & 1) {
+        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, hi[i], c, 4, 0, 2, ks, 0, scale[i]);
+        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, lo[i], c, 4, 0, 2, ks, 1, scale[i]);
+      } else {
+        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, hi[i], c, 4, 0, 0, ks, 0, scale[i]);
+        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, lo[i], c, 4, 0, 0, ks, 1, scale[i]);
+      }
+    }
+    return c;
+  }
+};
+
+// One workgroup: 128 rows (32 a wave) x one slice of the slots x DVC value channels, 64 slots a step.  Every wave reads the step's K
+// codes straight into registers; the V rows are widened once for the workgroup into one of two LDS buffers while the matrix cores work on
+// the other.  S^T = K Q^T and O^T = V^T P^T on 32x32 products: a lane holds one query, 16 keys of each 32, and these are again the
+// operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^8.
+template <int DK, int DVC, int PARTS>
+__global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1) void bank4_block_kernel(ReadArgs a) {
+  typedef typename ReadType<PARTS>::T T;
+  constexpr int VS = DVC + 32, NT = DVC / 32, VE = 64 * DVC / 32, VL = (VE + 255) / 256;
+  __shared__ __align__(16) __bf16 vt[2][64 * VS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
+  const int split = blockIdx.x, row0 = blockIdx.y * 128, r = row0 + wave * 32 + col;
+  const int64_t len = read_len(a, b);
+  const int cnt = read_count(a, b), t = r / a.group;
+  const bool live = r < a.rows && t < cnt;
+  const int limit = live ? (int)read_limit(a, len, cnt, t) : (int)len;
+  int last_t = (row0 + 127 < a.rows ? row0 + 127 : a.rows - 1) / a.group;
+  last_t = last_t < cnt ? last_t : cnt - 1;
+  const int seen = row0 / a.group < cnt ? (int)read_limit(a, len, cnt, last_t) : 0;
+  const int per = ((seen + 63) / 64 + a.nsplit - 1) / a.nsplit * 64;
+  const int s0 = (int64_t)split * per < seen ? split * per : seen, s1 = seen - s0 < per ? seen : s0 + per;
+  int low = limit, high = live ? limit : 0;          // over the wave's rows
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_xor(low, d), y = __shfl_xor(high, d);
+    low = x < low ? x : low;
+    high = y > high ? y : high;
+  }
+  low = __builtin_amdgcn_readfirstlane(low);
+  high = __builtin_amdgcn_readfirstlane(high);
+
+  QueryCols<DK, PARTS> q;
+  q.load((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign);
+  f32x16 o[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const int64_t row_base = (int64_t)bh * a.slots;
+  const int last = (int)a.slots - 1;
+  KeyRow<DK> k[2], kn[2];
+  u32x4 vc[VL];
+  uint32_t vs[VL];
+
+  auto load_keys = [&](KeyRow<DK> *to, int base) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int slot = base + s * 32 + col;
+      to[s].load(a.kc, a.ks, row_base + (slot < last ? slot : last), half);
+    }
+  };
+  auto load_values = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int e = i * 256 + tid, slot = base + e / (DVC / 32), blk = e % (DVC / 32);
+      if (VE < 256 && e >= VE) break;
+      const int64_t row = row_base + (slot < last ? slot : last);
+      vc[i] = *reinterpret_cast<const u32x4 *>(a.vc + row * (a.value_dim / 2) + chunk * (DVC / 2) + blk * 16);
+      vs[i] = a.vs[row * (a.value_dim / 32) + chunk * (DVC / 32) + blk];
+      if (slot >= s1) { vc[i] = u32x4{0u, 0u, 0u, 0u}; vs[i] = 127; }      // never-written memory may stand for NaN
+    }
+  };
+  auto store_values = [&](__bf16 *to) {
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int e = i * 256 + tid, vr = e / (DVC / 32), blk = e % (DVC / 32);
+      if (VE < 256 && e >= VE) break;
+      const float sc = bank4_scale(vs[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(to + vr * VS + blk * 32 + j * 8) = bank4_unpack8(vc[i][j], sc);
+    }
+  };
+
+  if (s0 < s1) {
+    load_keys(k, s0);
+    load_values(s0);
+    store_values(vt[0]);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int base = s0; base < s1; base += 64, buf ^= 1) {
+    const bool more = base + 64 < s1;
+    if (more) {
+      load_keys(kn, base + 64);
+      load_values(base + 64);
+    }
+    if (base < high) {
+      f32x16 x[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) x[s] = q.dot(k[s]);
+      if (base + 64 > low || base + 64 > s1) {
+        const int lim = limit < s1 ? limit : s1;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[s][j] = base + s * 32 + mfma32_row(j, lane) < lim ? x[s][j] : -INFINITY;
+      }
+      float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+      for (int j = 1; j < 16; ++j) top = fmaxf(fmaxf(top, x[0][j]), x[1][j]);
+      top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+      if (__any(top > m + 8.f)) {
+        const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[i] *= alpha;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {           // 16 slots: keys 16 s + {0..3, 8..11} + 4 half
+        f32x8 p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], a.scale_log2, -mu));
+          l += p[j];
+        }
+        bf16x8 pf[PARTS];
+        split8<PARTS>(p, pf);
+        const __bf16 *at = vt[buf] + (s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          typedef __attribute__((address_space(3))) s16x4 *lds_p;
+          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + i * 32));
+          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + i * 32 + 8 * VS));
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int w = 0; w < PARTS; ++w) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[w], o[i], 0, 0, 0);
+        }
+      }
+    }
+    if (more) {
+      store_values(vt[buf ^ 1]);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) k[s] = kn[s];
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32);
+  if (r >= a.rows) return;
+  if (a.part_o) {
+    const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + r;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4 *>(a.part_o + at * a.value_dim + chunk * DVC + i * 32 + j * 8 + half * 4) =
+            f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+    if (half == 0 && chunk == 0) { a.part_ml[at * 2] = live ? m : -INFINITY; a.part_ml[at * 2 + 1] = live ? l : 0.f; }
+  } else {
+    const float inv = live && l != 0.f ? 1.f / l : 0.f;
+    T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + h * a.group + r - t * a.group) * a.value_dim + chunk * DVC;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        typedef T Tx4 __attribute__((ext_vector_type(4)));
+        Tx4 y;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = (T)(inv == 0.f ? 0.f : o[i][4 * j + c] * inv);
+        *reinterpret_cast<Tx4 *>(out + i * 32 + j * 8 + half * 4) = y;
+      }
+  }
+}
+
+// weight[s] += sum over the rows of exp2(logit - lse[row]): the logits once more, now S = Q K^T, so that a lane holds one slot and its sum
+// runs over registers.  One workgroup: NS x 32 slots, their keys widened once into registers; the waves take 32 rows in turn.
+template <int DK, int PARTS>
+__global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
+  typedef typename ReadType<PARTS>::T T;
+  constexpr int NS = DK <= 128 ? 4 : 2, KS = DK / 16;
+  __shared__ float sums[4][NS * 32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  const int bh = blockIdx.y, b = bh / a.heads, h = bh - b * a.heads, base = blockIdx.x * NS * 32;
+  const int len = (int)read_len(a, b), cnt = read_count(a, b);
+  if (base >= len) return;
+  const int64_t row_base = (int64_t)bh * a.slots;
+  bf16x8 kf[NS][KS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const int slot = base + s * 32 + col;
+    KeyRow<DK> k;
+    k.load(a.kc, a.ks, row_base + (slot < len ? slot : len - 1), half);
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) kf[s][i * 4 + u] = bank4_unpack8(k.codes[i][u], k.scale(i));
+  }
+  float acc[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) acc[s] = 0.f;
+  const int rows = cnt * a.group < a.rows ? cnt * a.group : a.rows;       // rows behind the count have no weight
+  for (int r0 = wave * 32; r0 < rows; r0 += 128) {
+    if (a.causal && read_limit(a, len, cnt, (r0 + 31 < rows ? r0 + 31 : rows - 1) / a.group) <= base) continue;
+    const int r = r0 + col, t = r / a.group;
+    const bool live = r < rows;
+    const T *qrow = (const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh;
+    f32x16 x[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[s][j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      f32x8 y = load8(qrow + (i / 4) * 64 + half * 32 + (i & 3) * 8, a.q_vec);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = live ? y[j] * a.q_sign : 0.f;
+      bf16x8 qf[PARTS];
+      split8<PARTS>(y, qf);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) x[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[p], kf[s][i], x[s], 0, 0, 0);
+    }
+    const bool edge = a.causal || r0 + 32 > rows;
+    const float *lse = a.lse + (int64_t)bh * a.rows + r0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int rr = mfma32_row(j, lane), row = r0 + rr;
+      const float shift = lse[row < rows ? rr : rows - 1 - r0];
+      const int lim = !edge ? len : row < rows ? (int)read_limit(a, len, cnt, row / a.group) : 0;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift));
+        acc[s] += base + s * 32 + col < lim ? p : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    acc[s] += __shfl_xor(acc[s], 32);
+    if (half == 0) sums[wave][s * 32 + col] = acc[s];
+  }
+  __syncthreads();
+  if (tid < NS * 32 && base + tid < len) a.weight[row_base + base + tid] += sums[0][tid] + sums[1][tid] + sums[2][tid] + sums[3][tid];
+}
+
+// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum and log2 of the sum of the weights, and the
+// factors of its slices' accumulators.
+struct RowJoin {
+  float f[2], inv, lse;
+  __device__ __forceinline__ RowJoin(const ReadArgs &a, int bh, int row, int lane) {
+    const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + row) * 2;
+    float m[2], l[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int s = lane + 64 * k;
+      const f32x2 v = s < a.nsplit ? *reinterpret_cast<const f32x2 *>(ml + (int64_t)s * a.rows * 2) : f32x2{-INFINITY, 0.f};
+      m[k] = v.x;
+      l[k] = v.y;
+    }
+    float mm = fmaxf(m[0], m[1]);
+    for (int d = 1; d < 64; d <<= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
+    const float mu = mm == -INFINITY ? 0.f : mm;
+    f[0] = __builtin_amdgcn_exp2f(m[0] - mu);
+    f[1] = __builtin_amdgcn_exp2f(m[1] - mu);
+    float sum = f[0] * l[0] + f[1] * l[1];
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    inv = sum != 0.f ? 1.f / sum : 0.f;
+    lse = mu + (sum != 0.f ? __builtin_amdgcn_logf(sum) : 0.f);
+  }
+};
+
+// Joins the slices of a row (first `out_blocks` workgroups, one wave a row; QL lanes cover the value channels, 64 / QL slices at a time)
+// and adds the rows' weights to the slots (the others, 1024 slots each, the rows in order: the sum does not depend on timing).
+template <int PARTS, int QL>
 __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blocks) {
   typedef typename ReadType<PARTS>::T T;
-  __shared__ float lse[256];
-  __shared__ int lim[256];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int n_bh = a.batch * a.heads;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if ((int)blockIdx.x < out_blocks) {
-    const int64_t g = (int64_t)blockIdx.x * 4 + (tid >> 6);
-    if (g >= (int64_t)n_bh * a.rows) return;
+    const int64_t g = (int64_t)blockIdx.x * 4 + wave;
+    if (g >= (int64_t)a.batch * a.heads * a.rows) return;
     const int bh = (int)(g / a.rows), row = (int)(g - (int64_t)bh * a.rows), b = bh / a.heads, h = bh - b * a.heads;
-    const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + row) * 2;
-    float mm = -INFINITY, sum = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) mm = fmaxf(mm, ml[(int64_t)s * a.rows * 2]);
-    const float mu = mm == -INFINITY ? 0.f : mm;
-    for (int s = 0; s < a.nsplit; ++s) sum += __builtin_amdgcn_exp2f(ml[(int64_t)s * a.rows * 2] - mu) * ml[(int64_t)s * a.rows * 2 + 1];
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    const RowJoin J(a, bh, row, lane);
+    if (a.lse && lane == 0) a.lse[g] = J.lse;
     const int t = row / a.group, j = h * a.group + row - t * a.group;
     T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + j) * a.value_dim;
-    for (int dv = lane; dv < a.value_dim; dv += 64) {
-      float acc = 0.f;
-      for (int s = 0; s < a.nsplit; ++s)
-        acc += __builtin_amdgcn_exp2f(ml[(int64_t)s * a.rows * 2] - mu) * a.part_o[(((int64_t)bh * a.nsplit + s) * a.rows + row) * a.value_dim + dv];
-      out[dv] = (T)(acc * inv);
+    const float *part = a.part_o + ((int64_t)bh * a.nsplit * a.rows + row) * a.value_dim;
+    const int64_t stride = (int64_t)a.rows * a.value_dim;
+    for (int dv = lane % QL * 4; dv < a.value_dim; dv += QL * 4) {
+      f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int s0 = 0; s0 < a.nsplit; s0 += 64 / QL) {
+        const int s = s0 + lane / QL;
+        const float f0 = __shfl(J.f[0], s & 63), f1 = __shfl(J.f[1], s & 63), f = s < 64 ? f0 : f1;
+        if (s < a.nsplit && f != 0.f) acc += f * *reinterpret_cast<const f32x4 *>(part + s * stride + dv);     // (an empty slice's accumulators may be anything)
+      }
+#pragma unroll
+      for (int d = QL; d < 64; d <<= 1)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], d);
+      if (lane < QL) {
+        typedef T Tx4 __attribute__((ext_vector_type(4)));
+        Tx4 y;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = (T)(J.inv == 0.f ? 0.f : acc[c] * J.inv);
+        *reinterpret_cast<Tx4 *>(out + dv) = y;
+      }
     }
     return;
   }
+  __shared__ float lse[BLOCK_ROWS_MIN];
+  __shared__ int lim[BLOCK_ROWS_MIN];
   const int per = (int)((a.slots + 1023) / 1024), g = blockIdx.x - out_blocks, bh = g / per, b = bh / a.heads;
   const int64_t slot = (int64_t)(g - bh * per) * 1024 + tid * 4;
   const int64_t len = read_len(a, b);
+  if (slot - tid * 4 >= len) return;
   const int cnt = read_count(a, b);
-  f32x4 acc{0.f, 0.f, 0.f, 0.f};
-  for (int r0 = 0; r0 < a.rows; r0 += 256) {
-    const int n = a.rows - r0 < 256 ? a.rows - r0 : 256;
-    __syncthreads();
-    if (tid < n) {
-      const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + r0 + tid) * 2;
-      float mm = -INFINITY, sum = 0.f;
-      for (int s = 0; s < a.nsplit; ++s) mm = fmaxf(mm, ml[(int64_t)s * a.rows * 2]);
-      const float mu = mm == -INFINITY ? 0.f : mm;
-      for (int s = 0; s < a.nsplit; ++s) sum += __builtin_amdgcn_exp2f(ml[(int64_t)s * a.rows * 2] - mu) * ml[(int64_t)s * a.rows * 2 + 1];
-      lse[tid] = sum != 0.f ? mu + __builtin_amdgcn_logf(sum) : 0.f;
-      lim[tid] = (int)read_limit(a, len, cnt, (r0 + tid) / a.group);
-    }
-    __syncthreads();
-    if (slot < len)
-      for (int i = 0; i < n; ++i) {
-        if (slot >= lim[i]) continue;
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(a.logits + ((int64_t)bh * a.rows + r0 + i) * a.logit_stride + slot);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] += slot + j < lim[i] ? __builtin_amdgcn_exp2f(x[j] - lse[i]) : 0.f;
-      }
+  for (int i = wave; i < a.rows; i += 4) {
+    const RowJoin J(a, bh, i, lane);
+    if (lane == 0) { lse[i] = J.lse; lim[i] = (int)read_limit(a, len, cnt, i / a.group); }
   }
+  __syncthreads();
+  if (slot >= len) return;
+  f32x4 acc{0.f, 0.f, 0.f, 0.f};
+  const float *x0 = a.logits + (int64_t)bh * a.rows * a.logit_stride + slot;
+#pragma unroll 4
+  for (int i = 0; i < a.rows; ++i) {
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(x0 + (int64_t)i * a.logit_stride);   // written up to the row's limit only
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += slot + j < lim[i] ? __builtin_amdgcn_exp2f(x[j] - lse[i]) : 0.f;
+  }
+  float *w = a.weight + (int64_t)bh * a.slots + slot;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (slot + j < len) a.weight[(int64_t)bh * a.slots + slot + j] += acc[j];
+    if (slot + j < len) w[j] += acc[j];
 }
 
 // ---------------------------------------------------------------------------------------------- launch plan
 struct ReadPlan {
   int rows, tiles, nsplit, nvc, dvc;
+  bool block;                        // 128 rows a workgroup (else 16)
   bool parts;                        // partial results go through the workspace
-  int64_t part_o, part_ml, logits, logit_stride;      // bytes
+  int64_t part_o, part_ml, logits, lse, logit_stride;      // bytes
 };
+
 
 static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, ReadPlan *p) {
   if (q_heads < 1 || q_heads % k->heads || tokens < 0) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: %d query heads over %d bank heads, %d tokens", q_heads, k->heads, tokens);
@@ -288,28 +709,62 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, R
   const int64_t rows = (int64_t)tokens * (q_heads / k->heads);
   if (rows > (1 << 20)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: %lld rows a bank head (at most 2^20)", (long long)rows);
   p->rows = (int)rows;
-  p->tiles = cdiv(rows, 16);
+  p->block = rows >= BLOCK_ROWS_MIN;
+  p->tiles = cdiv(rows, p->block ? 128 : 16);
   p->dvc = k->value_dim % 128 ? 64 : 128;
   p->nvc = k->value_dim / p->dvc;
   const int64_t groups = (int64_t)p->tiles * k->batch * k->heads * p->nvc;
-  const int64_t want = groups ? (2048 + groups - 1) / groups : 1, most = (k->slots + 255) / 256;
-  p->nsplit = (int)(want < most ? want : most);
-  p->nsplit = p->nsplit > 128 ? 128 : p->nsplit < 1 ? 1 : p->nsplit;
+  if (p->block) {
+    // slices of a row tile's slots: the fewest rounds of the 512 workgroups that run at once, a slice costing its join (~3 % of a round)
+    const int most = (int)(k->slots / 512 < 1 ? 1 : k->slots / 512 > 32 ? 32 : k->slots / 512);
+    double best = 1e30;
+    for (int n = 1; n <= most; ++n) {
+      const double cost = (double)((groups * n + 511) / 512) / n + 0.03 * n;
+      if (cost < best - 1e-9) { best = cost; p->nsplit = n; }
+    }
+  } else {
+    const int64_t want = groups ? (2048 + groups - 1) / groups : 1, most = (k->slots + 255) / 256;
+    p->nsplit = (int)(want < most ? want : most);
+    p->nsplit = p->nsplit > 128 ? 128 : p->nsplit < 1 ? 1 : p->nsplit;
+  }
   p->parts = p->nsplit > 1 || weigh;
   const int64_t n = (int64_t)k->batch * k->heads * p->nsplit * rows;
   p->part_o = p->parts ? n * k->value_dim * 4 : 0;
   p->part_ml = p->parts ? (n * 8 + 15) / 16 * 16 : 0;
   p->logit_stride = (k->slots + 63) / 64 * 64;
-  p->logits = weigh ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
+  p->logits = weigh && !p->block ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
+  p->lse = weigh && p->block ? (int64_t)k->batch * k->heads * rows * 4 : 0;
   return MIVOS_OK;
 }
 
 template <int DK, int DVC>
 static void rows_launch(const ReadArgs &a, const ReadPlan &p, int dtype, hipStream_t s) {
   const dim3 grid(p.nsplit, p.tiles, a.batch * a.heads * p.nvc);
+  if (p.block) {
+    if (dtype == MIVOS_BF16) bank4_block_kernel<DK, DVC, 1><<<grid, 256, 0, s>>>(a);
+    else if (dtype == MIVOS_F16) bank4_block_kernel<DK, DVC, 2><<<grid, 256, 0, s>>>(a);
+    else bank4_block_kernel<DK, DVC, 3><<<grid, 256, 0, s>>>(a);
+    return;
+  }
   if (dtype == MIVOS_BF16) bank4_rows_kernel<DK, DVC, 1><<<grid, 256, 0, s>>>(a);
   else if (dtype == MIVOS_F16) bank4_rows_kernel<DK, DVC, 2><<<grid, 256, 0, s>>>(a);
   else bank4_rows_kernel<DK, DVC, 3><<<grid, 256, 0, s>>>(a);
+}
+
+template <int PARTS>
+static void join_launch(const ReadArgs &a, int blocks, int out_blocks, hipStream_t s) {
+  if (a.value_dim <= 64) bank4_join_kernel<PARTS, 16><<<blocks, 256, 0, s>>>(a, out_blocks);
+  else if (a.value_dim <= 128) bank4_join_kernel<PARTS, 32><<<blocks, 256, 0, s>>>(a, out_blocks);
+  else bank4_join_kernel<PARTS, 64><<<blocks, 256, 0, s>>>(a, out_blocks);
+}
+
+template <int DK>
+static void weigh_launch(const ReadArgs &a, int dtype, hipStream_t s) {
+  constexpr int keys = DK <= 128 ? 128 : 64;
+  const dim3 grid(cdiv(a.slots, keys), a.batch * a.heads);
+  if (dtype == MIVOS_BF16) bank4_weigh_kernel<DK, 1><<<grid, 256, 0, s>>>(a);
+  else if (dtype == MIVOS_F16) bank4_weigh_kernel<DK, 2><<<grid, 256, 0, s>>>(a);
+  else bank4_weigh_kernel<DK, 3><<<grid, 256, 0, s>>>(a);
 }
 
 }  // namespace mivos
@@ -320,7 +775,7 @@ extern "C" int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
   if (int rc = read_plan(bank, q_heads, tokens, weigh, &p)) return rc;
-  return p.part_o + p.part_ml + p.logits;
+  return p.part_o + p.part_ml + p.logits + p.lse;
 }
 
 extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t qb, int64_t qt, int64_t qh, int dtype, int q_heads, int tokens,
@@ -331,7 +786,7 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out))) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument");
   if (int rc = read_plan(bank, q_heads, tokens, weigh, &p)) return rc;
   if (p.rows == 0) return MIVOS_OK;
-  const int64_t need = p.part_o + p.part_ml + p.logits;
+  const int64_t need = p.part_o + p.part_ml + p.logits + p.lse;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: workspace of %lld bytes, 16-byte aligned", (long long)need);
   if (p.tiles > 65535 || (int64_t)bank->batch * bank->heads * p.nvc > 65535) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many row tiles");
@@ -341,10 +796,17 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   a.weight = bank->weight; a.lens = bank->lens; a.count = count; a.q = q; a.out = out; a.qb = qb; a.qt = qt; a.qh = qh;
   char *ws = (char *)workspace;
   if (p.parts) { a.part_o = (float *)ws; a.part_ml = (float *)(ws + p.part_o); }
-  if (weigh) a.logits = (float *)(ws + p.part_o + p.part_ml);
+  if (p.logits) a.logits = (float *)(ws + p.part_o + p.part_ml);
+  if (p.lse) a.lse = (float *)(ws + p.part_o + p.part_ml);
   a.slots = bank->slots; a.logit_stride = p.logit_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
   a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
+  a.q_sign = 1.f;
+  if (p.block) {            // logits are compared before they are scaled: a scale above 0 (0 itself as 2^-100: every weight rounds to 1)
+    a.q_sign = scale < 0.f ? -1.f : 1.f;
+    a.scale_log2 = a.scale_log2 * a.q_sign;
+    if (a.scale_log2 < 0x1p-100f) a.scale_log2 = 0x1p-100f;
+  }
   a.q_vec = (((qb | qt | qh) * dtype_bytes(dtype)) & 15) == 0 && ((uintptr_t)q & 15) == 0;
 #define GO(DK) (p.dvc == 64 ? rows_launch<DK, 64>(a, p, dtype, s) : rows_launch<DK, 128>(a, p, dtype, s))
   if (bank->key_dim == 64) GO(64);
@@ -354,10 +816,17 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (int rc = check_launch("bank4_read")) return rc;
   if (!p.parts) return MIVOS_OK;
   const int64_t out_blocks = ((int64_t)a.batch * a.heads * a.rows + 3) / 4;
-  const int64_t blocks = out_blocks + (weigh ? (int64_t)a.batch * a.heads * ((a.slots + 1023) / 1024) : 0);
+  const int64_t blocks = out_blocks + (a.logits ? (int64_t)a.batch * a.heads * ((a.slots + 1023) / 1024) : 0);
   if (blocks > 0x7fffffff) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many rows");
-  if (dtype == MIVOS_BF16) bank4_join_kernel<1><<<(int)blocks, 256, 0, s>>>(a, (int)out_blocks);
-  else if (dtype == MIVOS_F16) bank4_join_kernel<2><<<(int)blocks, 256, 0, s>>>(a, (int)out_blocks);
-  else bank4_join_kernel<3><<<(int)blocks, 256, 0, s>>>(a, (int)out_blocks);
+  if (dtype == MIVOS_BF16) join_launch<1>(a, (int)blocks, (int)out_blocks, s);
+  else if (dtype == MIVOS_F16) join_launch<2>(a, (int)blocks, (int)out_blocks, s);
+  else join_launch<3>(a, (int)blocks, (int)out_blocks, s);
+  if (int rc = check_launch("bank4_read")) return rc;
+  if (!a.lse) return MIVOS_OK;
+#define GO(DK) weigh_launch<DK>(a, dtype, s)
+  if (bank->key_dim == 64) GO(64);
+  else if (bank->key_dim == 128) GO(128);
+  else GO(256);
+#undef GO
   return check_launch("bank4_read");
 }

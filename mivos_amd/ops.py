@@ -7,6 +7,9 @@ slots) are passed as strides, never copied.  CPU tensors are rejected: there is 
 """
 import contextlib
 import ctypes as C
+import decimal
+import functools
+import struct
 
 import torch
 
@@ -54,7 +57,8 @@ def on_device(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the raw handle of torch.cuda.current_stream() without the Stream object around it (0.3 against 2.8 us a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 _PUBLISH = [True]
@@ -1051,10 +1055,14 @@ def interleave(planes, n, p, c_out, device):
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # mivos_dtype
 
 
-def _same_device(ref, *tensors):
-    for t in tensors:
-        if t is not None and t.device != ref.device:
+def _here(ref, *others):
+    """All operands on one device, and that device the current gfx950 (_ensure_device)."""
+    index = ref.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
             raise MivosHipError(f"operands live on {ref.device} and {t.device}")
+    if index not in _checked_devices or index != torch.cuda.current_device():
+        _ensure_device(ref)
 
 
 def _dtype_code(t):
@@ -1066,7 +1074,7 @@ def _dtype_code(t):
 
 def _head_rows(t, name, shape=None):
     """[B, N, heads, channels] with dense channels (any other strides); checks the shape."""
-    if t.dim() != 4 or (shape is not None and tuple(t.shape) != tuple(shape)):
+    if t.dim() != 4 or (shape is not None and t.shape != shape):
         raise MivosHipError(f"{name}: expected {'[batch, tokens, heads, channels]' if shape is None else list(shape)}, got {list(t.shape)}")
     if t.stride(3) != 1 and t.shape[3] > 1 and t.numel():
         raise MivosHipError(f"{name}: the channel stride must be 1")
@@ -1079,6 +1087,24 @@ def _int32_vector(t, n, name):
     return t
 
 
+@functools.lru_cache(maxsize=64)
+def _rotary_table(sections, base, shared):
+    """(turns a position in units of 2^-64 as signed integers, axis) of every channel pair; a ladder is one power and its multiples."""
+    with decimal.localcontext() as ctx:
+        ctx.prec = 50
+        turn = 2 ** 64 / (2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459"))
+        turns, axes, f = [], [], turn
+        for axis, n in enumerate(sections):
+            step = decimal.Decimal(base) ** (decimal.Decimal(-1) / (sum(sections) if shared else max(n, 1)))
+            f = f if shared else turn
+            for _ in range(n):
+                u = int(f.to_integral_value()) % 2 ** 64
+                turns.append(u - 2 ** 64 if u >= 2 ** 63 else u)
+                axes.append(axis)
+                f *= step
+    return turns, axes
+
+
 class RotaryAxes:
     """Plan of a rotary position with several axes: `sections[a]` channel pairs turn with axis a (time, height, width, ...), the channels
     behind the pairs are not turned.  Pair j of a section of n has the frequency base^(-j / n); shared=True: one ladder over all pairs,
@@ -1087,7 +1113,6 @@ class RotaryAxes:
     __slots__ = ("head_dim", "sections", "pairs", "interleaved", "freq", "axis")
 
     def __init__(self, head_dim, sections, base=10000.0, shared=False, interleaved=False, device="cuda"):
-        import decimal
         sections = tuple(int(n) for n in sections)
         pairs = sum(sections)
         if not sections or min(sections) < 0 or pairs < 1 or 2 * pairs > head_dim or head_dim > 512:
@@ -1095,20 +1120,28 @@ class RotaryAxes:
         if not 0 < base < float("inf"):
             raise MivosHipError(f"RotaryAxes: base {base}")
         self.head_dim, self.sections, self.pairs, self.interleaved = int(head_dim), sections, pairs, bool(interleaved)
-        with decimal.localcontext() as ctx:
-            ctx.prec = 60
-            D = decimal.Decimal
-            two_pi = 2 * D("3.14159265358979323846264338327950288419716939937510582097494459")
-            steps = [(D(i) / pairs if shared else D(j) / n, a) for i, (a, n, j) in enumerate((a, n, j) for a, n in enumerate(sections) for j in range(n))]
-            turns = [int((D(float(base)) ** -e / two_pi * 2 ** 64).to_integral_value()) % 2 ** 64 for e, _ in steps]
-        self.freq = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=device)
-        self.axis = torch.tensor([a for _, a in steps], dtype=torch.int32, device=device)
+        turns, axes = _rotary_table(sections, float(base), bool(shared))
+        self.freq = torch.tensor(turns, dtype=torch.int64, device=device)
+        self.axis = torch.tensor(axes, dtype=torch.int32, device=device)
         if self.freq.is_cuda:
             with torch.cuda.device(self.freq.device):
                 publish_constants()
 
 
-def _rotary_desc(q, k, positions, plan, inverse, eps):
+# mivos_rotary, packed at once: two mivos_rotary_rows (x, g, y, weight, six strides, heads), then the rest in order
+_ROTARY = struct.Struct("4Q6qii" * 2 + "4Q4q7if")
+
+
+def _rotary_rows(x, y, g=None, weight=None):
+    b, n, h, _ = x.stride()
+    gb, gn, gh = (0, 0, 0) if g is None else g.stride()[:3]
+    return x.data_ptr(), 0 if g is None else g.data_ptr(), y.data_ptr(), 0 if weight is None else weight.data_ptr(), b, n, h, gb, gn, gh, x.shape[2], 0
+
+
+_NO_ROWS = (0,) * 12
+
+
+def _rotary_check(q, k, positions, plan):
     _head_rows(q, "q")
     b, n, _, d = q.shape
     if d != plan.head_dim:
@@ -1117,42 +1150,29 @@ def _rotary_desc(q, k, positions, plan, inverse, eps):
         _head_rows(k, "k", (b, n, k.shape[2] if k.dim() == 4 else -1, d))
         if k.dtype != q.dtype:
             raise MivosHipError(f"q is {q.dtype}, k is {k.dtype}")
-    if positions.dtype != torch.int32 or tuple(positions.shape) != (b, n, len(plan.sections)):
+    if positions.dtype != torch.int32 or positions.shape != (b, n, len(plan.sections)):
         raise MivosHipError(f"positions: expected int32 {[b, n, len(plan.sections)]}, got {positions.dtype} {list(positions.shape)}")
-    code = _dtype_code(q)
-    _same_device(q, k, positions, plan.freq)
-    _ensure_device(q)
-    desc = RotaryDesc()
-    desc.positions, desc.freq, desc.axis = positions.data_ptr(), plan.freq.data_ptr(), plan.axis.data_ptr()
-    desc.pb, desc.pn, desc.pa = positions.stride()
-    desc.batch, desc.tokens, desc.dim, desc.pairs = b, n, d, plan.pairs
-    desc.dtype, desc.interleaved, desc.inverse, desc.eps = code, plan.interleaved, inverse, eps
-    return desc
+    return _dtype_code(q)
 
 
-def _rotary_rows(row, x, g=None, weight=None):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    row.x, row.y, row.heads = x.data_ptr(), y.data_ptr(), x.shape[2]
-    row.xb, row.xn, row.xh = x.stride()[:3]
-    if g is not None:
-        row.g = g.data_ptr()
-        row.gb, row.gn, row.gh = g.stride()[:3]
-    if weight is not None:
-        row.weight = weight.data_ptr()
-    return y
+def _rotary_desc(q, q_rows, k_rows, positions, plan, code, inverse, eps, ws=0, ws_bytes=0):
+    return RotaryDesc.from_buffer_copy(_ROTARY.pack(*q_rows, *k_rows, positions.data_ptr(), plan.freq.data_ptr(), plan.axis.data_ptr(), ws, *positions.stride(), ws_bytes,
+                        q.shape[0], q.shape[1], plan.head_dim, plan.pairs, code, plan.interleaved, inverse, eps))
 
 
 def _norm_weight(w, ref, name):
-    if w is None or w.dtype != torch.float32 or tuple(w.shape) != (ref.shape[3],) or not w.is_contiguous():
+    if w is None or w.dtype != torch.float32 or w.shape != ref.shape[3:] or not w.is_contiguous():
         raise MivosHipError(f"{name}: expected a dense float32 [{ref.shape[3]}] tensor")
-    _same_device(ref, w)
     return w
 
 
 def _rotary(q, k, positions, plan, inverse, eps, q_weight=None, k_weight=None):
-    desc = _rotary_desc(q, k, positions, plan, inverse, eps)
-    yq = _rotary_rows(desc.rows[0], q, None, q_weight)
-    yk = None if k is None else _rotary_rows(desc.rows[1], k, None, k_weight)
+    code = _rotary_check(q, k, positions, plan)
+    _here(q, k, positions, plan.freq, q_weight, k_weight)
+    yq = q.new_empty(q.shape)
+    yk = None if k is None else k.new_empty(k.shape)
+    desc = _rotary_desc(q, _rotary_rows(q, yq, None, q_weight), _NO_ROWS if k is None else _rotary_rows(k, yk, None, k_weight), positions, plan, code,
+                        inverse, eps)
     check(_lib.load().mivos_rotary_axes(desc, _stream()))
     return yq, yk
 
@@ -1194,15 +1214,15 @@ def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, plan, eps=1e-6
     for g in (dq, dk):
         if g is not None and g.dtype != q.dtype:
             raise MivosHipError(f"q is {q.dtype}, its gradient {g.dtype}")
-    desc = _rotary_desc(q, k, positions, plan, 1, float(eps))
-    _same_device(q, dq, dk)
+    code = _rotary_check(q, k, positions, plan)
+    _here(q, k, positions, plan.freq, dq, dk, q_weight, k_weight)
     lib = _lib.load()
-    ws = torch.empty(lib.mivos_norm_rotary_grad_workspace_bytes(q.shape[3]), dtype=torch.uint8, device=q.device)
-    desc.workspace, desc.workspace_bytes = ws.data_ptr(), ws.numel()
-    gq = _rotary_rows(desc.rows[0], q, dq, q_weight)
-    gk = None if k is None else _rotary_rows(desc.rows[1], k, dk, k_weight)
-    wq = torch.empty_like(q_weight)
-    wk = None if k is None else torch.empty_like(k_weight)
+    need = lib.mivos_norm_rotary_grad_workspace_bytes(q.shape[3])
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    gq, wq = q.new_empty(q.shape), torch.empty_like(q_weight)
+    gk, wk = (None, None) if k is None else (k.new_empty(k.shape), torch.empty_like(k_weight))
+    desc = _rotary_desc(q, _rotary_rows(q, gq, dq, q_weight), _NO_ROWS if k is None else _rotary_rows(k, gk, dk, k_weight), positions, plan, code, 1,
+                        float(eps), ws.data_ptr(), need)
     check(lib.mivos_norm_rotary_grad(desc, wq.data_ptr(), None if wk is None else wk.data_ptr(), _stream()))
     return gq, gk, wq, wk
 
@@ -1233,7 +1253,8 @@ class Bank4:
                 raise MivosHipError(f"Bank4: expected a dense {dtype} {list(shape)} buffer, got {t.dtype} {list(t.shape)}")
             if dtype == torch.uint8 and t.data_ptr() % 16:
                 raise MivosHipError("Bank4: codes and scales must be 16-byte aligned")
-        _same_device(key_codes, key_scales, value_codes, value_scales, weight, lens)
+        if any(t.device != lens.device for t in (key_codes, key_scales, value_codes, value_scales, weight)):
+            raise MivosHipError("Bank4: the buffers live on different devices")
         self.key_codes, self.key_scales, self.value_codes, self.value_scales, self.weight, self.lens = key_codes, key_scales, value_codes, value_scales, weight, lens
         self.batch, self.heads, self.slots, self.key_dim, self.value_dim = b, h, s, dk, dv
         self.status = torch.zeros(1 + b, dtype=torch.int32, device=lens.device)
@@ -1259,10 +1280,6 @@ class Bank4:
             raise MivosHipError(f"Bank4: appended tokens did not fit the {self.slots} slots")
 
 
-def _overlap(a, b):
-    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
-
-
 def bank4_append(bank, keys, values, at=None, count=None):
     """keys [B, T, H, Dk], values [B, T, H, Dv] (one type; dense channels) quantised into slots [at[b], at[b] + count[b]) of the bank (at None:
     behind what is there; count None: all T); their weight becomes 0 and bank.lens[b] = at[b] + count[b].  Tokens beyond the bank's last slot
@@ -1276,12 +1293,11 @@ def bank4_append(bank, keys, values, at=None, count=None):
         at = bank.lens
     else:
         _int32_vector(at, bank.batch, "at")
-        if at.data_ptr() != bank.lens.data_ptr() and _overlap(at, bank.lens):
+        if 0 < abs(at.data_ptr() - bank._desc.lens) < 4 * bank.batch:
             raise MivosHipError("at overlaps the bank's lengths")
-    if count is not None and _overlap(_int32_vector(count, bank.batch, "count"), bank.lens):
+    if count is not None and abs(_int32_vector(count, bank.batch, "count").data_ptr() - bank._desc.lens) < 4 * bank.batch:
         raise MivosHipError("count overlaps the bank's lengths")
-    _same_device(bank.lens, keys, values, at, count)
-    _ensure_device(keys)
+    _here(bank.lens, keys, values, at, count)
     ks, vs = keys.stride(), values.stride()
     check(_lib.load().mivos_bank4_append(bank._desc, keys.data_ptr(), ks[0], ks[1], ks[2], values.data_ptr(), vs[0], vs[1], vs[2], code, at.data_ptr(),
                                          None if count is None else count.data_ptr(), keys.shape[1], _stream()))
@@ -1297,10 +1313,9 @@ def bank4_values(bank, first=None, count=None, dtype=torch.bfloat16):
         raise MivosHipError(f"bank4_values: {count} of {bank.slots} slots")
     if first is not None:
         _int32_vector(first, bank.batch, "first")
-    _same_device(bank.lens, first)
-    _ensure_device(bank.lens)
-    keys = torch.empty((bank.batch, bank.heads, count, bank.key_dim), dtype=dtype, device=bank.lens.device)
-    values = torch.empty((bank.batch, bank.heads, count, bank.value_dim), dtype=dtype, device=bank.lens.device)
+    _here(bank.lens, first)
+    keys = bank.lens.new_empty((bank.batch, bank.heads, count, bank.key_dim), dtype=dtype)
+    values = bank.lens.new_empty((bank.batch, bank.heads, count, bank.value_dim), dtype=dtype)
     check(_lib.load().mivos_bank4_values(bank._desc, None if first is None else first.data_ptr(), count, keys.data_ptr(), values.data_ptr(), _DTYPES[dtype],
                                          _stream()))
     return keys, values
@@ -1318,14 +1333,13 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
     code = _dtype_code(queries)
     if count is not None:
         _int32_vector(count, b, "count")
-    _same_device(bank.lens, queries, count)
     lib = _lib.load()
     need = lib.mivos_bank4_read_workspace_bytes(bank._desc, hq, t, weigh)
     if need < 0:
         check(int(need))
-    _ensure_device(queries)
-    out = torch.empty((b, t, hq, bank.value_dim), dtype=queries.dtype, device=queries.device)
-    ws = torch.empty(need, dtype=torch.uint8, device=queries.device) if need else None
+    _here(bank.lens, queries, count)
+    out = queries.new_empty((b, t, hq, bank.value_dim))
+    ws = queries.new_empty(need, dtype=torch.uint8) if need else None
     qs = queries.stride()
     check(lib.mivos_bank4_read(bank._desc, queries.data_ptr(), qs[0], qs[1], qs[2], code, hq, t, None if count is None else count.data_ptr(),
                                d ** -0.5 if scale is None else float(scale), causal, weigh, out.data_ptr(), None if ws is None else ws.data_ptr(), need,
@@ -1344,8 +1358,7 @@ def bank4_evict(bank, keep, out, first=0, recent=0):
         raise MivosHipError("bank4_evict: the two banks share memory")
     if not 1 <= keep <= out.slots or first < 0 or recent < 0 or first + recent > keep:
         raise MivosHipError(f"bank4_evict: keep {keep} of {out.slots} slots, first {first}, recent {recent}")
-    _same_device(bank.lens, out.lens)
-    _ensure_device(bank.lens)
-    slots = torch.empty((bank.batch, bank.heads, keep), dtype=torch.int32, device=bank.lens.device)
+    _here(bank.lens, out.lens)
+    slots = bank.lens.new_empty((bank.batch, bank.heads, keep))
     check(_lib.load().mivos_bank4_evict(bank._desc, out._desc, keep, first, recent, slots.data_ptr(), _stream()))
     return slots

@@ -152,3 +152,4 @@ def test_c_entries_check_their_arguments_without_a_gpu():
     assert lib.mivos_rotary_axes(r, None) == -1 and b"positions" in lib.mivos_last_error()
     assert lib.mivos_norm_rotary_grad(r, None, None, None) == -1
     assert C.sizeof(_lib.RotaryRows) == 88 and C.sizeof(_lib.Bank4Desc) == 80
+    assert C.sizeof(_lib.RotaryDesc) == ops._ROTARY.size and _lib.RotaryDesc.eps.offset + 4 == ops._ROTARY.size
