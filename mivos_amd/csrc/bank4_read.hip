@@ -28,7 +28,7 @@ struct ReadArgs {
   float *part_o, *part_ml, *logits, *lse;
   int64_t slots, logit_stride;
   int batch, heads, group, tokens, rows, value_dim, nsplit, causal, weigh, q_vec;
-  float scale_log2;       // scale * log2(e): the softmax runs in powers of two; bank4_block / weigh: |scale|, its sign goes to the queries
+  float scale_log2;       // |scale| * log2(e): the softmax runs in powers of two; the sign of scale goes to the queries
   float q_sign;
 };
 
@@ -69,78 +69,174 @@ template <> struct ReadType<1> { typedef __bf16 T; };
 template <> struct ReadType<2> { typedef _Float16 T; };
 template <> struct ReadType<3> { typedef float T; };
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
+
+// Rows [0, n) of a bank array behind a wave-uniform address: loads take one per-lane offset and answer 0 behind the last row (codes 0, scale
+// byte 0: the value 0), so that what lies behind a stream's length is neither addressed nor looked at.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bank_rows(const uint8_t *p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes), 0x00020000);
+}
+
+// 16 channels of a bf16 query as two 8-bit floats each, in units of 2^e: the high four bits and (32 times) the rest.
+__device__ __forceinline__ void split_fp8(const float (&x)[16], float down, int *hi, int *lo) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    int h = 0, l = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float y0 = x[w * 4 + j * 2] * down, y1 = x[w * 4 + j * 2 + 1] * down;
+      const int pair = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
+      const float r0 = (y0 - __builtin_amdgcn_cvt_f32_fp8(pair, 0)) * 32.f, r1 = (y1 - __builtin_amdgcn_cvt_f32_fp8(pair, 1)) * 32.f;
+      h |= (pair & 0xffff) << (16 * j);
+      l |= (__builtin_amdgcn_cvt_pk_fp8_f32(r0, r1, 0, false) & 0xffff) << (16 * j);
+    }
+    hi[w] = h;
+    lo[w] = l;
+  }
+}
+__device__ __forceinline__ float load_fp8_piece(const __bf16 *p, bool vec, bool live, float sign, float (&x)[16]) {     // -> its largest magnitude
+  const f32x8 x0 = load8(p, vec), x1 = load8(p + 8, vec);
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    x[j] = live ? (j < 8 ? x0[j & 7] : x1[j & 7]) * sign : 0.f;
+    const float m = __builtin_fabsf(x[j]);
+    top = m < INFINITY ? fmaxf(top, m) : INFINITY;
+  }
+  return top;
+}
+// the block's largest goes to [128, 256) of the 8-bit format's 448; an infinity or NaN makes the block NaN
+__device__ __forceinline__ int fp8_exponent(float top, float &down) {
+  int e = (int)(__float_as_uint(top) >> 23) - 127 - 7;
+  e = e < -110 ? -110 : e;
+  down = top < INFINITY ? __uint_as_float((uint32_t)(127 - e) << 23) : NAN;
+  return e;
+}
+
+// The sum of a lane's softmax weights, as the second product uses them: bf16 queries round the weights, and the output is divided by the sum of
+// the rounded ones, so that what the rounding does to all of a row's weights alike drops out.
+template <int PARTS>
+__device__ __forceinline__ float weight_sum(float l, f32x8 p, const bf16x8 &pf) {
+  if constexpr (PARTS == 1) {
+    const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pf[2 * j], pf[2 * j + 1]}, one, l, false);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l += p[j];
+  }
+  return l;
+}
+
+constexpr float MAX_LAG = 8.f;      // the running maximum follows a logit that passes it by more than this (powers of two): fewer rescales
+
+// ------------------------------------------------------------------------------------------ few rows: 16 a workgroup
 // One workgroup: 16 rows x one slice of the slots x DVC value channels; its four waves take 64 slots in turn, each with a running
-// softmax of its own, and meet in LDS at the end.
+// softmax of its own, and meet in LDS at the end.  A step's codes and scales are fetched a step ahead, 64 slots x (DK + DVC) * 17 / 32 bytes a wave.
+// bf16 queries against keys of 128 or 256 channels: 16x16x128 block-scaled products take the codes and scales as they are, against the query in
+// two 8-bit floats a channel (8 bits in all, exact down to 2^-22 of a block's largest); the others widen the keys to bf16.
 template <int DK, int DVC, int PARTS>
-__global__ __launch_bounds__(256) void bank4_rows_kernel(ReadArgs a) {
+__global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_rows_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
-  constexpr int CPL = DK / 4, KSTEPS = DK / 32, VPAD = DVC + 16, OPAD = DVC + 4, NT = DVC / 16;
+  constexpr bool SCALED = PARTS == 1 && DK % 128 == 0;
+  constexpr int CPL = DK / 4, KSTEPS = DK / 32, VPAD = DVC + 16, OPAD = DVC + 4, NT = DVC / 16, VB = DVC / 32;
   constexpr int LDS_V = 4 * 32 * VPAD * 2, LDS_O = 4 * 16 * OPAD * 4;
   __shared__ __align__(16) char lds[LDS_V > LDS_O ? LDS_V : LDS_O];
-  __shared__ float stat[4][16][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+  __shared__ float stat[4][16][3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
   const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
   const int split = blockIdx.x, row0 = blockIdx.y * 16;
-  const int64_t len = read_len(a, b);
-  const int cnt = read_count(a, b);
+  const int len = (int)read_len(a, b), cnt = read_count(a, b);
   const int r = row0 + col, t = r / a.group;
-  const int64_t limit = r < a.rows ? read_limit(a, len, cnt, t) : 0;
-  const int last_row = row0 + 15 < a.rows ? row0 + 15 : a.rows - 1;
-  int last_t = last_row / a.group;
+  const bool live = r < a.rows && t < cnt;
+  const int limit = live ? (int)read_limit(a, len, cnt, t) : 0;
+  int last_t = (row0 + 15 < a.rows ? row0 + 15 : a.rows - 1) / a.group;
   last_t = last_t < cnt ? last_t : cnt - 1;
-  const int64_t seen = row0 / a.group < cnt ? read_limit(a, len, cnt, last_t) : 0;   // slots any row of the tile sees
-  const int64_t per = ((seen + 63) / 64 + a.nsplit - 1) / a.nsplit * 64;
-  const int64_t s0 = split * per, s1 = s0 + per < seen ? s0 + per : seen;
+  const int seen = row0 / a.group < cnt ? (int)read_limit(a, len, cnt, last_t) : 0;   // slots any row of the tile sees
+  const int per = ((seen + 63) / 64 + a.nsplit - 1) / a.nsplit * 64;
+  const int s0 = (int64_t)split * per < seen ? split * per : seen, s1 = seen - s0 < per ? seen : s0 + per;
+  int low = live ? limit : seen;                                                      // slots all rows see
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    const int x = __shfl_xor(low, d);
+    low = x < low ? x : low;
+  }
+  low = __builtin_amdgcn_readfirstlane(low);
 
-  bf16x8 qf[KSTEPS][PARTS];
-  {
-    const bool live = r < a.rows && t < cnt;
-    const T *qrow = (const T *)a.q + b * a.qb + (live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh + grp * CPL;
+  i32x8 q_hi[SCALED ? DK / 128 : 1], q_lo[SCALED ? DK / 128 : 1];
+  int q_scale[SCALED ? DK / 128 : 1];
+  bf16x8 qf[SCALED ? 1 : KSTEPS][PARTS];
+  const T *qrow = (const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh;
+  if constexpr (SCALED) {
+#pragma unroll
+    for (int i = 0; i < DK / 128; ++i) {      // an 8-bit operand's lane holds channels grp * 16 .. + 15 of both halves of the 128
+      int e[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x[16], down;
+        float top = load_fp8_piece((const __bf16 *)qrow + i * 128 + k * 64 + grp * 16, a.q_vec, live, a.q_sign, x);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        e[k] = fp8_exponent(top, down);
+        int hi[4], lo[4];
+        split_fp8(x, down, hi, lo);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { q_hi[i][k * 4 + w] = hi[w]; q_lo[i][k * 4 + w] = lo[w]; }
+      }
+      // the scale a lane hands over is that of channels grp * 32 .. + 31
+      const int src = col + 32 * (grp & 1), e0 = __shfl(e[0], src), e1 = __shfl(e[1], src), mine = 127 + (grp < 2 ? e0 : e1);
+      q_scale[i] = mine | (mine - 5) << 8;
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < KSTEPS; ++i) {
-      f32x8 x = load8(qrow + i * 8, a.q_vec);
-      if (!live)
+      f32x8 x = load8(qrow + grp * CPL + i * 8, a.q_vec);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      for (int j = 0; j < 8; ++j) x[j] = live ? x[j] * a.q_sign : 0.f;
       split8<PARTS>(x, qf[i]);
     }
   }
   f32x4 o[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  const int64_t row_base = (int64_t)bh * a.slots;
+  float m = -INFINITY, l = 0.f, l_used = 0.f;
   __bf16 *vt = reinterpret_cast<__bf16 *>(lds) + wave * 32 * VPAD;
-  const int vs_row = a.value_dim / 32;
+  const int v_row = a.value_dim / 2, vs_row = a.value_dim / 32;
+  const uint8_t *kc = a.kc + (int64_t)bh * a.slots * (DK / 2), *ks = a.ks + (int64_t)bh * a.slots * (DK / 32);
+  const uint8_t *vc = a.vc + (int64_t)bh * a.slots * v_row + chunk * (DVC / 2), *vs = a.vs + (int64_t)bh * a.slots * vs_row + chunk * VB;
+  const int k_at = col * (DK / 2) + grp * (SCALED ? 16 : CPL / 2), ks_at = col * (DK / 32) + (SCALED ? grp : grp * CPL / 32);
+  const int v_at = lane / VB * v_row + lane % VB * 16, vs_at = lane / VB * vs_row + lane % VB;
 
-  // a step's codes and scales, fetched a step ahead: 64 slots x (DK + DVC) / 2 bytes a wave stay in flight while the last step is computed
   struct Step {
-    uint32_t kc[4][KSTEPS], ks[4][(KSTEPS + 7) / 8];
-    u32x4 vc[DVC / 32];
-    uint32_t vs[DVC / 32];
+    uint32_t kc[4][KSTEPS], ks[4][2];
+    u32x4 vc[VB];
+    uint32_t vs[VB];
   } now, next;
-  auto fetch = [&](Step &f, int64_t base) {
+  auto fetch = [&](Step &f, int base) {
+    const int64_t n = s1 - base, at = base;
+    const auto rk = bank_rows(kc + at * (DK / 2), n * (DK / 2)), rs = bank_rows(ks + at * (DK / 32), n * (DK / 32));
+    const auto rv = bank_rows(vc + at * v_row, n * v_row - chunk * (DVC / 2)), rw = bank_rows(vs + at * vs_row, n * vs_row - chunk * VB);
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      const int64_t slot = base + kt * 16 + col, row = row_base + (slot < a.slots ? slot : a.slots - 1);
-      const uint8_t *codes = a.kc + row * (DK / 2) + grp * (CPL / 2), *sc = a.ks + row * (DK / 32) + grp * CPL / 32;
-      if constexpr (KSTEPS == 2) *reinterpret_cast<u32x2 *>(f.kc[kt]) = *reinterpret_cast<const u32x2 *>(codes);
+      if constexpr (KSTEPS == 2) *reinterpret_cast<u32x2 *>(f.kc[kt]) = __builtin_amdgcn_raw_buffer_load_b64(rk, k_at + kt * 8 * DK, 0, 0);
       else
 #pragma unroll
-        for (int i = 0; i < KSTEPS / 4; ++i) *reinterpret_cast<u32x4 *>(f.kc[kt] + 4 * i) = reinterpret_cast<const u32x4 *>(codes)[i];
+        for (int i = 0; i < KSTEPS / 4; ++i)
+          *reinterpret_cast<u32x4 *>(f.kc[kt] + 4 * i) = __builtin_amdgcn_raw_buffer_load_b128(rk, k_at + kt * 8 * DK + i * (SCALED ? 64 : 16), 0, 0);
+      if constexpr (SCALED)
 #pragma unroll
-      for (int i = 0; i < (KSTEPS + 7) / 8; ++i) f.ks[kt][i] = KSTEPS == 8 ? *reinterpret_cast<const uint16_t *>(sc) : sc[i];
+        for (int i = 0; i < DK / 128; ++i) f.ks[kt][i] = __builtin_amdgcn_raw_buffer_load_b8(rs, ks_at + kt * (DK / 2) + i * 4, 0, 0);
+      else if constexpr (KSTEPS == 8) f.ks[kt][0] = __builtin_amdgcn_raw_buffer_load_b16(rs, ks_at + kt * (DK / 2), 0, 0);
+      else f.ks[kt][0] = __builtin_amdgcn_raw_buffer_load_b8(rs, ks_at + kt * (DK / 2), 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < DVC / 32; ++i) {       // 64 rows x DVC / 32 blocks of 16 bytes over 64 lanes
-      const int e = i * 64 + lane;
-      const int64_t slot = base + e / (DVC / 32), row = row_base + (slot < a.slots ? slot : a.slots - 1);
-      f.vc[i] = *reinterpret_cast<const u32x4 *>(a.vc + row * (a.value_dim / 2) + chunk * (DVC / 2) + e % (DVC / 32) * 16);
-      f.vs[i] = a.vs[row * vs_row + chunk * (DVC / 32) + e % (DVC / 32)];
+    for (int i = 0; i < VB; ++i) {       // 64 rows x VB blocks of 16 bytes over 64 lanes
+      f.vc[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, v_at, i * (64 / VB) * v_row, 0);
+      f.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, vs_at, i * (64 / VB) * vs_row, 0);
     }
   };
   if (s0 + wave * 64 < s1) fetch(next, s0 + wave * 64);
-  for (int64_t base = s0 + wave * 64; base < s1; base += 256) {
+  for (int base = s0 + wave * 64; base < s1; base += 256) {
     now = next;
     if (base + 256 < s1) fetch(next, base + 256);
     // ---- logits of 64 slots
@@ -148,115 +244,130 @@ __global__ __launch_bounds__(256) void bank4_rows_kernel(ReadArgs a) {
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
       x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (SCALED) {
 #pragma unroll
-      for (int i = 0; i < KSTEPS; ++i) {
-        const bf16x8 kf = bank4_unpack8(now.kc[kt][i], bank4_scale(KSTEPS == 8 ? (now.ks[kt][0] >> (i / 4 * 8)) & 255 : now.ks[kt][0]));
+        for (int i = 0; i < DK / 128; ++i) {
+          const i32x8 kf = {(int)now.kc[kt][4 * i], (int)now.kc[kt][4 * i + 1], (int)now.kc[kt][4 * i + 2], (int)now.kc[kt][4 * i + 3], 0, 0, 0, 0};
+          x[kt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_hi[i], x[kt], 4, 0, 0, (int)now.ks[kt][i], 0, q_scale[i]);
+          x[kt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_lo[i], x[kt], 4, 0, 0, (int)now.ks[kt][i], 1, q_scale[i]);
+        }
+      } else {
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][p], x[kt], 0, 0, 0);
+        for (int i = 0; i < KSTEPS; ++i) {
+          const bf16x8 kf = bank4_unpack8(now.kc[kt][i], bank4_scale(KSTEPS == 8 ? (now.ks[kt][0] >> (i / 4 * 8)) & 255 : now.ks[kt][0]));
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][p], x[kt], 0, 0, 0);
+        }
       }
     }
+    if (base + 64 > low || base + 64 > s1) {
+      const int lim = limit < s1 ? limit : s1;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[kt][j] = base + kt * 16 + grp * 4 + j < lim ? x[kt][j] : -INFINITY;
+    }
+    if (a.logits && chunk == 0 && r < a.rows)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+        *reinterpret_cast<f32x4 *>(a.logits + ((int64_t)bh * a.rows + r) * a.logit_stride + base + kt * 16 + grp * 4) = x[kt] * a.scale_log2;
     float top = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t slot = base + kt * 16 + grp * 4 + j;
-        x[kt][j] = slot < limit && slot < s1 ? x[kt][j] * a.scale_log2 : -INFINITY;
-        top = fmaxf(top, x[kt][j]);
-      }
-      if (a.weigh && chunk == 0 && r < a.rows)
-        *reinterpret_cast<f32x4 *>(a.logits + ((int64_t)bh * a.rows + r) * a.logit_stride + base + kt * 16 + grp * 4) = x[kt];
-    }
+    for (int kt = 0; kt < 4; ++kt) top = fmaxf(top, fmaxf(fmaxf(x[kt][0], x[kt][1]), fmaxf(x[kt][2], x[kt][3])));
     top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.f : mn, alpha = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
-    l *= alpha;
+    top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+    if (__any(top > m + MAX_LAG)) {
+      const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+      l_used *= alpha;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i] *= alpha;
+      for (int i = 0; i < NT; ++i) o[i] *= alpha;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
     // ---- V in two halves of 32 slots
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       f32x8 p;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(x[half * 2 + j / 4][j % 4] - mu);
-        l += p[j];
-      }
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[half * 2 + j / 4][j % 4], a.scale_log2, -mu));
       bf16x8 pf[PARTS];
       split8<PARTS>(p, pf);
+      l_used = weight_sum<PARTS>(l_used, p, pf[0]);
+      if (PARTS == 1 && a.logits)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) l += p[j];
       wave_lds_fence();
 #pragma unroll
-      for (int i = 0; i < DVC / 64; ++i) {
-        const int e = i * 64 + lane, vr = e / (DVC / 32), blk = e % (DVC / 32);
-        u32x4 codes = now.vc[half * (DVC / 64) + i];
-        uint32_t byte = now.vs[half * (DVC / 64) + i];
-        if (base + half * 32 + vr >= s1) { codes = u32x4{0u, 0u, 0u, 0u}; byte = 127; }      // never-written memory may stand for NaN
-        const float sc = bank4_scale(byte);
+      for (int i = 0; i < VB / 2; ++i) {
+        const int e = i * 64 + lane, vr = e / VB, blk = e % VB;
+        const float sc = bank4_scale(now.vs[half * (VB / 2) + i]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(vt + vr * VPAD + blk * 32 + j * 8) = bank4_unpack8(codes[j], sc);
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(vt + vr * VPAD + blk * 32 + j * 8) = bank4_unpack8(now.vc[half * (VB / 2) + i][j], sc);
       }
       wave_lds_fence();
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        typedef __attribute__((address_space(3))) s16x4 *lds_p;
         const __bf16 *at = vt + (grp * 4 + col / 4) * VPAD + i * 16 + (col % 4) * 4;
-        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at));
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + 16 * VPAD));
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 16 * VPAD));
         const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[q], o[i], 0, 0, 0);
       }
     }
   }
+  if (PARTS > 1) l = l_used;
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
+  l_used += __shfl_xor(l_used, 16);
+  l_used += __shfl_xor(l_used, 32);
   // ---- the four waves meet
   __syncthreads();
   float *om = reinterpret_cast<float *>(lds);
 #pragma unroll
   for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4 *>(om + (wave * 16 + col) * OPAD + i * 16 + grp * 4) = o[i];
-  if (grp == 0) { stat[wave][col][0] = m; stat[wave][col][1] = l; }
+  if (grp == 0) { stat[wave][col][0] = m; stat[wave][col][1] = l_used; stat[wave][col][2] = l; }
   __syncthreads();
   for (int e = tid; e < 16 * DVC; e += 256) {
     const int rr = e / DVC, dv = e % DVC, row = row0 + rr;
     if (row >= a.rows) break;
     const float mm = fmaxf(fmaxf(stat[0][rr][0], stat[1][rr][0]), fmaxf(stat[2][rr][0], stat[3][rr][0]));
     const float mu = mm == -INFINITY ? 0.f : mm;
-    float acc = 0.f, sum = 0.f;
+    float acc = 0.f, used = 0.f, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float f = __builtin_amdgcn_exp2f(stat[w][rr][0] - mu);
       acc += f * om[(w * 16 + rr) * OPAD + dv];
-      sum += f * stat[w][rr][1];
+      used += f * stat[w][rr][1];
+      sum += f * stat[w][rr][2];
     }
     if (a.part_o) {
       const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + row;
       a.part_o[at * a.value_dim + chunk * DVC + dv] = acc;
-      if (dv == 0 && chunk == 0) { a.part_ml[at * 2] = mm; a.part_ml[at * 2 + 1] = sum; }
+      if (dv == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = f32x4{mm, used, sum, 0.f};
     } else {
       const int tt = row / a.group, j = h * a.group + row - tt * a.group;
-      ((T *)a.out)[(((int64_t)b * a.tokens + tt) * a.heads * a.group + j) * a.value_dim + chunk * DVC + dv] = (T)(sum != 0.f ? acc / sum : 0.f);
+      ((T *)a.out)[(((int64_t)b * a.tokens + tt) * a.heads * a.group + j) * a.value_dim + chunk * DVC + dv] = (T)(used != 0.f ? acc / used : 0.f);
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------ many rows: 128 a workgroup
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 // K rows of a tile in a lane's registers: 32x32 products take row l % 32, channels i * 64 + (l / 32) * 32 .. + 31 of it.
 template <int DK>
 struct KeyRow {
   static constexpr int KI = DK / 64;
   u32x4 codes[KI];
   uint32_t scales[(KI + 1) / 2];        // byte 2 (i % 2) of word i / 2: the scale of the lane's block i
-  __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *ks, int64_t row, int half) {
+  // row `col` + `row` of the arrays behind rk / rs
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rs, int row, int col, int half) {
 #pragma unroll
-    for (int i = 0; i < KI; ++i) codes[i] = *reinterpret_cast<const u32x4 *>(kc + row * (DK / 2) + i * 32 + half * 16);
-    if constexpr (KI == 1) scales[0] = ks[row * 2 + half];
+    for (int i = 0; i < KI; ++i) codes[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, col * (DK / 2) + half * 16, row * (DK / 2) + i * 32, 0);
+    if constexpr (KI == 1) scales[0] = __builtin_amdgcn_raw_buffer_load_b8(rs, col * 2 + half, row * 2, 0);
     else
 #pragma unroll
-      for (int i = 0; i < KI / 2; ++i) scales[i] = reinterpret_cast<const uint32_t *>(ks + row * (DK / 32))[i] >> (8 * half);
+      for (int i = 0; i < KI / 2; ++i) scales[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, col * (DK / 32), row * (DK / 32) + i * 4, 0) >> (8 * half);
   }
   __device__ __forceinline__ float scale(int i) const { return bank4_scale((scales[i / 2] >> (16 * (i & 1))) & 255); }
 };
@@ -306,39 +417,17 @@ struct QueryCols<DK, 1> {
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i) {
       // an 8-bit operand's lane holds channels half * 16 .. + 15 of both blocks of the 64
-      float x[2][16], top[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const f32x8 x0 = load8(row + i * 64 + b * 32 + half * 16, vec), x1 = load8(row + i * 64 + b * 32 + half * 16 + 8, vec);
-        top[b] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          x[b][j] = live ? (j < 8 ? x0[j & 7] : x1[j & 7]) * sign : 0.f;
-          const float m = __builtin_fabsf(x[b][j]);
-          top[b] = m < INFINITY ? fmaxf(top[b], m) : INFINITY;
-        }
-        top[b] = fmaxf(top[b], __shfl_xor(top[b], 32));
-      }
       int e[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {     // the block's largest in [128, 256); an infinity or NaN makes the block NaN
-        e[b] = (int)(__float_as_uint(top[b]) >> 23) - 127 - 7;
-        e[b] = e[b] < -110 ? -110 : e[b];
-        const float down = top[b] < INFINITY ? __uint_as_float((uint32_t)(127 - e[b]) << 23) : NAN;
+      for (int b = 0; b < 2; ++b) {
+        float x[16], down;
+        float top = load_fp8_piece(row + i * 64 + b * 32 + half * 16, vec, live, sign, x);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        e[b] = fp8_exponent(top, down);
+        int h[4], l[4];
+        split_fp8(x, down, h, l);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          int h = 0, l = 0;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float y0 = x[b][w * 4 + j * 2] * down, y1 = x[b][w * 4 + j * 2 + 1] * down;
-            const int pair = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
-            const float r0 = (y0 - __builtin_amdgcn_cvt_f32_fp8(pair, 0)) * 32.f, r1 = (y1 - __builtin_amdgcn_cvt_f32_fp8(pair, 1)) * 32.f;
-            h |= (pair & 0xffff) << (16 * j);
-            l |= (__builtin_amdgcn_cvt_pk_fp8_f32(r0, r1, 0, false) & 0xffff) << (16 * j);
-          }
-          hi[i][b * 4 + w] = h;
-          lo[i][b * 4 + w] = l;
-        }
+        for (int w = 0; w < 4; ++w) { hi[i][b * 4 + w] = h[w]; lo[i][b * 4 + w] = l[w]; }
       }
       const int mine = 127 + (half ? e[1] : e[0]);
       scale[i] = mine | (mine - 5) << 8;
@@ -371,9 +460,9 @@ struct QueryCols<DK, 1> {
 template <int DK, int DVC, int PARTS>
 __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1) void bank4_block_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
-  constexpr int VS = DVC + 32, NT = DVC / 32, VE = 64 * DVC / 32, VL = (VE + 255) / 256;
-  __shared__ __align__(16) __bf16 vt[2][64 * VS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+  constexpr int VS = DVC + 32, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB, VL = (VE + 255) / 256;
+  extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
   const int split = blockIdx.x, row0 = blockIdx.y * 128, r = row0 + wave * 32 + col;
   const int64_t len = read_len(a, b);
@@ -402,46 +491,45 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  const int64_t row_base = (int64_t)bh * a.slots;
-  const int last = (int)a.slots - 1;
+  float m = -INFINITY, l = 0.f, l_used = 0.f;
+  const int v_row = a.value_dim / 2, vs_row = a.value_dim / 32;
+  const uint8_t *kc = a.kc + (int64_t)bh * a.slots * (DK / 2), *ks = a.ks + (int64_t)bh * a.slots * (DK / 32);
+  const uint8_t *vc = a.vc + (int64_t)bh * a.slots * v_row + chunk * (DVC / 2), *vs = a.vs + (int64_t)bh * a.slots * vs_row + chunk * VB;
   KeyRow<DK> k[2], kn[2];
-  u32x4 vc[VL];
-  uint32_t vs[VL];
+  u32x4 vn[VL];
+  uint32_t vsn[VL];
 
   auto load_keys = [&](KeyRow<DK> *to, int base) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int slot = base + s * 32 + col;
-      to[s].load(a.kc, a.ks, row_base + (slot < last ? slot : last), half);
-    }
+    const int64_t n = s1 - base, at = base;
+    const auto rk = bank_rows(kc + at * (DK / 2), n * (DK / 2)), rs = bank_rows(ks + at * (DK / 32), n * (DK / 32));
+    to[0].load(rk, rs, 0, col, half);
+    to[1].load(rk, rs, 32, col, half);
   };
   auto load_values = [&](int base) {
+    const int64_t n = s1 - base, at = base;
+    const auto rv = bank_rows(vc + at * v_row, n * v_row - chunk * (DVC / 2)), rw = bank_rows(vs + at * vs_row, n * vs_row - chunk * VB);
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
-      const int e = i * 256 + tid, slot = base + e / (DVC / 32), blk = e % (DVC / 32);
-      if (VE < 256 && e >= VE) break;
-      const int64_t row = row_base + (slot < last ? slot : last);
-      vc[i] = *reinterpret_cast<const u32x4 *>(a.vc + row * (a.value_dim / 2) + chunk * (DVC / 2) + blk * 16);
-      vs[i] = a.vs[row * (a.value_dim / 32) + chunk * (DVC / 32) + blk];
-      if (slot >= s1) { vc[i] = u32x4{0u, 0u, 0u, 0u}; vs[i] = 127; }      // never-written memory may stand for NaN
+      if (VE < 256 && tid >= VE) break;
+      vn[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, tid / VB * v_row + tid % VB * 16, i * (256 / VB) * v_row, 0);
+      vsn[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, tid / VB * vs_row + tid % VB, i * (256 / VB) * vs_row, 0);
     }
   };
   auto store_values = [&](__bf16 *to) {
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
-      const int e = i * 256 + tid, vr = e / (DVC / 32), blk = e % (DVC / 32);
+      const int e = i * 256 + tid, vr = e / VB, blk = e % VB;
       if (VE < 256 && e >= VE) break;
-      const float sc = bank4_scale(vs[i]);
+      const float sc = bank4_scale(vsn[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(to + vr * VS + blk * 32 + j * 8) = bank4_unpack8(vc[i][j], sc);
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(to + vr * VS + blk * 32 + j * 8) = bank4_unpack8(vn[i][j], sc);
     }
   };
 
   if (s0 < s1) {
     load_keys(k, s0);
     load_values(s0);
-    store_values(vt[0]);
+    store_values(vt);
   }
   __syncthreads();
   int buf = 0;
@@ -466,10 +554,11 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
 #pragma unroll
       for (int j = 1; j < 16; ++j) top = fmaxf(fmaxf(top, x[0][j]), x[1][j]);
       top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
-      if (__any(top > m + 8.f)) {
+      if (__any(top > m + MAX_LAG)) {
         const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
         m = mn;
         l *= alpha;
+        l_used *= alpha;
 #pragma unroll
         for (int i = 0; i < NT; ++i) o[i] *= alpha;
       }
@@ -478,18 +567,18 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       for (int s = 0; s < 4; ++s) {           // 16 slots: keys 16 s + {0..3, 8..11} + 4 half
         f32x8 p;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], a.scale_log2, -mu));
-          l += p[j];
-        }
+        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], a.scale_log2, -mu));
         bf16x8 pf[PARTS];
         split8<PARTS>(p, pf);
-        const __bf16 *at = vt[buf] + (s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        l_used = weight_sum<PARTS>(l_used, p, pf[0]);
+        if (PARTS == 1 && a.weigh)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) l += p[j];
+        const __bf16 *at = vt + (buf * 64 + s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          typedef __attribute__((address_space(3))) s16x4 *lds_p;
-          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + i * 32));
-          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + i * 32 + 8 * VS));
+          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32));
+          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32 + 8 * VS));
           const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
           for (int w = 0; w < PARTS; ++w) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[w], o[i], 0, 0, 0);
@@ -497,13 +586,15 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       }
     }
     if (more) {
-      store_values(vt[buf ^ 1]);
+      store_values(vt + (buf ^ 1) * 64 * VS);
 #pragma unroll
       for (int s = 0; s < 2; ++s) k[s] = kn[s];
     }
     __syncthreads();
   }
+  if (PARTS > 1) l = l_used;
   l += __shfl_xor(l, 32);
+  l_used += __shfl_xor(l_used, 32);
   if (r >= a.rows) return;
   if (a.part_o) {
     const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + r;
@@ -513,9 +604,9 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<f32x4 *>(a.part_o + at * a.value_dim + chunk * DVC + i * 32 + j * 8 + half * 4) =
             f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
-    if (half == 0 && chunk == 0) { a.part_ml[at * 2] = live ? m : -INFINITY; a.part_ml[at * 2 + 1] = live ? l : 0.f; }
+    if (half == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = live ? f32x4{m, l_used, l, 0.f} : f32x4{-INFINITY, 0.f, 0.f, 0.f};
   } else {
-    const float inv = live && l != 0.f ? 1.f / l : 0.f;
+    const float inv = live && l_used != 0.f ? 1.f / l_used : 0.f;
     T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + h * a.group + r - t * a.group) * a.value_dim + chunk * DVC;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -542,12 +633,13 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   const int len = (int)read_len(a, b), cnt = read_count(a, b);
   if (base >= len) return;
   const int64_t row_base = (int64_t)bh * a.slots;
+  const auto rk = bank_rows(a.kc + (row_base + base) * (DK / 2), (int64_t)(len - base) * (DK / 2));
+  const auto rs = bank_rows(a.ks + (row_base + base) * (DK / 32), (int64_t)(len - base) * (DK / 32));
   bf16x8 kf[NS][KS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    const int slot = base + s * 32 + col;
     KeyRow<DK> k;
-    k.load(a.kc, a.ks, row_base + (slot < len ? slot : len - 1), half);
+    k.load(rk, rs, s * 32, col, half);
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i)
 #pragma unroll
@@ -607,23 +699,24 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
 struct RowJoin {
   float f[2], inv, lse;
   __device__ __forceinline__ RowJoin(const ReadArgs &a, int bh, int row, int lane) {
-    const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + row) * 2;
-    float m[2], l[2];
+    const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + row) * 4;
+    float m[2], u[2], l[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int s = lane + 64 * k;
-      const f32x2 v = s < a.nsplit ? *reinterpret_cast<const f32x2 *>(ml + (int64_t)s * a.rows * 2) : f32x2{-INFINITY, 0.f};
+      const f32x4 v = s < a.nsplit ? *reinterpret_cast<const f32x4 *>(ml + (int64_t)s * a.rows * 4) : f32x4{-INFINITY, 0.f, 0.f, 0.f};
       m[k] = v.x;
-      l[k] = v.y;
+      u[k] = v.y;
+      l[k] = v.z;
     }
     float mm = fmaxf(m[0], m[1]);
     for (int d = 1; d < 64; d <<= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     const float mu = mm == -INFINITY ? 0.f : mm;
     f[0] = __builtin_amdgcn_exp2f(m[0] - mu);
     f[1] = __builtin_amdgcn_exp2f(m[1] - mu);
-    float sum = f[0] * l[0] + f[1] * l[1];
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    inv = sum != 0.f ? 1.f / sum : 0.f;
+    float used = f[0] * u[0] + f[1] * u[1], sum = f[0] * l[0] + f[1] * l[1];
+    for (int d = 1; d < 64; d <<= 1) { used += __shfl_xor(used, d); sum += __shfl_xor(sum, d); }
+    inv = used != 0.f ? 1.f / used : 0.f;
     lse = mu + (sum != 0.f ? __builtin_amdgcn_logf(sum) : 0.f);
   }
 };
@@ -702,6 +795,12 @@ struct ReadPlan {
 };
 
 
+// Value channels a workgroup accumulates: every chunk computes the logits again, so as many as the registers hold.
+static int read_dvc(int dk, int dv, bool block) {
+  if (block && dk <= 128 && dv % 256 == 0) return 256;
+  return dv % 128 ? 64 : 128;
+}
+
 static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, ReadPlan *p) {
   if (q_heads < 1 || q_heads % k->heads || tokens < 0) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: %d query heads over %d bank heads, %d tokens", q_heads, k->heads, tokens);
   if (k->key_dim != 64 && k->key_dim != 128 && k->key_dim != 256) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: keys of %d channels (64, 128 or 256)", k->key_dim);
@@ -711,7 +810,7 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, R
   p->rows = (int)rows;
   p->block = rows >= BLOCK_ROWS_MIN;
   p->tiles = cdiv(rows, p->block ? 128 : 16);
-  p->dvc = k->value_dim % 128 ? 64 : 128;
+  p->dvc = read_dvc(k->key_dim, k->value_dim, p->block);
   p->nvc = k->value_dim / p->dvc;
   const int64_t groups = (int64_t)p->tiles * k->batch * k->heads * p->nvc;
   if (p->block) {
@@ -730,25 +829,41 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, R
   p->parts = p->nsplit > 1 || weigh;
   const int64_t n = (int64_t)k->batch * k->heads * p->nsplit * rows;
   p->part_o = p->parts ? n * k->value_dim * 4 : 0;
-  p->part_ml = p->parts ? (n * 8 + 15) / 16 * 16 : 0;
+  p->part_ml = p->parts ? n * 16 : 0;
   p->logit_stride = (k->slots + 63) / 64 * 64;
   p->logits = weigh && !p->block ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
   p->lse = weigh && p->block ? (int64_t)k->batch * k->heads * rows * 4 : 0;
   return MIVOS_OK;
 }
 
-template <int DK, int DVC>
-static void rows_launch(const ReadArgs &a, const ReadPlan &p, int dtype, hipStream_t s) {
+template <int DK, int DVC, int PARTS>
+static int block_launch(const ReadArgs &a, const dim3 grid, hipStream_t s) {
+  constexpr size_t lds = 2 * 64 * (DVC + 32) * 2;
+  if constexpr (lds > 65536) {
+    static std::atomic<uint64_t> raised{0};
+    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS>, lds, raised, "bank4_read")) return rc;
+  }
+  bank4_block_kernel<DK, DVC, PARTS><<<grid, 256, lds, s>>>(a);
+  return MIVOS_OK;
+}
+
+template <int DK, int PARTS>
+static int read_launch(const ReadArgs &a, const ReadPlan &p, hipStream_t s) {
   const dim3 grid(p.nsplit, p.tiles, a.batch * a.heads * p.nvc);
   if (p.block) {
-    if (dtype == MIVOS_BF16) bank4_block_kernel<DK, DVC, 1><<<grid, 256, 0, s>>>(a);
-    else if (dtype == MIVOS_F16) bank4_block_kernel<DK, DVC, 2><<<grid, 256, 0, s>>>(a);
-    else bank4_block_kernel<DK, DVC, 3><<<grid, 256, 0, s>>>(a);
-    return;
+    if constexpr (DK <= 128)
+      if (p.dvc == 256) return block_launch<DK, 256, PARTS>(a, grid, s);
+    return p.dvc == 64 ? block_launch<DK, 64, PARTS>(a, grid, s) : block_launch<DK, 128, PARTS>(a, grid, s);
   }
-  if (dtype == MIVOS_BF16) bank4_rows_kernel<DK, DVC, 1><<<grid, 256, 0, s>>>(a);
-  else if (dtype == MIVOS_F16) bank4_rows_kernel<DK, DVC, 2><<<grid, 256, 0, s>>>(a);
-  else bank4_rows_kernel<DK, DVC, 3><<<grid, 256, 0, s>>>(a);
+  if (p.dvc == 64) bank4_rows_kernel<DK, 64, PARTS><<<grid, 256, 0, s>>>(a);
+  else bank4_rows_kernel<DK, 128, PARTS><<<grid, 256, 0, s>>>(a);
+  return MIVOS_OK;
+}
+
+template <int DK>
+static int read_launch(const ReadArgs &a, const ReadPlan &p, int dtype, hipStream_t s) {
+  if (dtype == MIVOS_BF16) return read_launch<DK, 1>(a, p, s);
+  return dtype == MIVOS_F16 ? read_launch<DK, 2>(a, p, s) : read_launch<DK, 3>(a, p, s);
 }
 
 template <int PARTS>
@@ -801,18 +916,13 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   a.slots = bank->slots; a.logit_stride = p.logit_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
   a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
-  a.q_sign = 1.f;
-  if (p.block) {            // logits are compared before they are scaled: a scale above 0 (0 itself as 2^-100: every weight rounds to 1)
-    a.q_sign = scale < 0.f ? -1.f : 1.f;
-    a.scale_log2 = a.scale_log2 * a.q_sign;
-    if (a.scale_log2 < 0x1p-100f) a.scale_log2 = 0x1p-100f;
-  }
+  // logits are compared before they are scaled: a scale above 0, its sign with the queries (0 itself as 2^-100: every weight rounds to 1)
+  a.q_sign = scale < 0.f ? -1.f : 1.f;
+  a.scale_log2 *= a.q_sign;
+  if (a.scale_log2 < 0x1p-100f) a.scale_log2 = 0x1p-100f;
   a.q_vec = (((qb | qt | qh) * dtype_bytes(dtype)) & 15) == 0 && ((uintptr_t)q & 15) == 0;
-#define GO(DK) (p.dvc == 64 ? rows_launch<DK, 64>(a, p, dtype, s) : rows_launch<DK, 128>(a, p, dtype, s))
-  if (bank->key_dim == 64) GO(64);
-  else if (bank->key_dim == 128) GO(128);
-  else GO(256);
-#undef GO
+  if (int rc = bank->key_dim == 64 ? read_launch<64>(a, p, dtype, s) : bank->key_dim == 128 ? read_launch<128>(a, p, dtype, s) : read_launch<256>(a, p, dtype, s))
+    return rc;
   if (int rc = check_launch("bank4_read")) return rc;
   if (!p.parts) return MIVOS_OK;
   const int64_t out_blocks = ((int64_t)a.batch * a.heads * a.rows + 3) / 4;
@@ -823,10 +933,8 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   else join_launch<3>(a, (int)blocks, (int)out_blocks, s);
   if (int rc = check_launch("bank4_read")) return rc;
   if (!a.lse) return MIVOS_OK;
-#define GO(DK) weigh_launch<DK>(a, dtype, s)
-  if (bank->key_dim == 64) GO(64);
-  else if (bank->key_dim == 128) GO(128);
-  else GO(256);
-#undef GO
+  if (bank->key_dim == 64) weigh_launch<64>(a, dtype, s);
+  else if (bank->key_dim == 128) weigh_launch<128>(a, dtype, s);
+  else weigh_launch<256>(a, dtype, s);
   return check_launch("bank4_read");
 }
