@@ -135,7 +135,7 @@ PROTOTYPES = {
     "mivos_norm_rotary_grad": (C.c_int, [C.POINTER(RotaryDesc), vp, vp, vp]),
     "mivos_bank4_append": (C.c_int, [C.POINTER(Bank4Desc), vp, i64, i64, i64, vp, i64, i64, i64, C.c_int, vp, vp, C.c_int, vp]),
     "mivos_bank4_values": (C.c_int, [C.POINTER(Bank4Desc), vp, i64, vp, vp, C.c_int, vp]),
-    "mivos_bank4_read_workspace_bytes": (i64, [C.POINTER(Bank4Desc), C.c_int, C.c_int, C.c_int]),
+    "mivos_bank4_read_workspace_bytes": (i64, [C.POINTER(Bank4Desc), C.c_int, C.c_int, C.c_int, C.c_int]),
     "mivos_bank4_read": (C.c_int, [C.POINTER(Bank4Desc), vp, i64, i64, i64, C.c_int, C.c_int, C.c_int, vp, f32, C.c_int, C.c_int, vp, vp, i64, vp]),
     "mivos_bank4_evict": (C.c_int, [C.POINTER(Bank4Desc), C.POINTER(Bank4Desc), i64, i64, i64, vp, vp]),
     "mivos_interleave_planes": (C.c_int, [C.POINTER(InterleaveDesc), vp, C.c_int, i64, vp]),

@@ -457,10 +457,10 @@ struct QueryCols<DK, 1> {
 // codes straight into registers; the V rows are widened once for the workgroup into one of two LDS buffers while the matrix cores work on
 // the other.  S^T = K Q^T and O^T = V^T P^T on 32x32 products: a lane holds one query, 16 keys of each 32, and these are again the
 // operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^8.
-template <int DK, int DVC, int PARTS>
+template <int DK, int DVC, int PARTS, bool WEIGH>
 __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1) void bank4_block_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
-  constexpr int VS = DVC + 32, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB, VL = (VE + 255) / 256;
+  constexpr int VS = DVC + 16, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB, VL = (VE + 255) / 256;
   extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
@@ -495,7 +495,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   const int v_row = a.value_dim / 2, vs_row = a.value_dim / 32;
   const uint8_t *kc = a.kc + (int64_t)bh * a.slots * (DK / 2), *ks = a.ks + (int64_t)bh * a.slots * (DK / 32);
   const uint8_t *vc = a.vc + (int64_t)bh * a.slots * v_row + chunk * (DVC / 2), *vs = a.vs + (int64_t)bh * a.slots * vs_row + chunk * VB;
-  KeyRow<DK> k[2], kn[2];
+  KeyRow<DK> ka[2], kb[2];
   u32x4 vn[VL];
   uint32_t vsn[VL];
 
@@ -526,71 +526,85 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
     }
   };
 
+  // The logits run one step ahead: their products are issued among the exponentials of the step before, their maximum among its second
+  // products, so that neither pipe waits for the other inside a wave.
+  float top;
+  auto row_top = [&](const f32x16 (&x)[2]) {
+    float t = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+    for (int j = 1; j < 16; ++j) t = fmaxf(fmaxf(t, x[0][j]), x[1][j]);
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * a.scale_log2;
+  };
+  auto settle = [&](f32x16 (&x)[2], int base) {      // masks the logits of a step that not all rows see, moves the maximum if it has to
+    if (base + 64 > low || base + 64 > s1) {
+      const int lim = limit < s1 ? limit : s1;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[s][j] = base + s * 32 + mfma32_row(j, lane) < lim ? x[s][j] : -INFINITY;
+      top = row_top(x);
+    }
+    if (__any(top > m + MAX_LAG)) {
+      const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      l *= alpha;
+      l_used *= alpha;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) o[i] *= alpha;
+    }
+  };
+  auto step = [&](f32x16 (&x)[2], f32x16 (&xn)[2], const KeyRow<DK> (&k)[2], KeyRow<DK> (&kn)[2], int base, const __bf16 *now, __bf16 *then) {
+    load_values(base + 64);                  // (behind the slice: nothing is read, zeros come back)
+    load_keys(kn, base + 128);
+    const float mu = m == -INFINITY ? 0.f : m;
+    xn[0] = q.dot(k[0]);
+    xn[1] = q.dot(k[1]);
+    bf16x8 pf[4][PARTS];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {           // 16 slots: keys 16 s + {0..3, 8..11} + 4 half
+      f32x8 p;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], a.scale_log2, -mu));
+      split8<PARTS>(p, pf[s]);
+      l_used = weight_sum<PARTS>(l_used, p, pf[s][0]);
+      if (PARTS == 1 && WEIGH)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) l += p[j];
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const __bf16 *at = now + (s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32 + 8 * VS));
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int w = 0; w < PARTS; ++w) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s][w], o[i], 0, 0, 0);
+      }
+    }
+    top = row_top(xn);
+    store_values(then);
+    __syncthreads();
+    settle(xn, base + 64);
+  };
+  f32x16 xa[2], xb[2];
   if (s0 < s1) {
-    load_keys(k, s0);
+    load_keys(ka, s0);
     load_values(s0);
+    xa[0] = q.dot(ka[0]);
+    xa[1] = q.dot(ka[1]);
+    load_keys(ka, s0 + 64);
     store_values(vt);
+    top = row_top(xa);
+    settle(xa, s0);
   }
   __syncthreads();
-  int buf = 0;
-  for (int base = s0; base < s1; base += 64, buf ^= 1) {
-    const bool more = base + 64 < s1;
-    if (more) {
-      load_keys(kn, base + 64);
-      load_values(base + 64);
-    }
-    if (base < high) {
-      f32x16 x[2];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) x[s] = q.dot(k[s]);
-      if (base + 64 > low || base + 64 > s1) {
-        const int lim = limit < s1 ? limit : s1;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) x[s][j] = base + s * 32 + mfma32_row(j, lane) < lim ? x[s][j] : -INFINITY;
-      }
-      float top = fmaxf(x[0][0], x[1][0]);
-#pragma unroll
-      for (int j = 1; j < 16; ++j) top = fmaxf(fmaxf(top, x[0][j]), x[1][j]);
-      top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
-      if (__any(top > m + MAX_LAG)) {
-        const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-        m = mn;
-        l *= alpha;
-        l_used *= alpha;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) o[i] *= alpha;
-      }
-      const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {           // 16 slots: keys 16 s + {0..3, 8..11} + 4 half
-        f32x8 p;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], a.scale_log2, -mu));
-        bf16x8 pf[PARTS];
-        split8<PARTS>(p, pf);
-        l_used = weight_sum<PARTS>(l_used, p, pf[0]);
-        if (PARTS == 1 && a.weigh)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) l += p[j];
-        const __bf16 *at = vt + (buf * 64 + s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32));
-          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32 + 8 * VS));
-          const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int w = 0; w < PARTS; ++w) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[w], o[i], 0, 0, 0);
-        }
-      }
-    }
-    if (more) {
-      store_values(vt + (buf ^ 1) * 64 * VS);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) k[s] = kn[s];
-    }
-    __syncthreads();
+  for (int base = s0; base < s1; base += 128) {
+    step(xa, xb, ka, kb, base, vt, vt + 64 * VS);
+    if (base + 64 >= s1) break;
+    step(xb, xa, kb, ka, base + 64, vt + 64 * VS, vt);
   }
   if (PARTS > 1) l = l_used;
   l += __shfl_xor(l, 32);
@@ -801,7 +815,9 @@ static int read_dvc(int dk, int dv, bool block) {
   return dv % 128 ? 64 : 128;
 }
 
-static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, ReadPlan *p) {
+constexpr int block_occupancy(int dk, int dvc, int dtype) { return dtype == MIVOS_BF16 && dk <= 128 && dvc <= 128 ? 2 : 1; }
+
+static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, int dtype, ReadPlan *p) {
   if (q_heads < 1 || q_heads % k->heads || tokens < 0) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: %d query heads over %d bank heads, %d tokens", q_heads, k->heads, tokens);
   if (k->key_dim != 64 && k->key_dim != 128 && k->key_dim != 256) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: keys of %d channels (64, 128 or 256)", k->key_dim);
   if (k->value_dim % 64) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: values of %d channels (a multiple of 64)", k->value_dim);
@@ -814,11 +830,13 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, R
   p->nvc = k->value_dim / p->dvc;
   const int64_t groups = (int64_t)p->tiles * k->batch * k->heads * p->nvc;
   if (p->block) {
-    // slices of a row tile's slots: the fewest rounds of the 512 workgroups that run at once, a slice costing its join (~3 % of a round)
+    // Slices of a row tile's slots: the fewest rounds of the workgroups that run at once (two a CU where their registers allow it), a slice
+    // costing its join (its accumulators are written and read once more) and its start.
+    const int at_once = 256 * block_occupancy(k->key_dim, p->dvc, dtype);
     const int most = (int)(k->slots / 512 < 1 ? 1 : k->slots / 512 > 32 ? 32 : k->slots / 512);
     double best = 1e30;
     for (int n = 1; n <= most; ++n) {
-      const double cost = (double)((groups * n + 511) / 512) / n + 0.03 * n;
+      const double cost = (double)((groups * n + at_once - 1) / at_once) / n * (1 + 0.01 * n);
       if (cost < best - 1e-9) { best = cost; p->nsplit = n; }
     }
   } else {
@@ -836,15 +854,23 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, R
   return MIVOS_OK;
 }
 
-template <int DK, int DVC, int PARTS>
-static int block_launch(const ReadArgs &a, const dim3 grid, hipStream_t s) {
-  constexpr size_t lds = 2 * 64 * (DVC + 32) * 2;
+template <int DK, int DVC, int PARTS, bool WEIGH>
+static int block_launch_one(const ReadArgs &a, const dim3 grid, hipStream_t s) {
+  constexpr size_t lds = 2 * 64 * (DVC + 16) * 2;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
-    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS>, lds, raised, "bank4_read")) return rc;
+    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, WEIGH>, lds, raised, "bank4_read")) return rc;
   }
-  bank4_block_kernel<DK, DVC, PARTS><<<grid, 256, lds, s>>>(a);
+  bank4_block_kernel<DK, DVC, PARTS, WEIGH><<<grid, 256, lds, s>>>(a);
   return MIVOS_OK;
+}
+
+// (only rounded weights need a second sum: with 2 or 3 parts the one in use is exact)
+template <int DK, int DVC, int PARTS>
+static int block_launch(const ReadArgs &a, const dim3 grid, hipStream_t s) {
+  if constexpr (PARTS == 1)
+    if (a.weigh) return block_launch_one<DK, DVC, 1, true>(a, grid, s);
+  return block_launch_one<DK, DVC, PARTS, false>(a, grid, s);
 }
 
 template <int DK, int PARTS>
@@ -886,10 +912,10 @@ static void weigh_launch(const ReadArgs &a, int dtype, hipStream_t s) {
 
 using namespace mivos;
 
-extern "C" int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int q_heads, int tokens, int weigh) {
+extern "C" int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int q_heads, int tokens, int dtype, int weigh) {
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
-  if (int rc = read_plan(bank, q_heads, tokens, weigh, &p)) return rc;
+  if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
   return p.part_o + p.part_ml + p.logits + p.lse;
 }
 
@@ -899,7 +925,7 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
   if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out))) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument");
-  if (int rc = read_plan(bank, q_heads, tokens, weigh, &p)) return rc;
+  if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
   if (p.rows == 0) return MIVOS_OK;
   const int64_t need = p.part_o + p.part_ml + p.logits + p.lse;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))

@@ -1334,7 +1334,7 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
     if count is not None:
         _int32_vector(count, b, "count")
     lib = _lib.load()
-    need = lib.mivos_bank4_read_workspace_bytes(bank._desc, hq, t, weigh)
+    need = lib.mivos_bank4_read_workspace_bytes(bank._desc, hq, t, code, weigh)
     if need < 0:
         check(int(need))
     _here(bank.lens, queries, count)

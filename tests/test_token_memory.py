@@ -133,9 +133,9 @@ def test_c_entries_check_their_arguments_without_a_gpu():
     lib = _lib.load()
     b = _bank()
     d = b._desc
-    assert lib.mivos_bank4_read_workspace_bytes(d, 3, 1, 0) == -1 and b"query heads" in lib.mivos_last_error()
-    assert lib.mivos_bank4_read_workspace_bytes(d, 4, 5, 1) >= 2 * 2 * 10 * 64 * 4
-    assert lib.mivos_bank4_read_workspace_bytes(None, 4, 5, 1) == -1
+    assert lib.mivos_bank4_read_workspace_bytes(d, 3, 1, 0, 0) == -1 and b"query heads" in lib.mivos_last_error()
+    assert lib.mivos_bank4_read_workspace_bytes(d, 4, 5, 0, 1) >= 2 * 2 * 10 * 64 * 4
+    assert lib.mivos_bank4_read_workspace_bytes(None, 4, 5, 0, 1) == -1
     assert lib.mivos_bank4_read(d, 1, 0, 0, 0, 0, 4, 5, None, 1.0, 0, 1, 1, None, 0, None) == -1 and b"workspace" in lib.mivos_last_error()
     assert lib.mivos_bank4_append(d, None, 0, 0, 0, None, 0, 0, 0, 0, None, None, 1, None) == -1
     assert lib.mivos_bank4_append(d, 1, 0, 0, 0, 1, 0, 0, 0, 7, 1, None, 1, None) == -1
