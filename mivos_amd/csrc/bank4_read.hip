@@ -26,8 +26,9 @@ struct ReadArgs {
   void *out;
   int64_t qb, qt, qh;
   float *part_o, *part_ml, *logits, *lse;
-  int64_t slots, logit_stride;
-  int batch, heads, group, tokens, rows, value_dim, nsplit, causal, weigh, q_vec;
+  __bf16 *q_pack;
+  int64_t slots, logit_stride, lse_stride;
+  int batch, heads, group, tokens, rows, key_dim, value_dim, nsplit, causal, weigh, q_vec;
   float scale_log2;       // |scale| * log2(e): the softmax runs in powers of two; the sign of scale goes to the queries
   float q_sign;
 };
@@ -636,16 +637,18 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
 }
 
 // weight[s] += sum over the rows of exp2(logit - lse[row]): the logits once more, now S = Q K^T, so that a lane holds one slot and its sum
-// runs over registers.  One workgroup: NS x 32 slots, their keys widened once into registers; the waves take 32 rows in turn.
-template <int DK, int PARTS>
+// runs over registers, the rows in order.  One workgroup: 128 * NS slots, NS x 32 a wave, their keys widened once into registers; 32 rows a
+// step go through LDS, copied as bank4_join has packed them in operand order.  (A wave that reads its rows as they lie in memory touches a
+// cache line a lane and load, and with 64 slots a workgroup the queries cross the L2 1.3 GB at 1620 x 32 400 x 2: 150 and 115 us.)
+template <int DK, int PARTS, int NS>
 __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
-  typedef typename ReadType<PARTS>::T T;
-  constexpr int NS = DK <= 128 ? 4 : 2, KS = DK / 16;
-  __shared__ float sums[4][NS * 32];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-  const int bh = blockIdx.y, b = bh / a.heads, h = bh - b * a.heads, base = blockIdx.x * NS * 32;
+  constexpr int KS = DK / 16, TILE = KS * PARTS * 64, TL = TILE / 256;       // 16-byte words a tile, a thread
+  extern __shared__ __align__(16) u32x4 qs[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+  const int bh = blockIdx.y, b = bh / a.heads, first = blockIdx.x * (128 * NS), base = first + wave * (32 * NS);
   const int len = (int)read_len(a, b), cnt = read_count(a, b);
-  if (base >= len) return;
+  const int rows = cnt * a.group;                       // (rows behind the count have no weight)
+  if (first >= len || rows == 0) return;
   const int64_t row_base = (int64_t)bh * a.slots;
   const auto rk = bank_rows(a.kc + (row_base + base) * (DK / 2), (int64_t)(len - base) * (DK / 2));
   const auto rs = bank_rows(a.ks + (row_base + base) * (DK / 32), (int64_t)(len - base) * (DK / 32));
@@ -662,50 +665,66 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   float acc[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) acc[s] = 0.f;
-  const int rows = cnt * a.group < a.rows ? cnt * a.group : a.rows;       // rows behind the count have no weight
-  for (int r0 = wave * 32; r0 < rows; r0 += 128) {
-    if (a.causal && read_limit(a, len, cnt, (r0 + 31 < rows ? r0 + 31 : rows - 1) / a.group) <= base) continue;
-    const int r = r0 + col, t = r / a.group;
-    const bool live = r < rows;
-    const T *qrow = (const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh;
+  const u32x4 *q = reinterpret_cast<const u32x4 *>(a.q_pack) + (int64_t)bh * (a.lse_stride / 32) * TILE + tid;
+  const float *lse = a.lse + (int64_t)bh * a.lse_stride + half * 4;          // (rows behind the last hold anything: not added)
+  const int tiles = (rows + 31) / 32;
+  int tile0 = 0;                                        // causal: the first rows that see the workgroup's first slot
+  if (a.causal) {
+    const int64_t t0 = (int64_t)first - len + cnt;      // token t sees slots < len - cnt + t + 1
+    tile0 = t0 > 0 ? (int)(t0 * a.group / 32) : 0;
+  }
+  u32x4 next[TL];
+#pragma unroll
+  for (int i = 0; i < TL; ++i) qs[i * 256 + tid] = q[(int64_t)tile0 * TILE + i * 256];
+  __syncthreads();
+  for (int tile = tile0, buf = 0; tile < tiles; ++tile, buf ^= 1) {
+    const int more = tile + 1 < tiles ? tile + 1 : tile;
+#pragma unroll
+    for (int i = 0; i < TL; ++i) next[i] = q[(int64_t)more * TILE + i * 256];
+    const int r0 = tile * 32;
+    f32x4 shift[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) shift[g] = *reinterpret_cast<const f32x4 *>(lse + r0 + g * 8);
     f32x16 x[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[s][j] = 0.f;
+    const bf16x8 *qt = reinterpret_cast<const bf16x8 *>(qs) + buf * TILE + lane;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      f32x8 y = load8(qrow + (i / 4) * 64 + half * 32 + (i & 3) * 8, a.q_vec);
+    for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = live ? y[j] * a.q_sign : 0.f;
-      bf16x8 qf[PARTS];
-      split8<PARTS>(y, qf);
+      for (int p = 0; p < PARTS; ++p) {
+        const bf16x8 qf = qt[(i * PARTS + p) * 64];
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) x[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[p], kf[s][i], x[s], 0, 0, 0);
-    }
-    const bool edge = a.causal || r0 + 32 > rows;
-    const float *lse = a.lse + (int64_t)bh * a.rows + r0;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int rr = mfma32_row(j, lane), row = r0 + rr;
-      const float shift = lse[row < rows ? rr : rows - 1 - r0];
-      const int lim = !edge ? len : row < rows ? (int)read_limit(a, len, cnt, row / a.group) : 0;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift));
-        acc[s] += base + s * 32 + col < lim ? p : 0.f;
+        for (int s = 0; s < NS; ++s) x[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[s][i], x[s], 0, 0, 0);
       }
+    if (r0 + 32 > rows || (a.causal && read_limit(a, len, cnt, r0 / a.group) < base + 32 * NS)) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int row = r0 + mfma32_row(j, lane), lim = row < rows ? (int)read_limit(a, len, cnt, row / a.group) : 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4]));
+          acc[s] += base + s * 32 + col < lim ? p : 0.f;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) acc[s] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4]));
     }
+#pragma unroll
+    for (int i = 0; i < TL; ++i) qs[(buf ^ 1) * TILE + i * 256 + tid] = next[i];
+    __syncthreads();
   }
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     acc[s] += __shfl_xor(acc[s], 32);
-    if (half == 0) sums[wave][s * 32 + col] = acc[s];
+    const int slot = base + s * 32 + col;
+    if (half == 0 && slot < len) a.weight[row_base + slot] += acc[s];
   }
-  __syncthreads();
-  if (tid < NS * 32 && base + tid < len) a.weight[row_base + base + tid] += sums[0][tid] + sums[1][tid] + sums[2][tid] + sums[3][tid];
 }
 
 // A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum and log2 of the sum of the weights, and the
@@ -736,7 +755,8 @@ struct RowJoin {
 };
 
 // Joins the slices of a row (first `out_blocks` workgroups, one wave a row; QL lanes cover the value channels, 64 / QL slices at a time)
-// and adds the rows' weights to the slots (the others, 1024 slots each, the rows in order: the sum does not depend on timing).
+// and adds the rows' weights to the slots (the others, 1024 slots each, the rows in order: the sum does not depend on timing) or, ahead of
+// bank4_weigh, packs its queries.
 template <int PARTS, int QL>
 __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blocks) {
   typedef typename ReadType<PARTS>::T T;
@@ -746,7 +766,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
     if (g >= (int64_t)a.batch * a.heads * a.rows) return;
     const int bh = (int)(g / a.rows), row = (int)(g - (int64_t)bh * a.rows), b = bh / a.heads, h = bh - b * a.heads;
     const RowJoin J(a, bh, row, lane);
-    if (a.lse && lane == 0) a.lse[g] = J.lse;
+    if (a.lse && lane == 0) a.lse[(int64_t)bh * a.lse_stride + row] = J.lse;
     const int t = row / a.group, j = h * a.group + row - t * a.group;
     T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + j) * a.value_dim;
     const float *part = a.part_o + ((int64_t)bh * a.nsplit * a.rows + row) * a.value_dim;
@@ -770,6 +790,26 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
         for (int c = 0; c < 4; ++c) y[c] = (T)(J.inv == 0.f ? 0.f : acc[c] * J.inv);
         *reinterpret_cast<Tx4 *>(out + dv) = y;
       }
+    }
+    return;
+  }
+  if (a.q_pack) {                     // 32 rows a wave, as bf16 parts in the order of bank4_weigh's operand
+    const int tiles = (int)(a.lse_stride / 32), KS = a.key_dim / 16;
+    const int64_t g = (int64_t)(blockIdx.x - out_blocks) * 4 + wave;
+    if (g >= (int64_t)a.batch * a.heads * tiles) return;
+    const int bh = (int)(g / tiles), tile = (int)(g - (int64_t)bh * tiles), b = bh / a.heads, h = bh - b * a.heads, half = lane >> 5;
+    const int r = tile * 32 + (lane & 31), t = r / a.group;
+    const bool live = r < a.rows && t < read_count(a, b);
+    const T *row = (const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh;
+    bf16x8 *to = reinterpret_cast<bf16x8 *>(a.q_pack) + g * (KS * PARTS * 64) + lane;
+    for (int i = 0; i < KS; ++i) {
+      f32x8 y = load8(row + (i / 4) * 64 + half * 32 + (i & 3) * 8, a.q_vec);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) y[c] = live ? y[c] * a.q_sign : 0.f;
+      bf16x8 qf[PARTS];
+      split8<PARTS>(y, qf);
+#pragma unroll
+      for (int p = 0; p < PARTS; ++p) to[(i * PARTS + p) * 64] = qf[p];
     }
     return;
   }
@@ -805,7 +845,7 @@ struct ReadPlan {
   int rows, tiles, nsplit, nvc, dvc;
   bool block;                        // 128 rows a workgroup (else 16)
   bool parts;                        // partial results go through the workspace
-  int64_t part_o, part_ml, logits, lse, logit_stride;      // bytes
+  int64_t part_o, part_ml, logits, lse, q_pack, logit_stride, lse_stride;      // bytes; strides in elements
 };
 
 
@@ -850,7 +890,9 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   p->part_ml = p->parts ? n * 16 : 0;
   p->logit_stride = (k->slots + 63) / 64 * 64;
   p->logits = weigh && !p->block ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
-  p->lse = weigh && p->block ? (int64_t)k->batch * k->heads * rows * 4 : 0;
+  p->lse_stride = (rows + 31) / 32 * 32;
+  p->lse = weigh && p->block ? (int64_t)k->batch * k->heads * p->lse_stride * 4 : 0;
+  p->q_pack = p->lse / 4 * k->key_dim * 2 * (dtype == MIVOS_BF16 ? 1 : dtype == MIVOS_F16 ? 2 : 3);
   return MIVOS_OK;
 }
 
@@ -899,13 +941,27 @@ static void join_launch(const ReadArgs &a, int blocks, int out_blocks, hipStream
   else bank4_join_kernel<PARTS, 64><<<blocks, 256, 0, s>>>(a, out_blocks);
 }
 
+template <int DK, int PARTS, int NS>
+static int weigh_launch_one(const ReadArgs &a, hipStream_t s) {
+  constexpr size_t lds = 2 * (DK / 16) * PARTS * 64 * 16;
+  if constexpr (lds > 65536) {
+    static std::atomic<uint64_t> raised{0};
+    if (int rc = ensure_dynamic_lds((const void *)bank4_weigh_kernel<DK, PARTS, NS>, lds, raised, "bank4_read")) return rc;
+  }
+  bank4_weigh_kernel<DK, PARTS, NS><<<dim3(cdiv(a.slots, 128 * NS), a.batch * a.heads), 256, lds, s>>>(a);
+  return MIVOS_OK;
+}
+
+// 256 slots a workgroup where that still gives every CU one; else 128
+template <int DK, int PARTS>
+static int weigh_launch(const ReadArgs &a, hipStream_t s) {
+  if (a.batch * a.heads * (a.slots / 256) >= 240) return weigh_launch_one<DK, PARTS, 2>(a, s);
+  return weigh_launch_one<DK, PARTS, 1>(a, s);
+}
+
 template <int DK>
-static void weigh_launch(const ReadArgs &a, int dtype, hipStream_t s) {
-  constexpr int keys = DK <= 128 ? 128 : 64;
-  const dim3 grid(cdiv(a.slots, keys), a.batch * a.heads);
-  if (dtype == MIVOS_BF16) bank4_weigh_kernel<DK, 1><<<grid, 256, 0, s>>>(a);
-  else if (dtype == MIVOS_F16) bank4_weigh_kernel<DK, 2><<<grid, 256, 0, s>>>(a);
-  else bank4_weigh_kernel<DK, 3><<<grid, 256, 0, s>>>(a);
+static int weigh_launch(const ReadArgs &a, int dtype, hipStream_t s) {
+  return dtype == MIVOS_BF16 ? weigh_launch<DK, 1>(a, s) : dtype == MIVOS_F16 ? weigh_launch<DK, 2>(a, s) : weigh_launch<DK, 3>(a, s);
 }
 
 }  // namespace mivos
@@ -916,7 +972,7 @@ extern "C" int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
-  return p.part_o + p.part_ml + p.logits + p.lse;
+  return p.part_o + p.part_ml + p.logits + p.lse + p.q_pack;
 }
 
 extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t qb, int64_t qt, int64_t qh, int dtype, int q_heads, int tokens,
@@ -927,7 +983,7 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out))) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument");
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
   if (p.rows == 0) return MIVOS_OK;
-  const int64_t need = p.part_o + p.part_ml + p.logits + p.lse;
+  const int64_t need = p.part_o + p.part_ml + p.logits + p.lse + p.q_pack;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: workspace of %lld bytes, 16-byte aligned", (long long)need);
   if (p.tiles > 65535 || (int64_t)bank->batch * bank->heads * p.nvc > 65535) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many row tiles");
@@ -938,10 +994,10 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   char *ws = (char *)workspace;
   if (p.parts) { a.part_o = (float *)ws; a.part_ml = (float *)(ws + p.part_o); }
   if (p.logits) a.logits = (float *)(ws + p.part_o + p.part_ml);
-  if (p.lse) a.lse = (float *)(ws + p.part_o + p.part_ml);
-  a.slots = bank->slots; a.logit_stride = p.logit_stride;
+  if (p.lse) { a.lse = (float *)(ws + p.part_o + p.part_ml); a.q_pack = (__bf16 *)(ws + p.part_o + p.part_ml + p.lse); }
+  a.slots = bank->slots; a.logit_stride = p.logit_stride; a.lse_stride = p.lse_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
-  a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
+  a.key_dim = bank->key_dim; a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
   // logits are compared before they are scaled: a scale above 0, its sign with the queries (0 itself as 2^-100: every weight rounds to 1)
   a.q_sign = scale < 0.f ? -1.f : 1.f;
   a.scale_log2 *= a.q_sign;
@@ -952,15 +1008,15 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (int rc = check_launch("bank4_read")) return rc;
   if (!p.parts) return MIVOS_OK;
   const int64_t out_blocks = ((int64_t)a.batch * a.heads * a.rows + 3) / 4;
-  const int64_t blocks = out_blocks + (a.logits ? (int64_t)a.batch * a.heads * ((a.slots + 1023) / 1024) : 0);
+  int64_t blocks = out_blocks + (a.logits ? (int64_t)a.batch * a.heads * ((a.slots + 1023) / 1024) : 0);
+  if (a.q_pack) blocks += (a.batch * a.heads * (a.lse_stride / 32) + 3) / 4;
   if (blocks > 0x7fffffff) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many rows");
   if (dtype == MIVOS_BF16) join_launch<1>(a, (int)blocks, (int)out_blocks, s);
   else if (dtype == MIVOS_F16) join_launch<2>(a, (int)blocks, (int)out_blocks, s);
   else join_launch<3>(a, (int)blocks, (int)out_blocks, s);
   if (int rc = check_launch("bank4_read")) return rc;
   if (!a.lse) return MIVOS_OK;
-  if (bank->key_dim == 64) weigh_launch<64>(a, dtype, s);
-  else if (bank->key_dim == 128) weigh_launch<128>(a, dtype, s);
-  else weigh_launch<256>(a, dtype, s);
+  if (int rc = bank->key_dim == 64 ? weigh_launch<64>(a, dtype, s) : bank->key_dim == 128 ? weigh_launch<128>(a, dtype, s) : weigh_launch<256>(a, dtype, s))
+    return rc;
   return check_launch("bank4_read");
 }
