@@ -558,6 +558,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   auto step = [&](f32x16 (&x)[2], f32x16 (&xn)[2], const KeyRow<DK> (&k)[2], KeyRow<DK> (&kn)[2], int base, const __bf16 *now, __bf16 *then) {
     load_values(base + 64);                  // (behind the slice: nothing is read, zeros come back)
     load_keys(kn, base + 128);
+
     const float mu = m == -INFINITY ? 0.f : m;
     xn[0] = q.dot(k[0]);
     xn[1] = q.dot(k[1]);
