@@ -112,26 +112,33 @@ __global__ __launch_bounds__(256) void bank4_values_kernel(mivos_bank4 bank, con
 }
 
 // ---------------------------------------------------------------------------------------------- evict
-// Order of the weights as unsigned integers: larger weight, larger key; NaN lowest; -0 = +0.
+// Order of the weights as unsigned integers: larger weight, larger key; NaN lowest; -0 = +0.  From 1 (NaN) to 0xff800000 (infinity): 0 is left
+// for what is no slot, KEY_STAYS for what is protected.
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (w != w) return 0u;
+  if (w != w) return 1u;
   const uint32_t b = __float_as_uint(w + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t KEY_STAYS = 0xffffffffu;
 
-constexpr int EVICT_THREADS = 1024;
+constexpr int EVICT_THREADS = 1024, EVICT_WAVES = EVICT_THREADS / 64, EVICT_BINS = 2048, EVICT_COPIES = 4;
+constexpr int EVICT_KEYS = 32;      // keys a lane holds: banks of up to 32 768 slots are read once
 
-// Which slots of one (stream, head) stay: a radix select of the keep-th largest key among the unprotected slots (four passes of
-// 8 bits, the counts in LDS), then one ordered pass that writes the kept slots ascending.  Equal weights: the lowest slots stay.
+// Which slots of one (stream, head) stay: a radix select of the keep-th largest key (protected slots have the largest), 11 + 11 + 10 bits, the
+// counts in LDS (four copies: most weights of a bank share a few exponents, and a bin's increments are serial), then one ordered pass that
+// writes the kept slots ascending.  Equal weights: the lowest slots stay.  A wave owns a run of slots, so a slot's place follows from ballots
+// of its wave and one sum over the waves before: (larger keys before it) + min(equal ones before it, equal ones that stay).
+// One workgroup a (stream, head): bound by latency, 12 barriers and three passes of LDS counts (@@ us at 21 060 slots; slots visited one
+// 1024-wide row at a time with a scan each, and 8-bit digits, took 49 us).
+template <bool REGS>
 __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float *__restrict__ weight, const int32_t *__restrict__ lens, int heads, int64_t slots,
                                                                     int keep, int first, int recent, int32_t *__restrict__ slots_out,
                                                                     int32_t *__restrict__ lens_out) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t chosen[2];
-  __shared__ int base[2];
-  __shared__ int wave_kept[EVICT_THREADS / 64], wave_ties[EVICT_THREADS / 64];
+  __shared__ uint32_t hist[EVICT_COPIES][EVICT_BINS];
+  __shared__ uint32_t sums[EVICT_WAVES], chosen[2];
+  __shared__ int larger[EVICT_WAVES], equal[EVICT_WAVES];
   const int bh = blockIdx.x, b = bh / heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int64_t n64 = lens[b];
+  const int64_t n64 = lens[b];
   const int n = (int)(n64 < 0 ? 0 : n64 > slots ? slots : n64);
   const float *w = weight + (int64_t)bh * slots;
   int32_t *out = slots_out + (int64_t)bh * keep;
@@ -141,93 +148,136 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
     for (int i = tid; i < keep; i += EVICT_THREADS) out[i] = i < n ? i : -1;
     return;
   }
-  const int lo = first, hi = n - recent;                             // unprotected slots [lo, hi); first + recent <= keep < n
-  int want = keep - first - recent;                                  // of which this many stay
-  uint32_t prefix = 0, mask = 0;
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    for (int i = tid; i < 256; i += EVICT_THREADS) hist[i] = 0;
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += EVICT_THREADS) {
-      const uint32_t k = weight_key(w[i]);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+  const int hi = n - recent;                                         // slots [0, first) and [hi, n) are protected; first + recent <= keep < n
+  int want = keep;
+  const int rounds = (n + EVICT_THREADS - 1) / EVICT_THREADS, run = rounds * 64, base = wave * run + lane;     // the wave's slots: base + 64 j, j < rounds
+  uint32_t held[REGS ? EVICT_KEYS : 1];
+  auto slot_weight = [&](int j) { const int i = base + j * 64; return w[i < n ? i : n - 1]; };      // (no branch: all loads go out together)
+  auto slot_key = [&](int j, float x) {
+    const int i = base + j * 64;
+    return i >= n ? 0u : i < first || i >= hi ? KEY_STAYS : weight_key(x);
+  };
+  if constexpr (REGS) {
+    float x[EVICT_KEYS];
+#pragma unroll
+    for (int j = 0; j < EVICT_KEYS; ++j) x[j] = slot_weight(j < rounds ? j : 0);
+#pragma unroll
+    for (int j = 0; j < EVICT_KEYS; ++j) held[j] = slot_key(j, x[j]);
+  }
+  auto each = [&](auto &&use) {      // use(slot, key) for the wave's slots in order; every lane takes part in every call
+    if constexpr (REGS) {
+#pragma unroll
+      for (int j = 0; j < EVICT_KEYS; ++j)
+        if (j < rounds) use(base + j * 64, held[j]);
+    } else {
+      for (int j = 0; j < rounds; j += 8) {
+        float x[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x[c] = slot_weight(j + c < rounds ? j + c : 0);
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (j + c < rounds) use(base + (j + c) * 64, slot_key(j + c, x[c]));
+      }
     }
+  };
+  uint32_t prefix = 0, mask = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    for (int i = tid; i < EVICT_COPIES * EVICT_BINS; i += EVICT_THREADS) (&hist[0][0])[i] = 0;
     __syncthreads();
-    if (tid < 64) {                                                  // lane l: bins 255 - 4l .. 252 - 4l, from the top
-      uint32_t c[4], sum = 0;
+    each([&](int i, uint32_t k) {
+      if ((k & mask) == prefix) atomicAdd(&hist[wave % EVICT_COPIES][(k >> shift) & (bins - 1)], 1u);
+    });
+    __syncthreads();
+    // thread t: bins 2 t, 2 t + 1 counted from the top
+    uint32_t c[2], sum = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += c[j] = hist[255 - 4 * tid - j];
-      uint32_t before = sum;
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(before, d);
-        if (tid >= d) before += o;
-      }
-      before -= sum;
+    for (int j = 0; j < 2; ++j) {
+      const int bin = bins - 1 - (2 * tid + j);
+      c[j] = 0;
+      if (bin >= 0)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (before < (uint32_t)want && (uint32_t)want <= before + c[j]) { chosen[0] = 255 - 4 * tid - j; chosen[1] = before; }
-        before += c[j];
-      }
+        for (int v = 0; v < EVICT_COPIES; ++v) c[j] += hist[v][bin];
+      sum += c[j];
+    }
+    uint32_t before = sum;
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(before, d);
+      if (lane >= d) before += o;
+    }
+    if (lane == 63) sums[wave] = before;
+    __syncthreads();
+    before -= sum;
+    for (int v = 0; v < wave; ++v) before += sums[v];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (before < (uint32_t)want && (uint32_t)want <= before + c[j]) { chosen[0] = bins - 1 - (2 * tid + j); chosen[1] = before; }
+      before += c[j];
     }
     __syncthreads();
     prefix |= chosen[0] << shift;
-    mask |= 255u << shift;
+    mask |= (uint32_t)(bins - 1) << shift;
     want -= (int)chosen[1];
-    __syncthreads();
   }
   // now: keys above `prefix` stay, and the first `want` of those equal to it
-  const bool any = keep - first - recent > 0;
-  if (tid == 0) base[0] = base[1] = 0;
+  int n_larger = 0, n_equal = 0;
+  each([&](int, uint32_t k) {
+    n_larger += __popcll(__ballot(k > prefix));
+    n_equal += __popcll(__ballot(k == prefix));
+  });
+  if (lane == 0) { larger[wave] = n_larger; equal[wave] = n_equal; }
   __syncthreads();
-  for (int i0 = 0; i0 < n; i0 += EVICT_THREADS) {
-    const int i = i0 + tid;
-    bool stays = false, tie = false;
-    if (i < n) {
-      if (i < lo || i >= hi) stays = true;
-      else if (any) {
-        const uint32_t k = weight_key(w[i]);
-        stays = k > prefix;
-        tie = k == prefix;
-      }
-    }
-    const uint64_t below = (1ull << lane) - 1;
-    const uint64_t ties = __ballot(tie);
-    if (lane == 0) wave_ties[wave] = __popcll(ties);
-    __syncthreads();
-    int tie_rank = base[1] + __popcll(ties & below);
-    for (int v = 0; v < wave; ++v) tie_rank += wave_ties[v];
-    stays |= tie && tie_rank < want;
-    const uint64_t kept = __ballot(stays);
-    if (lane == 0) wave_kept[wave] = __popcll(kept);
-    __syncthreads();
-    int rank = base[0] + __popcll(kept & below);
-    for (int v = 0; v < wave; ++v) rank += wave_kept[v];
-    if (stays) out[rank] = i;
-    __syncthreads();
-    if (tid == 0)
-      for (int v = 0; v < EVICT_THREADS / 64; ++v) { base[0] += wave_kept[v]; base[1] += wave_ties[v]; }
-    __syncthreads();
-  }
+  n_larger = n_equal = 0;
+  for (int v = 0; v < wave; ++v) { n_larger += larger[v]; n_equal += equal[v]; }
+  each([&](int i, uint32_t k) {
+    const uint64_t ba = __ballot(k > prefix), bt = __ballot(k == prefix);
+    const int ties = n_equal + __builtin_amdgcn_mbcnt_hi((uint32_t)(bt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bt, 0));
+    const int place = n_larger + __builtin_amdgcn_mbcnt_hi((uint32_t)(ba >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ba, 0)) + (ties < want ? ties : want);
+    if (k > prefix || (k == prefix && ties < want)) out[place] = i;
+    n_larger += __popcll(ba);
+    n_equal += __popcll(bt);
+  });
 }
 
-// Moves the kept rows: one thread a 4-byte word of codes; the scales and the weight go with the row's first threads.
+// Moves the kept rows: a thread a block of 32 channels, 16 bytes of codes; every fourth the scales of four blocks (WIDE: both rows have a
+// multiple of 128 channels; else each its own), the first the weight.  Four rows in flight a thread.
+template <bool WIDE>
 __global__ __launch_bounds__(256) void bank4_move_kernel(mivos_bank4 from, mivos_bank4 to, int keep, const int32_t *__restrict__ slots) {
   const int bh = blockIdx.y;
-  const int ku = from.key_dim / 8, units = ku + from.value_dim / 8;
-  const int64_t total = (int64_t)keep * units;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const uint32_t j = (uint32_t)(i / units);
-    int u = (int)(i - (int64_t)j * units);
-    const int32_t slot = slots[(int64_t)bh * keep + j];
-    if (slot < 0) continue;
-    const int64_t src = (int64_t)bh * from.slots + slot, dst = (int64_t)bh * to.slots + j;
-    if (u == 0) to.weight[dst] = from.weight[src];
-    const bool is_key = u < ku;
-    u = is_key ? u : u - ku;
-    const int dim = is_key ? from.key_dim : from.value_dim;
-    const uint8_t *sc = is_key ? from.key_codes : from.value_codes, *ss = is_key ? from.key_scales : from.value_scales;
-    uint8_t *dc = is_key ? to.key_codes : to.value_codes, *ds = is_key ? to.key_scales : to.value_scales;
-    reinterpret_cast<uint32_t *>(dc + dst * (dim / 2))[u] = reinterpret_cast<const uint32_t *>(sc + src * (dim / 2))[u];
-    if ((u & 3) == 0) ds[dst * (dim / 32) + (u >> 2)] = ss[src * (dim / 32) + (u >> 2)];
+  const int kb = from.key_dim / 32, vb = from.value_dim / 32, units = kb + vb, rows = 256 / units;      // units <= 64
+  const int u = threadIdx.x % units, r = threadIdx.x / units;
+  if (r >= rows) return;
+  const bool is_key = u < kb;
+  const int blk = is_key ? u : u - kb, nb = is_key ? kb : vb;
+  const u32x4 *sc = reinterpret_cast<const u32x4 *>(is_key ? from.key_codes : from.value_codes) + (int64_t)bh * from.slots * nb + blk;
+  const uint8_t *ss = (is_key ? from.key_scales : from.value_scales) + (int64_t)bh * from.slots * nb + blk;
+  u32x4 *dc = reinterpret_cast<u32x4 *>(is_key ? to.key_codes : to.value_codes) + (int64_t)bh * to.slots * nb + blk;
+  uint8_t *ds = (is_key ? to.key_scales : to.value_scales) + (int64_t)bh * to.slots * nb + blk;
+  const int32_t *from_slot = slots + (int64_t)bh * keep;
+  const int stride = gridDim.x * rows;
+  for (int64_t j0 = (int64_t)blockIdx.x * rows + r; j0 < keep; j0 += 4 * (int64_t)stride) {
+    int32_t slot[4];
+    u32x4 codes[4];
+    uint32_t scale[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) slot[c] = j0 + c * (int64_t)stride < keep ? from_slot[j0 + c * (int64_t)stride] : -1;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (slot[c] >= 0) {
+        codes[c] = sc[(int64_t)slot[c] * nb];
+        if (!WIDE) scale[c] = ss[(int64_t)slot[c] * nb];
+        else if ((blk & 3) == 0) scale[c] = *reinterpret_cast<const uint32_t *>(ss + (int64_t)slot[c] * nb);
+      }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (slot[c] >= 0) {
+        const int64_t j = j0 + c * (int64_t)stride;
+        dc[j * nb] = codes[c];
+        if (!WIDE) ds[j * nb] = (uint8_t)scale[c];
+        else if ((blk & 3) == 0) *reinterpret_cast<uint32_t *>(ds + j * nb) = scale[c];
+        if (u == 0) to.weight[(int64_t)bh * to.slots + j] = from.weight[(int64_t)bh * from.slots + slot[c]];
+      }
   }
 }
 
@@ -281,10 +331,15 @@ extern "C" int mivos_bank4_evict(const mivos_bank4 *bank, const mivos_bank4 *out
   if (keep < 1 || keep > out->slots || first < 0 || recent < 0 || first + recent > keep || !slots_out)
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_evict: keep %lld of %lld slots, first %lld, recent %lld", (long long)keep, (long long)out->slots,
                 (long long)first, (long long)recent);
-  const int rows = bank->batch * bank->heads, units = (bank->key_dim + bank->value_dim) / 8;
+  const int rows = bank->batch * bank->heads, a_row = 256 / ((bank->key_dim + bank->value_dim) / 32);
   hipStream_t s = (hipStream_t)stream;
-  bank4_select_kernel<<<rows, EVICT_THREADS, 0, s>>>(bank->weight, bank->lens, bank->heads, bank->slots, (int)keep, (int)first, (int)recent, slots_out, out->lens);
+  if (bank->slots <= EVICT_THREADS * EVICT_KEYS)
+    bank4_select_kernel<true><<<rows, EVICT_THREADS, 0, s>>>(bank->weight, bank->lens, bank->heads, bank->slots, (int)keep, (int)first, (int)recent, slots_out, out->lens);
+  else
+    bank4_select_kernel<false><<<rows, EVICT_THREADS, 0, s>>>(bank->weight, bank->lens, bank->heads, bank->slots, (int)keep, (int)first, (int)recent, slots_out, out->lens);
   if (int rc = check_launch("bank4_evict")) return rc;
-  bank4_move_kernel<<<dim3(grid_x(keep * units, rows), rows), 256, 0, s>>>(*bank, *out, (int)keep, slots_out);
+  const dim3 grid(grid_x(keep * 64 / a_row, rows), rows);
+  if (bank->key_dim % 128 == 0 && bank->value_dim % 128 == 0) bank4_move_kernel<true><<<grid, 256, 0, s>>>(*bank, *out, (int)keep, slots_out);
+  else bank4_move_kernel<false><<<grid, 256, 0, s>>>(*bank, *out, (int)keep, slots_out);
   return check_launch("bank4_evict");
 }

@@ -883,7 +883,7 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   } else {
     const int64_t want = groups ? (2048 + groups - 1) / groups : 1, most = (k->slots + 255) / 256;
     p->nsplit = (int)(want < most ? want : most);
-    p->nsplit = p->nsplit > 128 ? 128 : p->nsplit < 1 ? 1 : p->nsplit;
+    p->nsplit = p->nsplit > 128 ? 128 : p->nsplit < 1 || k->slots <= 1024 ? 1 : p->nsplit;     // (a short bank: no second launch)
   }
   p->parts = p->nsplit > 1 || weigh;
   const int64_t n = (int64_t)k->batch * k->heads * p->nsplit * rows;

@@ -288,6 +288,7 @@ __global__ __launch_bounds__(256) void rotary_weight_sum_kernel(const float *__r
   const int per = (groups + 15) / 16, g1 = (run + 1) * per < groups ? (run + 1) * per : groups;
   float sum = 0.f;
   if (col < width)
+#pragma unroll 16
     for (int g = run * per; g < g1; ++g) sum += partial[(int64_t)g * width + col];
   part[run][threadIdx.x & 15] = sum;
   __syncthreads();

@@ -406,7 +406,21 @@ EVICT = [
     (1, 2, 3000, (2999,), 2998, 10, 100),
     (3, 1, 1500, (1500, 0, 700), 600, 300, 300),                   # nothing left to choose
     (1, 1, 20000, (19999,), 12345, 1, 1),
+    (2, 1, 32768, (32768, 32767), 8000, 7, 9),
+    (1, 1, 45000, (44000,), 30001, 100, 0),                          # more keys than the registers of a workgroup hold
 ]
+
+
+def test_evict_wide_rows():
+    """Rows of whole dwords of scales (128 / 512 channels): every byte and weight of the kept slots, in order."""
+    bank, out = _filled(2, 1, 300, 128, 512, (300, 250)), _dirty(2, 1, 200, 128, 512, seed=3)
+    bank.weight.copy_(torch.rand(bank.weight.shape, generator=torch.Generator().manual_seed(1)))
+    got = ops.bank4_evict(bank, 190, out, first=3, recent=20).cpu().long()
+    assert torch.equal(got.int(), O.evict(bank.weight.cpu(), bank.lens.cpu(), 190, 3, 20)[0])
+    for src, dst in ((bank.key_codes, out.key_codes), (bank.key_scales, out.key_scales), (bank.value_codes, out.value_codes),
+                     (bank.value_scales, out.value_scales), (bank.weight[..., None], out.weight[..., None])):
+        for b in range(2):
+            assert torch.equal(dst[b, 0, :190].cpu(), src[b, 0].cpu()[got[b, 0]])
 
 
 @pytest.mark.parametrize("ties", (False, True))
