@@ -128,7 +128,7 @@ constexpr int EVICT_KEYS = 32;      // keys a lane holds: banks of up to 32 768 
 // counts in LDS (four copies: most weights of a bank share a few exponents, and a bin's increments are serial), then one ordered pass that
 // writes the kept slots ascending.  Equal weights: the lowest slots stay.  A wave owns a run of slots, so a slot's place follows from ballots
 // of its wave and one sum over the waves before: (larger keys before it) + min(equal ones before it, equal ones that stay).
-// One workgroup a (stream, head): bound by latency, 12 barriers and three passes of LDS counts (@@ us at 21 060 slots; slots visited one
+// One workgroup a (stream, head): bound by latency, 12 barriers and three passes of LDS counts (21 us at 21 060 slots; slots visited one
 // 1024-wide row at a time with a scan each, and 8-bit digits, took 49 us).
 template <bool REGS>
 __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float *__restrict__ weight, const int32_t *__restrict__ lens, int heads, int64_t slots,

@@ -70,49 +70,12 @@ template <> struct ReadType<1> { typedef __bf16 T; };
 template <> struct ReadType<2> { typedef _Float16 T; };
 template <> struct ReadType<3> { typedef float T; };
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
 
 // Rows [0, n) of a bank array behind a wave-uniform address: loads take one per-lane offset and answer 0 behind the last row (codes 0, scale
 // byte 0: the value 0), so that what lies behind a stream's length is neither addressed nor looked at.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t bank_rows(const uint8_t *p, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes), 0x00020000);
-}
-
-// 16 channels of a bf16 query as two 8-bit floats each, in units of 2^e: the high four bits and (32 times) the rest.
-__device__ __forceinline__ void split_fp8(const float (&x)[16], float down, int *hi, int *lo) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    int h = 0, l = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float y0 = x[w * 4 + j * 2] * down, y1 = x[w * 4 + j * 2 + 1] * down;
-      const int pair = __builtin_amdgcn_cvt_pk_fp8_f32(y0, y1, 0, false);
-      const float r0 = (y0 - __builtin_amdgcn_cvt_f32_fp8(pair, 0)) * 32.f, r1 = (y1 - __builtin_amdgcn_cvt_f32_fp8(pair, 1)) * 32.f;
-      h |= (pair & 0xffff) << (16 * j);
-      l |= (__builtin_amdgcn_cvt_pk_fp8_f32(r0, r1, 0, false) & 0xffff) << (16 * j);
-    }
-    hi[w] = h;
-    lo[w] = l;
-  }
-}
-__device__ __forceinline__ float load_fp8_piece(const __bf16 *p, bool vec, bool live, float sign, float (&x)[16]) {     // -> its largest magnitude
-  const f32x8 x0 = load8(p, vec), x1 = load8(p + 8, vec);
-  float top = 0.f;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    x[j] = live ? (j < 8 ? x0[j & 7] : x1[j & 7]) * sign : 0.f;
-    const float m = __builtin_fabsf(x[j]);
-    top = m < INFINITY ? fmaxf(top, m) : INFINITY;
-  }
-  return top;
-}
-// the block's largest goes to [128, 256) of the 8-bit format's 448; an infinity or NaN makes the block NaN
-__device__ __forceinline__ int fp8_exponent(float top, float &down) {
-  int e = (int)(__float_as_uint(top) >> 23) - 127 - 7;
-  e = e < -110 ? -110 : e;
-  down = top < INFINITY ? __uint_as_float((uint32_t)(127 - e) << 23) : NAN;
-  return e;
 }
 
 // The sum of a lane's softmax weights, as the second product uses them: bf16 queries round the weights, and the output is divided by the sum of
@@ -135,12 +98,11 @@ constexpr float MAX_LAG = 8.f;      // the running maximum follows a logit that 
 // ------------------------------------------------------------------------------------------ few rows: 16 a workgroup
 // One workgroup: 16 rows x one slice of the slots x DVC value channels; its four waves take 64 slots in turn, each with a running
 // softmax of its own, and meet in LDS at the end.  A step's codes and scales are fetched a step ahead, 64 slots x (DK + DVC) * 17 / 32 bytes a wave.
-// bf16 queries against keys of 128 or 256 channels: 16x16x128 block-scaled products take the codes and scales as they are, against the query in
-// two 8-bit floats a channel (8 bits in all, exact down to 2^-22 of a block's largest); the others widen the keys to bf16.
+// (The block-scaled 4 x 8-bit products would take the codes as they are and the query in two 8-bit floats a channel, but they line up a
+// product's terms in a window of about 13 bits: logits off by 2^-12, weights by 0.2 %.  They are not used.)
 template <int DK, int DVC, int PARTS>
 __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_rows_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
-  constexpr bool SCALED = PARTS == 1 && DK % 128 == 0;
   constexpr int CPL = DK / 4, KSTEPS = DK / 32, VPAD = DVC + 16, OPAD = DVC + 4, NT = DVC / 16, VB = DVC / 32;
   constexpr int LDS_V = 4 * 32 * VPAD * 2, LDS_O = 4 * 16 * OPAD * 4;
   __shared__ __align__(16) char lds[LDS_V > LDS_O ? LDS_V : LDS_O];
@@ -165,37 +127,14 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
   }
   low = __builtin_amdgcn_readfirstlane(low);
 
-  i32x8 q_hi[SCALED ? DK / 128 : 1], q_lo[SCALED ? DK / 128 : 1];
-  int q_scale[SCALED ? DK / 128 : 1];
-  bf16x8 qf[SCALED ? 1 : KSTEPS][PARTS];
+  bf16x8 qf[KSTEPS][PARTS];
   const T *qrow = (const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh;
-  if constexpr (SCALED) {
 #pragma unroll
-    for (int i = 0; i < DK / 128; ++i) {      // an 8-bit operand's lane holds channels grp * 16 .. + 15 of both halves of the 128
-      int e[2];
+  for (int i = 0; i < KSTEPS; ++i) {
+    f32x8 x = load8(qrow + grp * CPL + i * 8, a.q_vec);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float x[16], down;
-        float top = load_fp8_piece((const __bf16 *)qrow + i * 128 + k * 64 + grp * 16, a.q_vec, live, a.q_sign, x);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        e[k] = fp8_exponent(top, down);
-        int hi[4], lo[4];
-        split_fp8(x, down, hi, lo);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) { q_hi[i][k * 4 + w] = hi[w]; q_lo[i][k * 4 + w] = lo[w]; }
-      }
-      // the scale a lane hands over is that of channels grp * 32 .. + 31
-      const int src = col + 32 * (grp & 1), e0 = __shfl(e[0], src), e1 = __shfl(e[1], src), mine = 127 + (grp < 2 ? e0 : e1);
-      q_scale[i] = mine | (mine - 5) << 8;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < KSTEPS; ++i) {
-      f32x8 x = load8(qrow + grp * CPL + i * 8, a.q_vec);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = live ? x[j] * a.q_sign : 0.f;
-      split8<PARTS>(x, qf[i]);
-    }
+    for (int j = 0; j < 8; ++j) x[j] = live ? x[j] * a.q_sign : 0.f;
+    split8<PARTS>(x, qf[i]);
   }
   f32x4 o[NT];
 #pragma unroll
@@ -205,11 +144,11 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
   const int v_row = a.value_dim / 2, vs_row = a.value_dim / 32;
   const uint8_t *kc = a.kc + (int64_t)bh * a.slots * (DK / 2), *ks = a.ks + (int64_t)bh * a.slots * (DK / 32);
   const uint8_t *vc = a.vc + (int64_t)bh * a.slots * v_row + chunk * (DVC / 2), *vs = a.vs + (int64_t)bh * a.slots * vs_row + chunk * VB;
-  const int k_at = col * (DK / 2) + grp * (SCALED ? 16 : CPL / 2), ks_at = col * (DK / 32) + (SCALED ? grp : grp * CPL / 32);
+  const int k_at = col * (DK / 2) + grp * (CPL / 2), ks_at = col * (DK / 32) + grp * CPL / 32;
   const int v_at = lane / VB * v_row + lane % VB * 16, vs_at = lane / VB * vs_row + lane % VB;
 
   struct Step {
-    uint32_t kc[4][KSTEPS], ks[4][2];
+    uint32_t kc[4][KSTEPS], ks[4];
     u32x4 vc[VB];
     uint32_t vs[VB];
   } now, next;
@@ -223,12 +162,9 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
       else
 #pragma unroll
         for (int i = 0; i < KSTEPS / 4; ++i)
-          *reinterpret_cast<u32x4 *>(f.kc[kt] + 4 * i) = __builtin_amdgcn_raw_buffer_load_b128(rk, k_at + kt * 8 * DK + i * (SCALED ? 64 : 16), 0, 0);
-      if constexpr (SCALED)
-#pragma unroll
-        for (int i = 0; i < DK / 128; ++i) f.ks[kt][i] = __builtin_amdgcn_raw_buffer_load_b8(rs, ks_at + kt * (DK / 2) + i * 4, 0, 0);
-      else if constexpr (KSTEPS == 8) f.ks[kt][0] = __builtin_amdgcn_raw_buffer_load_b16(rs, ks_at + kt * (DK / 2), 0, 0);
-      else f.ks[kt][0] = __builtin_amdgcn_raw_buffer_load_b8(rs, ks_at + kt * (DK / 2), 0, 0);
+          *reinterpret_cast<u32x4 *>(f.kc[kt] + 4 * i) = __builtin_amdgcn_raw_buffer_load_b128(rk, k_at + kt * 8 * DK + i * 16, 0, 0);
+      if constexpr (KSTEPS == 8) f.ks[kt] = __builtin_amdgcn_raw_buffer_load_b16(rs, ks_at + kt * (DK / 2), 0, 0);
+      else f.ks[kt] = __builtin_amdgcn_raw_buffer_load_b8(rs, ks_at + kt * (DK / 2), 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < VB; ++i) {       // 64 rows x VB blocks of 16 bytes over 64 lanes
@@ -245,20 +181,11 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
       x[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (SCALED) {
 #pragma unroll
-        for (int i = 0; i < DK / 128; ++i) {
-          const i32x8 kf = {(int)now.kc[kt][4 * i], (int)now.kc[kt][4 * i + 1], (int)now.kc[kt][4 * i + 2], (int)now.kc[kt][4 * i + 3], 0, 0, 0, 0};
-          x[kt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_hi[i], x[kt], 4, 0, 0, (int)now.ks[kt][i], 0, q_scale[i]);
-          x[kt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_lo[i], x[kt], 4, 0, 0, (int)now.ks[kt][i], 1, q_scale[i]);
-        }
-      } else {
+      for (int i = 0; i < KSTEPS; ++i) {
+        const bf16x8 kf = bank4_unpack8(now.kc[kt][i], bank4_scale(KSTEPS == 8 ? (now.ks[kt] >> (i / 4 * 8)) & 255 : now.ks[kt]));
 #pragma unroll
-        for (int i = 0; i < KSTEPS; ++i) {
-          const bf16x8 kf = bank4_unpack8(now.kc[kt][i], bank4_scale(KSTEPS == 8 ? (now.ks[kt][0] >> (i / 4 * 8)) & 255 : now.ks[kt][0]));
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][p], x[kt], 0, 0, 0);
-        }
+        for (int p = 0; p < PARTS; ++p) x[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[i][p], x[kt], 0, 0, 0);
       }
     }
     if (base + 64 > low || base + 64 > s1) {
@@ -373,10 +300,7 @@ struct KeyRow {
   __device__ __forceinline__ float scale(int i) const { return bank4_scale((scales[i / 2] >> (16 * (i & 1))) & 255); }
 };
 
-// Queries of a lane (column l % 32).  bf16 queries are held as two 8-bit floats a channel, each with a power-of-two scale a block of 32
-// channels - high four bits and the rest: the 8 bits of a bf16 number, exact down to 2^-22 of the block's largest - and multiply the
-// bank's codes and scales as they are (the block-scaled product takes 4-bit codes beside 8-bit floats).  fp16 and fp32 queries are 2 / 3 bf16 numbers and
-// multiply widened keys.
+// Queries of a lane (column l % 32), in the channel order of KeyRow.
 template <int DK, int PARTS>
 struct QueryCols {
   bf16x8 f[DK / 16][PARTS];
@@ -404,50 +328,6 @@ struct QueryCols {
         const bf16x8 kf = bank4_unpack8(k.codes[i][u], sc);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, f[i * 4 + u][p], c, 0, 0, 0);
-      }
-    }
-    return c;
-  }
-};
-
-template <int DK>
-struct QueryCols<DK, 1> {
-  i32x8 hi[DK / 64], lo[DK / 64];
-  int scale[DK / 64];                   // byte 0 / 1: the scale of hi / lo of block i * 64 + half * 32
-  __device__ __forceinline__ void load(const __bf16 *row, int half, bool live, bool vec, float sign) {
-#pragma unroll
-    for (int i = 0; i < DK / 64; ++i) {
-      // an 8-bit operand's lane holds channels half * 16 .. + 15 of both blocks of the 64
-      int e[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        float x[16], down;
-        float top = load_fp8_piece(row + i * 64 + b * 32 + half * 16, vec, live, sign, x);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        e[b] = fp8_exponent(top, down);
-        int h[4], l[4];
-        split_fp8(x, down, h, l);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) { hi[i][b * 4 + w] = h[w]; lo[i][b * 4 + w] = l[w]; }
-      }
-      const int mine = 127 + (half ? e[1] : e[0]);
-      scale[i] = mine | (mine - 5) << 8;
-    }
-  }
-  __device__ __forceinline__ f32x16 dot(const KeyRow<DK> &k) const {
-    f32x16 c;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) c[r] = 0.f;
-#pragma unroll
-    for (int i = 0; i < DK / 64; ++i) {
-      const i32x8 kf = {(int)k.codes[i].x, (int)k.codes[i].y, (int)k.codes[i].z, (int)k.codes[i].w, 0, 0, 0, 0};
-      const int ks = (int)k.scales[i / 2];
-      if (i & 1) {
-        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, hi[i], c, 4, 0, 2, ks, 0, scale[i]);
-        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, lo[i], c, 4, 0, 2, ks, 1, scale[i]);
-      } else {
-        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, hi[i], c, 4, 0, 0, ks, 0, scale[i]);
-        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, lo[i], c, 4, 0, 0, ks, 1, scale[i]);
       }
     }
     return c;

@@ -12,6 +12,8 @@
 //
 // Bound: bytes.  Every row is read once and written once (backward: x and dy once, dx once); a row of 16 * U channels is held by
 // 2^ceil(log2 U) neighbouring lanes, 16 channels a lane, so the mean is log2 lane exchanges and nothing is staged.
+#include <type_traits>
+
 #include "bank4.h"
 
 namespace mivos {
@@ -22,6 +24,7 @@ struct RotaryRows {
   const float *weight;
   int64_t xb, xn, xh, gb, gn, gh;
   int heads;
+  uint32_t magic;     // row / heads = the high word of row * magic for rows of a tile (row * heads < 2^32)
 };
 struct RotaryArgs {
   RotaryRows rows[2];
@@ -29,8 +32,8 @@ struct RotaryArgs {
   int64_t pb, pn, pa;
   const uint64_t *freq;
   const int32_t *axis;
-  float *partial;                     // backward: [workgroup][2][dim]
-  int batch, tokens, dim, pairs, interleaved, norm, tile, n_tiles;
+  float *partial;                     // backward: a share of a weight gradient a row of dim, `split` rows of q_weight's, then k_weight's
+  int batch, tokens, dim, pairs, interleaved, norm, tile, n_tiles, split;
   float eps, sign;
 };
 
@@ -130,7 +133,7 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(RotaryArgs a) {
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * a.dim; i += 256) {
       const int w = i / a.dim, c = i - w * a.dim;
-      a.partial[(int64_t)blockIdx.x * 2 * a.dim + i] = dw[0][w][c] + dw[1][w][c] + dw[2][w][c] + dw[3][w][c];
+      a.partial[((int64_t)w * gridDim.x + blockIdx.x) * a.dim + c] = dw[0][w][c] + dw[1][w][c] + dw[2][w][c] + dw[3][w][c];
     }
   }
 }
@@ -168,135 +171,169 @@ __device__ __forceinline__ void unit_turn(f32x8 &lo, f32x8 &hi, const f32x2 *cs)
   hi = oh;
 }
 
+// x summed over a row's lanes (neighbours, a power of two): lane permutations inside the 16 lanes of a row, no LDS round trip
+__device__ __forceinline__ float lanes_sum(float x, int lanes) {
+  auto add = [&](auto ctrl) { x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+  if (lanes >= 2) add(std::integral_constant<int, 0xb1>{});      // neighbours
+  if (lanes >= 4) add(std::integral_constant<int, 0x4e>{});      // pairs of a quad
+  if (lanes >= 8) add(std::integral_constant<int, 0x141>{});     // half row mirrored: the other quad
+  if (lanes >= 16) add(std::integral_constant<int, 0x140>{});    // row mirrored: the other eight
+  if (lanes >= 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
+// A workgroup's tokens in tiles: the tile's sines and cosines in LDS once, then the rows of its queries and of its keys, `slots` at a time; the
+// next row is fetched while one is worked on, the first ones while the table is built.  Backward: the first `a.split` workgroups take the queries,
+// the others the keys (one set of weights and sums in registers, so that three workgroups fit a CU: 61 -> 58 us at 16 200 tokens x 20 heads x 128).
 template <typename T, bool INTER, bool NORM, bool GRAD>
-__global__ __launch_bounds__(256) void rotary_rows_kernel(RotaryArgs a, int lanes /* a row, a power of two */) {
+__global__ __launch_bounds__(256, GRAD || sizeof(T) == 4 ? 3 : 4) void rotary_rows_kernel(RotaryArgs a, int lanes /* a row, a power of two */) {
   extern __shared__ __align__(16) f32x2 table[];     // [tile][pairs] (cos, sin); backward: the weight gradients afterwards
-  const int tid = threadIdx.x, units = a.dim / 16, slots = 256 / lanes, u = tid & (lanes - 1);
+  const int tid = threadIdx.x, units = a.dim / 16, slots = 256 / lanes, u = tid & (lanes - 1), row0 = tid / lanes;
   int c0, c1;
   bool rot;
   unit_channels<INTER>(u, a.pairs, c0, c1, rot);
   const bool live = u < units;
-  f32x8 acc[2][2], w[2][2];
+  constexpr int KINDS = GRAD ? 1 : 2;                // operands a workgroup works on: rows[kind0], rows[kind0 + 1], ...
+  const int kind0 = GRAD ? blockIdx.x >= a.split : 0, group = GRAD && kind0 ? blockIdx.x - a.split : blockIdx.x;
+  const int groups = !GRAD ? gridDim.x : kind0 ? gridDim.x - a.split : a.split;
+  f32x8 acc0, acc1, w[KINDS][2];
   if constexpr (NORM || GRAD) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (live && a.rows[k].heads) {
-        w[k][0] = load8(a.rows[k].weight + c0, false);
-        w[k][1] = load8(a.rows[k].weight + c1, false);
+    for (int k = 0; k < KINDS; ++k)
+      if (live && a.rows[kind0 + k].heads) {
+        w[k][0] = load8(a.rows[kind0 + k].weight + c0, false);
+        w[k][1] = load8(a.rows[kind0 + k].weight + c1, false);
       }
   }
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[k][0][j] = acc[k][1][j] = 0.f;
+  for (int j = 0; j < 8; ++j) acc0[j] = acc1[j] = 0.f;
 
-  for (int tile = blockIdx.x; tile < a.n_tiles; tile += gridDim.x) {
-    const int64_t first = (int64_t)tile * a.tile, all = (int64_t)a.batch * a.tokens;
-    const int n_tok = (int)(all - first < a.tile ? all - first : a.tile);
+  struct Row { u32x4 v[GRAD ? 4 : 2][sizeof(T) / 2]; int t, h; };      // as they lie in memory: x | x, or dy | dy | x | x
+  auto take = [&](Row &f, int i, const T *p) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) f.v[i][j] = reinterpret_cast<const u32x4 *>(p)[j];
+  };
+  auto wide = [&](const Row &f, int i) { return load8(reinterpret_cast<const T *>(f.v[i]), true); };
+  for (int tile = group; tile < a.n_tiles; tile += groups) {
+    const uint32_t first = (uint32_t)tile * a.tile, all = (uint32_t)a.batch * a.tokens;       // at most 2^30 tokens
+    const int n_tok = (int)(all - first < (uint32_t)a.tile ? all - first : a.tile);
+    const uint32_t b0 = first / a.tokens, n0 = first - b0 * a.tokens;
+    auto place = [&](int t, uint32_t &b, uint32_t &n) {
+      b = b0;
+      n = n0 + t;
+      if (n >= (uint32_t)a.tokens) { const uint32_t q = n / a.tokens; b += q; n -= q * a.tokens; }
+    };
+    auto fetch = [&](Row &f, const RotaryRows &R, int row) {
+      f.t = R.heads == 1 ? row : (int)__umulhi((uint32_t)row, R.magic);       // row / heads
+      f.h = row - f.t * R.heads;
+#pragma unroll
+      for (int i = 0; i < (GRAD ? 4 : 2); ++i)
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) f.v[i][j] = u32x4{0u, 0u, 0u, 0u};
+      if (!live || row >= n_tok * R.heads) return;
+      uint32_t b, n;
+      place(f.t, b, n);
+      const T *x = (const T *)R.x + b * R.xb + n * R.xn + f.h * R.xh;
+      if constexpr (GRAD) {
+        const T *g = (const T *)R.g + b * R.gb + n * R.gn + f.h * R.gh;
+        take(f, 0, g + c0);
+        take(f, 1, g + c1);
+        take(f, 2, x + c0);
+        take(f, 3, x + c1);
+      } else {
+        take(f, 0, x + c0);
+        take(f, 1, x + c1);
+      }
+    };
+    Row now, next;
+    fetch(next, a.rows[kind0], row0);
     __syncthreads();
     for (int e = tid; e < n_tok * a.pairs; e += 256) {
       const int t = e / a.pairs, i = e - t * a.pairs;
-      const int b = (int)((first + t) / a.tokens), n = (int)(first + t - (int64_t)b * a.tokens);
+      uint32_t b, n;
+      place(t, b, n);
       float s, c;
       turn_sincos(a.pos[b * a.pb + n * a.pn + a.axis[i] * a.pa], a.freq[i], a.sign, s, c);
       table[t * a.pairs + i] = f32x2{c, s};
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const RotaryRows &R = a.rows[k];
+    for (int k = 0; k < KINDS; ++k) {
+      const RotaryRows &R = a.rows[kind0 + k];
       const int n_rows = n_tok * R.heads;
-      for (int row = tid / lanes; row < n_rows; row += slots) {
-        const int t = row / R.heads, h = row - t * R.heads;
-        const int b = (int)((first + t) / a.tokens), n = (int)(first + t - (int64_t)b * a.tokens);
-        f32x8 lo, hi, xl, xh;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) lo[j] = hi[j] = xl[j] = xh[j] = 0.f;
-        if (live) {
-          const T *x = (const T *)R.x + b * R.xb + n * R.xn + h * R.xh;
-          if constexpr (GRAD) {
-            const T *g = (const T *)R.g + b * R.gb + n * R.gn + h * R.gh;
-            xl = load8(x + c0, true);
-            xh = load8(x + c1, true);
-            lo = load8(g + c0, true);
-            hi = load8(g + c1, true);
-          } else {
-            lo = load8(x + c0, true);
-            hi = load8(x + c1, true);
-          }
-        }
+      for (int row = row0; row < n_rows; row += slots) {
+        now = next;
+        if (row + slots < n_rows) fetch(next, R, row + slots);
+        else if (k + 1 < KINDS) fetch(next, a.rows[1], row0);
+        f32x8 lo = wide(now, 0), hi = wide(now, 1);
         if constexpr (NORM) {
           float ss = 0.f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) ss += lo[j] * lo[j] + hi[j] * hi[j];
-          for (int d = 1; d < lanes; d <<= 1) ss += __shfl_xor(ss, d);
+          ss = lanes_sum(ss, lanes);
           const float r = 1.f / sqrtf(ss / a.dim + a.eps);
           lo *= r * w[k][0];
           hi *= r * w[k][1];
         }
-        if (rot && live) unit_turn<INTER>(lo, hi, table + t * a.pairs + 8 * u);
+        if (rot && live) unit_turn<INTER>(lo, hi, table + now.t * a.pairs + 8 * u);
         if constexpr (GRAD) {
-          const f32x8 gl = lo * w[k][0], gh = hi * w[k][1];
+          const f32x8 gl = lo * w[k][0], gh = hi * w[k][1], xl = wide(now, 2), xh = wide(now, 3);
           float ss = 0.f, dot = 0.f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             ss += xl[j] * xl[j] + xh[j] * xh[j];
             dot += live ? gl[j] * xl[j] + gh[j] * xh[j] : 0.f;
           }
-          for (int d = 1; d < lanes; d <<= 1) { ss += __shfl_xor(ss, d); dot += __shfl_xor(dot, d); }
+          ss = lanes_sum(ss, lanes);
+          dot = lanes_sum(dot, lanes);
           const float r = 1.f / sqrtf(ss / a.dim + a.eps), q = r * r * dot / a.dim;
-          acc[k][0] += lo * xl * r;
-          acc[k][1] += hi * xh * r;
+          acc0 += lo * xl * r;
+          acc1 += hi * xh * r;
           lo = r * (gl - xl * q);
           hi = r * (gh - xh * q);
         }
         if (live) {
-          T *y = (T *)R.y + ((first + t) * R.heads + h) * a.dim;
+          T *y = (T *)R.y + ((int64_t)(first + now.t) * R.heads + now.h) * a.dim;
           store8(y + c0, lo);
           store8(y + c1, hi);
         }
       }
+      if (k + 1 < KINDS && row0 >= n_rows) fetch(next, a.rows[1], row0);      // (a slot without a query row)
     }
   }
-  if constexpr (GRAD) {                               // the workgroup's share of both weight gradients, its row slots in order
+  if constexpr (GRAD) {                               // the workgroup's share of its weight gradient, its row slots in order
     float *dw = reinterpret_cast<float *>(table);     // [slots][16 * lanes]
-    for (int k = 0; k < 2; ++k) {
-      __syncthreads();
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        dw[tid * 16 + j] = k ? acc[1][0][j] : acc[0][0][j];
-        dw[tid * 16 + 8 + j] = k ? acc[1][1][j] : acc[0][1][j];
-      }
-      __syncthreads();
-      for (int i = tid; i < units * 16; i += 256) {
-        int d0, d1;
-        bool r2;
-        unit_channels<INTER>(i / 16, a.pairs, d0, d1, r2);
-        const int c = (i & 8 ? d1 : d0) + (i & 7);
-        float sum = 0.f;
-        for (int s = 0; s < slots; ++s) sum += dw[s * 16 * lanes + i];
-        a.partial[((int64_t)blockIdx.x * 2 + k) * a.dim + c] = sum;
-      }
+    for (int j = 0; j < 8; ++j) { dw[tid * 16 + j] = acc0[j]; dw[tid * 16 + 8 + j] = acc1[j]; }
+    __syncthreads();
+    for (int i = tid; i < units * 16; i += 256) {
+      int d0, d1;
+      bool r2;
+      unit_channels<INTER>(i / 16, a.pairs, d0, d1, r2);
+      const int c = (i & 8 ? d1 : d0) + (i & 7);
+      float sum = 0.f;
+      for (int s = 0; s < slots; ++s) sum += dw[s * 16 * lanes + i];
+      a.partial[(int64_t)blockIdx.x * a.dim + c] = sum;
     }
   }
 }
 
-// dw[k][c] = the workgroups' shares in order: 16 columns a workgroup, 16 runs of workgroups each
-__global__ __launch_bounds__(256) void rotary_weight_sum_kernel(const float *__restrict__ partial, int groups, int dim, float *dq, float *dk) {
+// dw[k][c] = the shares of workgroups [k ? split : 0, k ? groups : split) in order: 16 columns a workgroup, 16 runs of shares each
+__global__ __launch_bounds__(256) void rotary_weight_sum_kernel(const float *__restrict__ partial, int split, int groups, int dim, float *dq, float *dk) {
   __shared__ float part[16][17];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4, width = 2 * dim;
-  const int per = (groups + 15) / 16, g1 = (run + 1) * per < groups ? (run + 1) * per : groups;
+  const int k = blockIdx.y, col = blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
+  const int first = k ? split : 0, end = k ? groups : split, per = (end - first + 15) / 16, g0 = first + run * per, g1 = g0 + per < end ? g0 + per : end;
   float sum = 0.f;
-  if (col < width)
+  if (col < dim)
 #pragma unroll 16
-    for (int g = run * per; g < g1; ++g) sum += partial[(int64_t)g * width + col];
+    for (int g = g0; g < g1; ++g) sum += partial[(int64_t)g * dim + col];
   part[run][threadIdx.x & 15] = sum;
   __syncthreads();
-  if (run == 0 && col < width) {
+  if (run == 0 && col < dim) {
     float t = 0.f;
     for (int r = 0; r < 16; ++r) t += part[r][threadIdx.x];
-    float *out = col < dim ? dq : dk;
-    if (out) out[col < dim ? col : col - dim] = t;
+    (k ? dk : dq)[col] = t;
   }
 }
 
@@ -304,7 +341,7 @@ constexpr int ROTARY_GRAD_GROUPS = 1024;   // workgroups of a backward launch (4
 
 struct RotaryPlan {
   bool rows;            // 16 channels a lane (else one wave a row)
-  int lanes, grid;
+  int lanes, grid, groups;      // groups: shares of the weight gradients
   size_t lds;
 };
 
@@ -313,7 +350,7 @@ static int rotary_plan(const mivos_rotary *d, RotaryArgs *a, RotaryPlan *p, bool
   uintptr_t bits = 0;
   for (int k = 0; k < 2; ++k) {
     const mivos_rotary_rows &r = d->rows[k];
-    a->rows[k] = RotaryRows{r.x, r.g, r.y, r.weight, r.xb, r.xn, r.xh, r.gb, r.gn, r.gh, r.heads};
+    a->rows[k] = RotaryRows{r.x, r.g, r.y, r.weight, r.xb, r.xn, r.xh, r.gb, r.gn, r.gh, r.heads, r.heads > 1 ? 0xffffffffu / (uint32_t)r.heads + 1 : 0};
     if (!r.heads) continue;
     bits |= (uintptr_t)r.x | (uintptr_t)r.y | (uintptr_t)((r.xb | r.xn | r.xh) * es);
     if (grad) bits |= (uintptr_t)r.g | (uintptr_t)((r.gb | r.gn | r.gh) * es);
@@ -334,12 +371,20 @@ static int rotary_plan(const mivos_rotary *d, RotaryArgs *a, RotaryPlan *p, bool
     p->lds = (size_t)tile * d->pairs * 8;
     if (grad && p->lds < 256 * 16 * 4) p->lds = 256 * 16 * 4;
     p->grid = a->n_tiles;
-    if (grad && p->grid > ROTARY_GRAD_GROUPS) p->grid = ROTARY_GRAD_GROUPS;
-    else if (p->grid > (1 << 20)) p->grid = 1 << 20;
+    if (!grad && p->grid > (1 << 20)) p->grid = 1 << 20;
+    if (grad) {                                           // shared out by their heads
+      const int hq = d->rows[0].heads, hk = d->rows[1].heads, most = ROTARY_GRAD_GROUPS;
+      const int gq = hk ? (int)((int64_t)most * hq / (hq + hk)) : most, gk = most - gq;
+      a->split = gq < 1 ? 1 : gq < a->n_tiles ? gq : a->n_tiles;
+      p->groups = a->split + (hk ? (gk < 1 ? 1 : gk < a->n_tiles ? gk : a->n_tiles) : 0);
+      p->grid = p->groups;
+    }
   } else {
     const int64_t rows = all * (d->rows[0].heads + d->rows[1].heads);
     const int64_t most = grad ? ROTARY_GRAD_GROUPS : 256 * 64;
     p->grid = (int)((rows + 3) / 4 < most ? (rows + 3) / 4 : most);
+    a->split = p->grid;
+    p->groups = 2 * p->grid;
   }
   return MIVOS_OK;
 }
@@ -390,7 +435,7 @@ extern "C" int mivos_rotary_axes(const mivos_rotary *d, void *stream) {
   return check_launch("rotary_axes");
 }
 
-extern "C" int64_t mivos_norm_rotary_grad_workspace_bytes(int dim) { return (int64_t)ROTARY_GRAD_GROUPS * 2 * dim * 4; }
+extern "C" int64_t mivos_norm_rotary_grad_workspace_bytes(int dim) { return ((int64_t)ROTARY_GRAD_GROUPS + 1) * 2 * dim * 4; }
 
 extern "C" int mivos_norm_rotary_grad(const mivos_rotary *d, float *dq_weight, float *dk_weight, void *stream) {
   if (int rc = rotary_check(d, true, "norm_rotary_grad")) return rc;
@@ -405,6 +450,6 @@ extern "C" int mivos_norm_rotary_grad(const mivos_rotary *d, float *dq_weight, f
     else if (d->dtype == MIVOS_F16) rotary_launch<_Float16, true>(a, p, s);
     else rotary_launch<__bf16, true>(a, p, s);
   }
-  rotary_weight_sum_kernel<<<cdiv(2 * d->dim, 16), 256, 0, s>>>(a.partial, p.grid, d->dim, dq_weight, dk_weight);
+  rotary_weight_sum_kernel<<<dim3(cdiv(d->dim, 16), d->rows[1].heads ? 2 : 1), 256, 0, s>>>(a.partial, a.split, p.groups, d->dim, dq_weight, dk_weight);
   return check_launch("norm_rotary_grad");
 }

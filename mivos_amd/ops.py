@@ -1110,7 +1110,7 @@ class RotaryAxes:
     behind the pairs are not turned.  Pair j of a section of n has the frequency base^(-j / n); shared=True: one ladder over all pairs,
     base^(-i / sum(sections)).  interleaved=True pairs neighbouring channels, else channel i goes with i + sum(sections).  The device
     table keeps every frequency as a 64-bit fraction of a turn, so angles are exact for every int32 position."""
-    __slots__ = ("head_dim", "sections", "pairs", "interleaved", "freq", "axis")
+    __slots__ = ("head_dim", "sections", "pairs", "interleaved", "freq", "axis", "tables")
 
     def __init__(self, head_dim, sections, base=10000.0, shared=False, interleaved=False, device="cuda"):
         sections = tuple(int(n) for n in sections)
@@ -1123,6 +1123,7 @@ class RotaryAxes:
         turns, axes = _rotary_table(sections, float(base), bool(shared))
         self.freq = torch.tensor(turns, dtype=torch.int64, device=device)
         self.axis = torch.tensor(axes, dtype=torch.int32, device=device)
+        self.tables = self.freq.data_ptr(), self.axis.data_ptr()
         if self.freq.is_cuda:
             with torch.cuda.device(self.freq.device):
                 publish_constants()
@@ -1130,34 +1131,37 @@ class RotaryAxes:
 
 # mivos_rotary, packed at once: two mivos_rotary_rows (x, g, y, weight, six strides, heads), then the rest in order
 _ROTARY = struct.Struct("4Q6qii" * 2 + "4Q4q7if")
-
-
-def _rotary_rows(x, y, g=None, weight=None):
-    b, n, h, _ = x.stride()
-    gb, gn, gh = (0, 0, 0) if g is None else g.stride()[:3]
-    return x.data_ptr(), 0 if g is None else g.data_ptr(), y.data_ptr(), 0 if weight is None else weight.data_ptr(), b, n, h, gb, gn, gh, x.shape[2], 0
-
-
 _NO_ROWS = (0,) * 12
 
 
+def _head_operand(x, name, shape=None):
+    """Shape and strides of [batch, tokens, heads, channels] with dense channels; shape: (batch, tokens, None, channels) it has to have."""
+    try:
+        b, n, h, d = x.shape
+    except ValueError:
+        raise MivosHipError(f"{name}: expected [batch, tokens, heads, channels], got {list(x.shape)}") from None
+    if shape is not None and (b != shape[0] or n != shape[1] or d != shape[3] or (shape[2] is not None and h != shape[2])):
+        raise MivosHipError(f"{name}: expected {list(shape)}, got {list(x.shape)}")
+    sb, sn, sh, sc = x.stride()
+    if sc != 1 and d > 1 and x.numel():
+        raise MivosHipError(f"{name}: the channel stride must be 1")
+    return b, n, h, d, sb, sn, sh
+
+
 def _rotary_check(q, k, positions, plan):
-    _head_rows(q, "q")
-    b, n, _, d = q.shape
+    """-> (mivos_dtype, q's shape and strides, k's)"""
+    qd = _head_operand(q, "q")
+    b, n, _, d, _, _, _ = qd
     if d != plan.head_dim:
         raise MivosHipError(f"q has heads of {d} channels, the plan {plan.head_dim}")
+    kd = None
     if k is not None:
-        _head_rows(k, "k", (b, n, k.shape[2] if k.dim() == 4 else -1, d))
+        kd = _head_operand(k, "k", (b, n, None, d))
         if k.dtype != q.dtype:
             raise MivosHipError(f"q is {q.dtype}, k is {k.dtype}")
     if positions.dtype != torch.int32 or positions.shape != (b, n, len(plan.sections)):
         raise MivosHipError(f"positions: expected int32 {[b, n, len(plan.sections)]}, got {positions.dtype} {list(positions.shape)}")
-    return _dtype_code(q)
-
-
-def _rotary_desc(q, q_rows, k_rows, positions, plan, code, inverse, eps, ws=0, ws_bytes=0):
-    return RotaryDesc.from_buffer_copy(_ROTARY.pack(*q_rows, *k_rows, positions.data_ptr(), plan.freq.data_ptr(), plan.axis.data_ptr(), ws, *positions.stride(), ws_bytes,
-                        q.shape[0], q.shape[1], plan.head_dim, plan.pairs, code, plan.interleaved, inverse, eps))
+    return _dtype_code(q), qd, kd
 
 
 def _norm_weight(w, ref, name):
@@ -1167,13 +1171,16 @@ def _norm_weight(w, ref, name):
 
 
 def _rotary(q, k, positions, plan, inverse, eps, q_weight=None, k_weight=None):
-    code = _rotary_check(q, k, positions, plan)
+    code, (b, n, hq, d, qb, qn, qh), kd = _rotary_check(q, k, positions, plan)
     _here(q, k, positions, plan.freq, q_weight, k_weight)
-    yq = q.new_empty(q.shape)
-    yk = None if k is None else k.new_empty(k.shape)
-    desc = _rotary_desc(q, _rotary_rows(q, yq, None, q_weight), _NO_ROWS if k is None else _rotary_rows(k, yk, None, k_weight), positions, plan, code,
-                        inverse, eps)
-    check(_lib.load().mivos_rotary_axes(desc, _stream()))
+    yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    yk, k_rows = None, _NO_ROWS
+    if k is not None:
+        yk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_rows = (k.data_ptr(), 0, yk.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), *kd[4:], 0, 0, 0, kd[2], 0)
+    desc = _ROTARY.pack(q.data_ptr(), 0, yq.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), qb, qn, qh, 0, 0, 0, hq, 0, *k_rows,
+                        positions.data_ptr(), *plan.tables, 0, *positions.stride(), 0, b, n, d, plan.pairs, code, plan.interleaved, inverse, eps)
+    check(_lib.load().mivos_rotary_axes(RotaryDesc.from_buffer_copy(desc), _stream()))
     return yq, yk
 
 
@@ -1205,25 +1212,28 @@ def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, plan, eps=1e-6
     if not eps >= 0:
         raise MivosHipError(f"norm_rotary_grad: eps {eps}")
     _norm_weight(q_weight, _head_rows(q, "q"), "q_weight")
-    _head_rows(dq, "dq", q.shape)
     if (dk is None) != (k is None):
         raise MivosHipError("norm_rotary_grad: dk goes with k")
     if k is not None:
         _norm_weight(k_weight, _head_rows(k, "k"), "k_weight")
-        _head_rows(dk, "dk", k.shape)
+    qg = _head_operand(dq, "dq", q.shape)[4:]
+    kg = None if k is None else _head_operand(dk, "dk", k.shape)[4:]
     for g in (dq, dk):
         if g is not None and g.dtype != q.dtype:
             raise MivosHipError(f"q is {q.dtype}, its gradient {g.dtype}")
-    code = _rotary_check(q, k, positions, plan)
+    code, (b, n, hq, d, qb, qn, qh), kd = _rotary_check(q, k, positions, plan)
     _here(q, k, positions, plan.freq, dq, dk, q_weight, k_weight)
     lib = _lib.load()
-    need = lib.mivos_norm_rotary_grad_workspace_bytes(q.shape[3])
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    gq, wq = q.new_empty(q.shape), torch.empty_like(q_weight)
-    gk, wk = (None, None) if k is None else (k.new_empty(k.shape), torch.empty_like(k_weight))
-    desc = _rotary_desc(q, _rotary_rows(q, gq, dq, q_weight), _NO_ROWS if k is None else _rotary_rows(k, gk, dk, k_weight), positions, plan, code, 1,
-                        float(eps), ws.data_ptr(), need)
-    check(lib.mivos_norm_rotary_grad(desc, wq.data_ptr(), None if wk is None else wk.data_ptr(), _stream()))
+    need = lib.mivos_norm_rotary_grad_workspace_bytes(d)
+    ws = q.new_empty(need, dtype=torch.uint8)
+    gq, wq = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(q_weight)
+    gk, wk, k_rows = None, None, _NO_ROWS
+    if k is not None:
+        gk, wk = torch.empty_like(k, memory_format=torch.contiguous_format), torch.empty_like(k_weight)
+        k_rows = (k.data_ptr(), dk.data_ptr(), gk.data_ptr(), k_weight.data_ptr(), *kd[4:], *kg, kd[2], 0)
+    desc = _ROTARY.pack(q.data_ptr(), dq.data_ptr(), gq.data_ptr(), q_weight.data_ptr(), qb, qn, qh, *qg, hq, 0, *k_rows, positions.data_ptr(),
+                        *plan.tables, ws.data_ptr(), *positions.stride(), need, b, n, d, plan.pairs, code, plan.interleaved, 1, eps)
+    check(lib.mivos_norm_rotary_grad(RotaryDesc.from_buffer_copy(desc), wq.data_ptr(), None if wk is None else wk.data_ptr(), _stream()))
     return gq, gk, wq, wk
 
 
@@ -1284,8 +1294,8 @@ def bank4_append(bank, keys, values, at=None, count=None):
     """keys [B, T, H, Dk], values [B, T, H, Dv] (one type; dense channels) quantised into slots [at[b], at[b] + count[b]) of the bank (at None:
     behind what is there; count None: all T); their weight becomes 0 and bank.lens[b] = at[b] + count[b].  Tokens beyond the bank's last slot
     are dropped and remembered (Bank4.check_room)."""
-    _head_rows(keys, "keys", (bank.batch, keys.shape[1] if keys.dim() == 4 else -1, bank.heads, bank.key_dim))
-    _head_rows(values, "values", (bank.batch, keys.shape[1], bank.heads, bank.value_dim))
+    _, tokens, _, _, kb, kt, kh = _head_operand(keys, "keys", (bank.batch, keys.shape[1] if keys.dim() == 4 else -1, bank.heads, bank.key_dim))
+    _, _, _, _, vb, vt, vh = _head_operand(values, "values", (bank.batch, tokens, bank.heads, bank.value_dim))
     if keys.dtype != values.dtype:
         raise MivosHipError(f"keys are {keys.dtype}, values {values.dtype}")
     code = _dtype_code(keys)
@@ -1298,9 +1308,8 @@ def bank4_append(bank, keys, values, at=None, count=None):
     if count is not None and abs(_int32_vector(count, bank.batch, "count").data_ptr() - bank._desc.lens) < 4 * bank.batch:
         raise MivosHipError("count overlaps the bank's lengths")
     _here(bank.lens, keys, values, at, count)
-    ks, vs = keys.stride(), values.stride()
-    check(_lib.load().mivos_bank4_append(bank._desc, keys.data_ptr(), ks[0], ks[1], ks[2], values.data_ptr(), vs[0], vs[1], vs[2], code, at.data_ptr(),
-                                         None if count is None else count.data_ptr(), keys.shape[1], _stream()))
+    check(_lib.load().mivos_bank4_append(bank._desc, keys.data_ptr(), kb, kt, kh, values.data_ptr(), vb, vt, vh, code, at.data_ptr(),
+                                         None if count is None else count.data_ptr(), tokens, _stream()))
 
 
 def bank4_values(bank, first=None, count=None, dtype=torch.bfloat16):
@@ -1326,8 +1335,7 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
     the stream's filled slots (scale None: Dk^-0.5).  causal=True: the T tokens are the newest of the bank (appended before), token t sees the
     slots up to its own.  count int32 [B]: valid tokens of a padded batch; the others, and tokens that see no slot, give 0.  weigh=True also
     adds the softmax weights every slot receives from the stream's tokens and its head's queries to bank.weight, for bank4_evict."""
-    _head_rows(queries, "queries", (bank.batch, queries.shape[1] if queries.dim() == 4 else -1, queries.shape[2] if queries.dim() == 4 else -1, bank.key_dim))
-    b, t, hq, d = queries.shape
+    b, t, hq, d, qb, qt, qh = _head_operand(queries, "queries", (bank.batch, queries.shape[1] if queries.dim() == 4 else -1, None, bank.key_dim))
     if hq < 1 or hq % bank.heads:
         raise MivosHipError(f"{hq} query heads over {bank.heads} bank heads")
     code = _dtype_code(queries)
@@ -1340,8 +1348,7 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
     _here(bank.lens, queries, count)
     out = queries.new_empty((b, t, hq, bank.value_dim))
     ws = queries.new_empty(need, dtype=torch.uint8) if need else None
-    qs = queries.stride()
-    check(lib.mivos_bank4_read(bank._desc, queries.data_ptr(), qs[0], qs[1], qs[2], code, hq, t, None if count is None else count.data_ptr(),
+    check(lib.mivos_bank4_read(bank._desc, queries.data_ptr(), qb, qt, qh, code, hq, t, None if count is None else count.data_ptr(),
                                d ** -0.5 if scale is None else float(scale), causal, weigh, out.data_ptr(), None if ws is None else ws.data_ptr(), need,
                                _stream()))
     return out
