@@ -213,6 +213,20 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
     const float mu = m == -INFINITY ? 0.f : m;
+    if (a.causal) {        // a value block that stands for NaN makes it NaN for the rows that see its slot, and is 0 for the others (0 x NaN is none)
+#pragma unroll
+      for (int i = 0; i < VB; ++i) {
+        uint64_t bad = __ballot(now.vs[i] == kBank4NanScale);
+        if (now.vs[i] == kBank4NanScale) { now.vs[i] = 127; now.vc[i] = u32x4{0u, 0u, 0u, 0u}; }
+        for (; bad; bad &= bad - 1) {
+          const int e = i * 64 + __builtin_ctzll(bad);
+          const float add = base + e / VB < limit ? NAN : 0.f;
+#pragma unroll
+          for (int c = 0; c < VB; ++c)
+            if (c == e % VB) { o[2 * c] += add; o[2 * c + 1] += add; }
+        }
+      }
+    }
     // ---- V in two halves of 32 slots
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -338,18 +352,19 @@ struct QueryCols {
 // codes straight into registers; the V rows are widened once for the workgroup into one of two LDS buffers while the matrix cores work on
 // the other.  S^T = K Q^T and O^T = V^T P^T on 32x32 products: a lane holds one query, 16 keys of each 32, and these are again the
 // operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^8.
-template <int DK, int DVC, int PARTS, bool WEIGH>
+template <int DK, int DVC, int PARTS, bool WEIGH, bool CAUSAL>
 __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1) void bank4_block_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
   constexpr int VS = DVC + 16, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB, VL = (VE + 255) / 256;
   extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
+  __shared__ uint64_t nan_blocks[2][4][VL];            // causal: the value blocks of a buffer that stand for NaN, a bit a lane of the wave that stored it
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
   const int split = blockIdx.x, row0 = blockIdx.y * 128, r = row0 + wave * 32 + col;
   const int64_t len = read_len(a, b);
   const int cnt = read_count(a, b), t = r / a.group;
   const bool live = r < a.rows && t < cnt;
-  const int limit = live ? (int)read_limit(a, len, cnt, t) : (int)len;
+  const int limit = live && CAUSAL ? (int)read_limit(a, len, cnt, t) : (int)len;
   int last_t = (row0 + 127 < a.rows ? row0 + 127 : a.rows - 1) / a.group;
   last_t = last_t < cnt ? last_t : cnt - 1;
   const int seen = row0 / a.group < cnt ? (int)read_limit(a, len, cnt, last_t) : 0;
@@ -396,14 +411,37 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       vsn[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, tid / VB * vs_row + tid % VB, i * (256 / VB) * vs_row, 0);
     }
   };
-  auto store_values = [&](__bf16 *to) {
+  auto store_values = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
       const int e = i * 256 + tid, vr = e / VB, blk = e % VB;
-      if (VE < 256 && e >= VE) break;
-      const float sc = bank4_scale(vsn[i]);
+      if (VE < 256 && e >= VE) {
+        if (CAUSAL) nan_blocks[buf][wave][i] = 0;
+        break;
+      }
+      float sc = bank4_scale(vsn[i]);
+      if (CAUSAL) {
+        nan_blocks[buf][wave][i] = __ballot(vsn[i] == kBank4NanScale);
+        sc = vsn[i] == kBank4NanScale ? 1.f : sc;
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(to + vr * VS + blk * 32 + j * 8) = bank4_unpack8(vn[i][j], sc);
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(vt + (buf * 64 + vr) * VS + blk * 32 + j * 8) = bank4_unpack8(vn[i][j], sc);
+    }
+  };
+  // Causal: a value block that stands for NaN makes it NaN for the rows that see its slot and is finite for the others, whose weight there is 0.
+  auto add_nans = [&](int buf, int base) {
+    uint64_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4 * VL; ++i) any |= nan_blocks[buf][i / VL][i % VL];
+    if (!any) return;
+    for (int i = 0; i < 4 * VL; ++i) {
+      for (uint64_t bad = nan_blocks[buf][i / VL][i % VL]; bad; bad &= bad - 1) {
+        const int e = i % VL * 256 + i / VL * 64 + __builtin_ctzll(bad);
+        const float add = base + e / VB < limit ? NAN : 0.f;
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+          if (c == e % VB) o[c] += add;
+      }
     }
   };
 
@@ -435,7 +473,8 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
   };
-  auto step = [&](f32x16 (&x)[2], f32x16 (&xn)[2], const KeyRow<DK> (&k)[2], KeyRow<DK> (&kn)[2], int base, const __bf16 *now, __bf16 *then) {
+  auto step = [&](f32x16 (&x)[2], f32x16 (&xn)[2], const KeyRow<DK> (&k)[2], KeyRow<DK> (&kn)[2], int base, int buf) {
+    if (CAUSAL) add_nans(buf, base);
     load_values(base + 64);                  // (behind the slice: nothing is read, zeros come back)
     load_keys(kn, base + 128);
 
@@ -456,7 +495,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const __bf16 *at = now + (s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+      const __bf16 *at = vt + (buf * 64 + s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32));
@@ -467,7 +506,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       }
     }
     top = row_top(xn);
-    store_values(then);
+    store_values(buf ^ 1);
     __syncthreads();
     settle(xn, base + 64);
   };
@@ -478,15 +517,15 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
     xa[0] = q.dot(ka[0]);
     xa[1] = q.dot(ka[1]);
     load_keys(ka, s0 + 64);
-    store_values(vt);
+    store_values(0);
     top = row_top(xa);
     settle(xa, s0);
   }
   __syncthreads();
   for (int base = s0; base < s1; base += 128) {
-    step(xa, xb, ka, kb, base, vt, vt + 64 * VS);
+    step(xa, xb, ka, kb, base, 0);
     if (base + 64 >= s1) break;
-    step(xb, xa, kb, ka, base + 64, vt + 64 * VS, vt);
+    step(xb, xa, kb, ka, base + 64, 1);
   }
   if (PARTS > 1) l = l_used;
   l += __shfl_xor(l, 32);
@@ -609,7 +648,7 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
 }
 
 // A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum and log2 of the sum of the weights, and the
-// factors of its slices' accumulators.
+// factors of its slices' accumulators (-1: an empty slice).
 struct RowJoin {
   float f[2], inv, lse;
   __device__ __forceinline__ RowJoin(const ReadArgs &a, int bh, int row, int lane) {
@@ -632,6 +671,8 @@ struct RowJoin {
     for (int d = 1; d < 64; d <<= 1) { used += __shfl_xor(used, d); sum += __shfl_xor(sum, d); }
     inv = used != 0.f ? 1.f / used : 0.f;
     lse = mu + (sum != 0.f ? __builtin_amdgcn_logf(sum) : 0.f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) f[k] = m[k] == -INFINITY && u[k] == 0.f ? -1.f : f[k];       // an empty slice: its accumulators may be anything
   }
 };
 
@@ -658,7 +699,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
       for (int s0 = 0; s0 < a.nsplit; s0 += 64 / QL) {
         const int s = s0 + lane / QL;
         const float f0 = __shfl(J.f[0], s & 63), f1 = __shfl(J.f[1], s & 63), f = s < 64 ? f0 : f1;
-        if (s < a.nsplit && f != 0.f) acc += f * *reinterpret_cast<const f32x4 *>(part + s * stride + dv);     // (an empty slice's accumulators may be anything)
+        if (s < a.nsplit && f >= 0.f) acc += f * *reinterpret_cast<const f32x4 *>(part + s * stride + dv);
       }
 #pragma unroll
       for (int d = QL; d < 64; d <<= 1)
@@ -777,14 +818,14 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   return MIVOS_OK;
 }
 
-template <int DK, int DVC, int PARTS, bool WEIGH>
+template <int DK, int DVC, int PARTS, bool WEIGH, bool CAUSAL>
 static int block_launch_one(const ReadArgs &a, const dim3 grid, hipStream_t s) {
   constexpr size_t lds = 2 * 64 * (DVC + 16) * 2;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
-    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, WEIGH>, lds, raised, "bank4_read")) return rc;
+    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, WEIGH, CAUSAL>, lds, raised, "bank4_read")) return rc;
   }
-  bank4_block_kernel<DK, DVC, PARTS, WEIGH><<<grid, 256, lds, s>>>(a);
+  bank4_block_kernel<DK, DVC, PARTS, WEIGH, CAUSAL><<<grid, 256, lds, s>>>(a);
   return MIVOS_OK;
 }
 
@@ -792,8 +833,8 @@ static int block_launch_one(const ReadArgs &a, const dim3 grid, hipStream_t s) {
 template <int DK, int DVC, int PARTS>
 static int block_launch(const ReadArgs &a, const dim3 grid, hipStream_t s) {
   if constexpr (PARTS == 1)
-    if (a.weigh) return block_launch_one<DK, DVC, 1, true>(a, grid, s);
-  return block_launch_one<DK, DVC, PARTS, false>(a, grid, s);
+    if (a.weigh) return a.causal ? block_launch_one<DK, DVC, 1, true, true>(a, grid, s) : block_launch_one<DK, DVC, 1, true, false>(a, grid, s);
+  return a.causal ? block_launch_one<DK, DVC, PARTS, false, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, false, false>(a, grid, s);
 }
 
 template <int DK, int PARTS>
@@ -861,7 +902,7 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
                                 void *stream) {
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
-  if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out))) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument");
+  if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out)) || !(scale > -INFINITY && scale < INFINITY)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument");
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
   if (p.rows == 0) return MIVOS_OK;
   const int64_t need = p.part_o + p.part_ml + p.logits + p.lse + p.q_pack;
@@ -879,10 +920,10 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   a.slots = bank->slots; a.logit_stride = p.logit_stride; a.lse_stride = p.lse_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
   a.key_dim = bank->key_dim; a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
-  // logits are compared before they are scaled: a scale above 0, its sign with the queries (0 itself as 2^-100: every weight rounds to 1)
+  // logits are compared before they are scaled: a scale above 0, its sign with the queries (0 itself as 2^-126: every weight rounds to 1)
   a.q_sign = scale < 0.f ? -1.f : 1.f;
   a.scale_log2 *= a.q_sign;
-  if (a.scale_log2 < 0x1p-100f) a.scale_log2 = 0x1p-100f;
+  if (a.scale_log2 < 0x1p-126f) a.scale_log2 = 0x1p-126f;
   a.q_vec = (((qb | qt | qh) * dtype_bytes(dtype)) & 15) == 0 && ((uintptr_t)q & 15) == 0;
   if (int rc = bank->key_dim == 64 ? read_launch<64>(a, p, dtype, s) : bank->key_dim == 128 ? read_launch<128>(a, p, dtype, s) : read_launch<256>(a, p, dtype, s))
     return rc;

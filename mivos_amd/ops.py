@@ -9,6 +9,7 @@ import contextlib
 import ctypes as C
 import decimal
 import functools
+import math
 import struct
 
 import torch
@@ -177,7 +178,6 @@ class ConvLayer:
 
     def _f16x3_scale(self):
         """(2^s, scale * 2^-s): the exact power-of-two pre-scaling of the fp16 hi/lo weight split."""
-        import math
         wmax = float(self.w.abs().max())
         s = 14 - math.floor(math.log2(wmax)) if wmax > 0 else 0     # max |w * 2^s| in [2^14, 2^15)
         mult = 2.0 ** s
@@ -1237,6 +1237,10 @@ def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, plan, eps=1e-6
     return gq, gk, wq, wk
 
 
+def _overlap(x, y):
+    return x[0] < y[1] and y[0] < x[1]
+
+
 class Bank4:
     """A memory bank in 4 bits: per (stream, head, slot) a key row and a value row of blocks of 32 channels, one power-of-two scale a block
     (`mivos_bank4` in include/mivos_hip.h has the format: 17 bytes for 32 channels), the attention weight the slot has received, and the
@@ -1244,7 +1248,12 @@ class Bank4:
     keep and read): codes uint8 [B, H, S, D / 2], scales uint8 [B, H, S, D / 32], weight fp32 [B, H, S], lens int32 [B].  Calls on one bank
     belong to one stream at a time."""
     __slots__ = ("key_codes", "key_scales", "value_codes", "value_scales", "weight", "lens", "status", "batch", "heads", "slots", "key_dim",
-                 "value_dim", "_desc", "_storages")
+                 "value_dim", "_desc", "_storages", "_ranges")
+
+    def __setattr__(self, name, value):
+        if hasattr(self, name):      # the kernels hold the addresses
+            raise MivosHipError(f"Bank4: the bank's {name} is fixed; write into it, or make another bank")
+        object.__setattr__(self, name, value)
 
     def __init__(self, key_codes, key_scales, value_codes, value_scales, weight, lens):
         if key_codes.dim() != 4 or value_codes.dim() != 4:
@@ -1271,7 +1280,8 @@ class Bank4:
         buffers = (key_codes, key_scales, value_codes, value_scales, weight, lens, self.status)
         self._desc = Bank4Desc(*(t.data_ptr() for t in buffers), s, b, h, dk, dv)
         self._storages = frozenset(t.untyped_storage().data_ptr() for t in buffers)
-        if len(self._storages) != len(buffers):
+        self._ranges = tuple((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in buffers)
+        if len(self._storages) != len(buffers) and any(_overlap(x, y) for i, x in enumerate(self._ranges) for y in self._ranges[:i]):
             raise MivosHipError("Bank4: the buffers share memory")
 
     @classmethod
@@ -1339,6 +1349,9 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
     if hq < 1 or hq % bank.heads:
         raise MivosHipError(f"{hq} query heads over {bank.heads} bank heads")
     code = _dtype_code(queries)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise MivosHipError(f"bank4_read: scale {scale}")
     if count is not None:
         _int32_vector(count, b, "count")
     lib = _lib.load()
@@ -1349,7 +1362,7 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
     out = queries.new_empty((b, t, hq, bank.value_dim))
     ws = queries.new_empty(need, dtype=torch.uint8) if need else None
     check(lib.mivos_bank4_read(bank._desc, queries.data_ptr(), qb, qt, qh, code, hq, t, None if count is None else count.data_ptr(),
-                               d ** -0.5 if scale is None else float(scale), causal, weigh, out.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                               scale, causal, weigh, out.data_ptr(), None if ws is None else ws.data_ptr(), need,
                                _stream()))
     return out
 
@@ -1361,7 +1374,7 @@ def bank4_evict(bank, keep, out, first=0, recent=0):
     they came from, int32 [B, H, keep] (-1 behind out.lens).  Two banks used in turn keep a stream within its budget."""
     if (out.batch, out.heads, out.key_dim, out.value_dim) != (bank.batch, bank.heads, bank.key_dim, bank.value_dim):
         raise MivosHipError("bank4_evict: the two banks differ in streams, heads or channels")
-    if bank._storages & out._storages:
+    if bank is out or (bank._storages & out._storages and any(_overlap(x, y) for x in bank._ranges for y in out._ranges)):
         raise MivosHipError("bank4_evict: the two banks share memory")
     if not 1 <= keep <= out.slots or first < 0 or recent < 0 or first + recent > keep:
         raise MivosHipError(f"bank4_evict: keep {keep} of {out.slots} slots, first {first}, recent {recent}")

@@ -365,6 +365,29 @@ def test_read_not_a_number_block():
     assert bool(got[0, 20:].isnan().all()) and not bool(got[0, :20].isnan().any()) and not bool(got[1].isnan().any())
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("dv,tokens", [(64, 20), (64, 90), (128, 20), (256, 90)])
+def test_read_not_a_number_values(dv, tokens, dtype):
+    """A value block that stands for NaN: its 32 channels are NaN for the rows that see the slot, no others; what no row sees yet may hold anything."""
+    bank = _filled(2, 1, 200, 64, dv, (200, 150))
+    for b, slot, blk in ((0, 190, dv // 32 - 1), (0, 199, 0), (1, 149 - tokens // 2, 1)):
+        bank.value_scales[b, 0, slot, blk] = 255
+    q = torch.randn(2, tokens, 1, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    got = _check_read(bank, q, True, None, True).isnan().cpu()
+    assert int(got[0, tokens - 10, 0].sum()) == 32 and int(got[0, tokens - 11].sum()) == 0 and int(got[0, -1, 0].sum()) == 64
+    assert int(got[1].sum()) == 32 * (tokens - (tokens - 1 - tokens // 2))
+    _check_read(bank, q, False, None, False)
+
+
+def test_read_huge_logits_with_zero_scale_and_split_banks():
+    """scale = 0: every slot weighs the same; a bank long enough for many slices, one of them far ahead of the others."""
+    bank = _filled(1, 1, 9000, 64, 64, (8999,), spread=30.0)
+    for rows in (3, 80):
+        q = 100 * torch.randn(1, rows, 1, 64, generator=torch.Generator().manual_seed(3))
+        _check_read(bank, q, False, None, True, scale=0.0)
+        _check_read(bank, q, True, None, True)
+
+
 def test_read_same_twice_and_tokens_zero():
     bank = _filled(1, 2, 900, 128, 128, (900,))
     q = torch.randn(1, 33, 8, 128, generator=torch.Generator().manual_seed(3)).bfloat16().to(DEV)

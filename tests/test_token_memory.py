@@ -127,6 +127,17 @@ def test_bank_refusals():
         _raises("no CPU fallback", call)
 
 
+def test_bank_buffers_are_fixed_and_may_come_from_one_allocation():
+    b = _bank()
+    _raises("fixed", setattr, b, "lens", torch.zeros(2, dtype=torch.int32))
+    whole = torch.zeros(2, 2, 2, 16, 32, dtype=torch.uint8)          # codes of keys and values side by side
+    c = ops.Bank4(whole[0], b.key_scales, whole[1], b.value_scales, b.weight, b.lens)
+    _raises("share memory", ops.bank4_evict, b, 8, c)
+    _raises("share memory", ops.Bank4, whole[0], b.key_scales, whole[0], b.value_scales, b.weight, b.lens)
+    for scale in (math.inf, math.nan):
+        _raises("scale", ops.bank4_read, b, torch.zeros(2, 1, 2, 64), scale=scale)
+
+
 def test_c_entries_check_their_arguments_without_a_gpu():
     """The C ABI's own checks (a caller other than the Python wrappers): status codes, no launch."""
     import ctypes as C
