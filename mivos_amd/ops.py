@@ -1056,13 +1056,14 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # mivos_d
 
 
 def _here(ref, *others):
-    """All operands on one device, and that device the current gfx950 (_ensure_device)."""
+    """All operands on one device, and that device the current gfx950 (_ensure_device) -> its current stream."""
     index = ref.get_device()
     for t in others:
         if t is not None and t.get_device() != index:
             raise MivosHipError(f"operands live on {ref.device} and {t.device}")
-    if index not in _checked_devices or index != torch.cuda.current_device():
+    if index not in _checked_devices or index != torch._C._cuda_getDevice():
         _ensure_device(ref)
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _dtype_code(t):
@@ -1170,9 +1171,17 @@ def _norm_weight(w, ref, name):
     return w
 
 
+@functools.lru_cache(maxsize=None)
+def _packed_entry(name):
+    """The entry point taking its descriptor as packed bytes."""
+    entry = _lib.load()[name]
+    entry.restype, entry.argtypes = C.c_int, [C.c_char_p, C.c_void_p]
+    return entry
+
+
 def _rotary(q, k, positions, plan, inverse, eps, q_weight=None, k_weight=None):
     code, (b, n, hq, d, qb, qn, qh), kd = _rotary_check(q, k, positions, plan)
-    _here(q, k, positions, plan.freq, q_weight, k_weight)
+    stream = _here(q, k, positions, plan.freq, q_weight, k_weight)
     yq = torch.empty_like(q, memory_format=torch.contiguous_format)
     yk, k_rows = None, _NO_ROWS
     if k is not None:
@@ -1180,7 +1189,9 @@ def _rotary(q, k, positions, plan, inverse, eps, q_weight=None, k_weight=None):
         k_rows = (k.data_ptr(), 0, yk.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), *kd[4:], 0, 0, 0, kd[2], 0)
     desc = _ROTARY.pack(q.data_ptr(), 0, yq.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), qb, qn, qh, 0, 0, 0, hq, 0, *k_rows,
                         positions.data_ptr(), *plan.tables, 0, *positions.stride(), 0, b, n, d, plan.pairs, code, plan.interleaved, inverse, eps)
-    check(_lib.load().mivos_rotary_axes(RotaryDesc.from_buffer_copy(desc), _stream()))
+    rc = _packed_entry("mivos_rotary_axes")(desc, stream)
+    if rc:
+        check(rc)
     return yq, yk
 
 
@@ -1222,7 +1233,7 @@ def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, plan, eps=1e-6
         if g is not None and g.dtype != q.dtype:
             raise MivosHipError(f"q is {q.dtype}, its gradient {g.dtype}")
     code, (b, n, hq, d, qb, qn, qh), kd = _rotary_check(q, k, positions, plan)
-    _here(q, k, positions, plan.freq, dq, dk, q_weight, k_weight)
+    stream = _here(q, k, positions, plan.freq, dq, dk, q_weight, k_weight)
     lib = _lib.load()
     need = lib.mivos_norm_rotary_grad_workspace_bytes(d)
     ws = q.new_empty(need, dtype=torch.uint8)
@@ -1233,7 +1244,7 @@ def norm_rotary_grad(dq, dk, q, k, q_weight, k_weight, positions, plan, eps=1e-6
         k_rows = (k.data_ptr(), dk.data_ptr(), gk.data_ptr(), k_weight.data_ptr(), *kd[4:], *kg, kd[2], 0)
     desc = _ROTARY.pack(q.data_ptr(), dq.data_ptr(), gq.data_ptr(), q_weight.data_ptr(), qb, qn, qh, *qg, hq, 0, *k_rows, positions.data_ptr(),
                         *plan.tables, ws.data_ptr(), *positions.stride(), need, b, n, d, plan.pairs, code, plan.interleaved, 1, eps)
-    check(lib.mivos_norm_rotary_grad(RotaryDesc.from_buffer_copy(desc), wq.data_ptr(), None if wk is None else wk.data_ptr(), _stream()))
+    check(lib.mivos_norm_rotary_grad(RotaryDesc.from_buffer_copy(desc), wq.data_ptr(), None if wk is None else wk.data_ptr(), stream))
     return gq, gk, wq, wk
 
 
@@ -1317,9 +1328,9 @@ def bank4_append(bank, keys, values, at=None, count=None):
             raise MivosHipError("at overlaps the bank's lengths")
     if count is not None and abs(_int32_vector(count, bank.batch, "count").data_ptr() - bank._desc.lens) < 4 * bank.batch:
         raise MivosHipError("count overlaps the bank's lengths")
-    _here(bank.lens, keys, values, at, count)
+    stream = _here(bank.lens, keys, values, at, count)
     check(_lib.load().mivos_bank4_append(bank._desc, keys.data_ptr(), kb, kt, kh, values.data_ptr(), vb, vt, vh, code, at.data_ptr(),
-                                         None if count is None else count.data_ptr(), tokens, _stream()))
+                                         None if count is None else count.data_ptr(), tokens, stream))
 
 
 def bank4_values(bank, first=None, count=None, dtype=torch.bfloat16):
@@ -1332,11 +1343,11 @@ def bank4_values(bank, first=None, count=None, dtype=torch.bfloat16):
         raise MivosHipError(f"bank4_values: {count} of {bank.slots} slots")
     if first is not None:
         _int32_vector(first, bank.batch, "first")
-    _here(bank.lens, first)
+    stream = _here(bank.lens, first)
     keys = bank.lens.new_empty((bank.batch, bank.heads, count, bank.key_dim), dtype=dtype)
     values = bank.lens.new_empty((bank.batch, bank.heads, count, bank.value_dim), dtype=dtype)
     check(_lib.load().mivos_bank4_values(bank._desc, None if first is None else first.data_ptr(), count, keys.data_ptr(), values.data_ptr(), _DTYPES[dtype],
-                                         _stream()))
+                                         stream))
     return keys, values
 
 
@@ -1358,12 +1369,12 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
     need = lib.mivos_bank4_read_workspace_bytes(bank._desc, hq, t, code, weigh)
     if need < 0:
         check(int(need))
-    _here(bank.lens, queries, count)
+    stream = _here(bank.lens, queries, count)
     out = queries.new_empty((b, t, hq, bank.value_dim))
     ws = queries.new_empty(need, dtype=torch.uint8) if need else None
     check(lib.mivos_bank4_read(bank._desc, queries.data_ptr(), qb, qt, qh, code, hq, t, None if count is None else count.data_ptr(),
                                scale, causal, weigh, out.data_ptr(), None if ws is None else ws.data_ptr(), need,
-                               _stream()))
+                               stream))
     return out
 
 
@@ -1378,7 +1389,7 @@ def bank4_evict(bank, keep, out, first=0, recent=0):
         raise MivosHipError("bank4_evict: the two banks share memory")
     if not 1 <= keep <= out.slots or first < 0 or recent < 0 or first + recent > keep:
         raise MivosHipError(f"bank4_evict: keep {keep} of {out.slots} slots, first {first}, recent {recent}")
-    _here(bank.lens, out.lens)
+    stream = _here(bank.lens, out.lens)
     slots = bank.lens.new_empty((bank.batch, bank.heads, keep))
-    check(_lib.load().mivos_bank4_evict(bank._desc, out._desc, keep, first, recent, slots.data_ptr(), _stream()))
+    check(_lib.load().mivos_bank4_evict(bank._desc, out._desc, keep, first, recent, slots.data_ptr(), stream))
     return slots
