@@ -16,7 +16,11 @@
 namespace mivos {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int BLOCK_ROWS_MIN = 65;   // rows a bank head from which the 128-row kernel runs
+// Rows a bank head from which the 128-row kernel runs.  Both kernels, us without / with the weights gathered (bf16; 16-row tiles | 128 rows):
+//   4 heads x 16 384 slots, 2 streams   32 rows 35 / 44 | 28 / 34     64 rows 45 / 69 | 30 / 36     200 rows 57 / 169 | 41 / 52
+//   2 heads x 65 536 slots              32 rows 41 / 46 | 45 / 50     64 rows 46 / 64 | 44 / 50     200 rows 66 / 188 | 57 / 68
+//   8 heads x 4096 slots x 64, 4        32 rows 15 / 39 | 17 / 22     64 rows 23 / 64 | 19 / 24     200 rows 35 / 157 | 30 / 40
+constexpr int BLOCK_ROWS_MIN = 33;
 
 struct ReadArgs {
   const uint8_t *kc, *ks, *vc, *vs;
@@ -796,7 +800,7 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
     // Slices of a row tile's slots: the fewest rounds of the workgroups that run at once (two a CU where their registers allow it), a slice
     // costing its join (its accumulators are written and read once more) and its start.
     const int at_once = 256 * block_occupancy(k->key_dim, p->dvc, dtype);
-    const int most = (int)(k->slots / 512 < 1 ? 1 : k->slots / 512 > 32 ? 32 : k->slots / 512);
+    const int most = (int)(k->slots / 512 < 1 ? 1 : k->slots / 512 > 128 ? 128 : k->slots / 512);     // (8 steps a slice pay for its start)
     double best = 1e30;
     for (int n = 1; n <= most; ++n) {
       const double cost = (double)((groups * n + at_once - 1) / at_once) / n * (1 + 0.01 * n);
