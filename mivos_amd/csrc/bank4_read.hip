@@ -29,9 +29,9 @@ struct ReadArgs {
   const void *q;
   void *out;
   int64_t qb, qt, qh;
-  float *part_o, *part_ml, *logits, *lse;
+  float *part_o, *part_ml, *logits, *row_max, *row_inv;
   __bf16 *q_pack;
-  int64_t slots, logit_stride, lse_stride;
+  int64_t slots, logit_stride, row_stride;
   int batch, heads, group, tokens, rows, key_dim, value_dim, nsplit, causal, weigh, q_vec;
   float scale_log2;       // |scale| * log2(e): the softmax runs in powers of two; the sign of scale goes to the queries
   float q_sign;
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
     if (a.logits && chunk == 0 && r < a.rows)
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
-        *reinterpret_cast<f32x4 *>(a.logits + ((int64_t)bh * a.rows + r) * a.logit_stride + base + kt * 16 + grp * 4) = x[kt] * a.scale_log2;
+        *reinterpret_cast<f32x4 *>(a.logits + ((int64_t)bh * a.rows + r) * a.logit_stride + base + kt * 16 + grp * 4) = x[kt];
     float top = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) top = fmaxf(top, fmaxf(fmaxf(x[kt][0], x[kt][1]), fmaxf(x[kt][2], x[kt][3])));
@@ -561,7 +561,8 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   }
 }
 
-// weight[s] += sum over the rows of exp2(logit - lse[row]): the logits once more, now S = Q K^T, so that a lane holds one slot and its sum
+// weight[s] += sum over the rows of exp2(logit - maximum) / sum, each row's maximum and 1 / sum from bank4_join (one number, their logarithm
+// together, would cost every weight of a row 2^-24 of it): the logits once more, now S = Q K^T, so that a lane holds one slot and its sum
 // runs over registers, the rows in order.  One workgroup: 128 * NS slots, NS x 32 a wave, their keys widened once into registers; 32 rows a
 // step go through LDS, copied as bank4_join has packed them in operand order.  (A wave that reads its rows as they lie in memory touches a
 // cache line a lane and load, and with 64 slots a workgroup the queries cross the L2 1.3 GB at 1620 x 32 400 x 2: 150 and 115 us.)
@@ -590,8 +591,8 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   float acc[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) acc[s] = 0.f;
-  const u32x4 *q = reinterpret_cast<const u32x4 *>(a.q_pack) + (int64_t)bh * (a.lse_stride / 32) * TILE + tid;
-  const float *lse = a.lse + (int64_t)bh * a.lse_stride + half * 4;          // (rows behind the last hold anything: not added)
+  const u32x4 *q = reinterpret_cast<const u32x4 *>(a.q_pack) + (int64_t)bh * (a.row_stride / 32) * TILE + tid;
+  const float *row_max = a.row_max + (int64_t)bh * a.row_stride + half * 4, *row_inv = a.row_inv + (int64_t)bh * a.row_stride + half * 4;      // (rows behind the last hold anything: not added)
   const int tiles = (rows + 31) / 32;
   int tile0 = 0;                                        // causal: the first rows that see the workgroup's first slot
   if (a.causal) {
@@ -607,9 +608,12 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
 #pragma unroll
     for (int i = 0; i < TL; ++i) next[i] = q[(int64_t)more * TILE + i * 256];
     const int r0 = tile * 32;
-    f32x4 shift[4];
+    f32x4 shift[4], inv[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) shift[g] = *reinterpret_cast<const f32x4 *>(lse + r0 + g * 8);
+    for (int g = 0; g < 4; ++g) {
+      shift[g] = *reinterpret_cast<const f32x4 *>(row_max + r0 + g * 8);
+      inv[g] = *reinterpret_cast<const f32x4 *>(row_inv + r0 + g * 8);
+    }
     f32x16 x[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s)
@@ -630,7 +634,7 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
         const int row = r0 + mfma32_row(j, lane), lim = row < rows ? (int)read_limit(a, len, cnt, row / a.group) : 0;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4]));
+          const float p = inv[j / 4][j % 4] * __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4]));
           acc[s] += base + s * 32 + col < lim ? p : 0.f;
         }
       }
@@ -638,7 +642,8 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
 #pragma unroll
-        for (int s = 0; s < NS; ++s) acc[s] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4]));
+        for (int s = 0; s < NS; ++s)
+          acc[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4])), inv[j / 4][j % 4], acc[s]);
     }
 #pragma unroll
     for (int i = 0; i < TL; ++i) qs[(buf ^ 1) * TILE + i * 256 + tid] = next[i];
@@ -652,10 +657,11 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   }
 }
 
-// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum and log2 of the sum of the weights, and the
+// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum of the weights as the output uses them, 1 / their
+// exact sum, and the
 // factors of its slices' accumulators (-1: an empty slice).
 struct RowJoin {
-  float f[2], inv, lse;
+  float f[2], inv, top, inv_sum;
   __device__ __forceinline__ RowJoin(const ReadArgs &a, int bh, int row, int lane) {
     const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + row) * 4;
     float m[2], u[2], l[2];
@@ -675,7 +681,8 @@ struct RowJoin {
     float used = f[0] * u[0] + f[1] * u[1], sum = f[0] * l[0] + f[1] * l[1];
     for (int d = 1; d < 64; d <<= 1) { used += __shfl_xor(used, d); sum += __shfl_xor(sum, d); }
     inv = used != 0.f ? 1.f / used : 0.f;
-    lse = mu + (sum != 0.f ? __builtin_amdgcn_logf(sum) : 0.f);
+    top = mu;
+    inv_sum = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) f[k] = m[k] == -INFINITY && u[k] == 0.f ? -1.f : f[k];       // an empty slice: its accumulators may be anything
   }
@@ -693,7 +700,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
     if (g >= (int64_t)a.batch * a.heads * a.rows) return;
     const int bh = (int)(g / a.rows), row = (int)(g - (int64_t)bh * a.rows), b = bh / a.heads, h = bh - b * a.heads;
     const RowJoin J(a, bh, row, lane);
-    if (a.lse && lane == 0) a.lse[(int64_t)bh * a.lse_stride + row] = J.lse;
+    if (a.row_max && lane == 0) { a.row_max[(int64_t)bh * a.row_stride + row] = J.top; a.row_inv[(int64_t)bh * a.row_stride + row] = J.inv_sum; }
     const int t = row / a.group, j = h * a.group + row - t * a.group;
     T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + j) * a.value_dim;
     const float *part = a.part_o + ((int64_t)bh * a.nsplit * a.rows + row) * a.value_dim;
@@ -721,7 +728,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
     return;
   }
   if (a.q_pack) {                     // 32 rows a wave, as bf16 parts in the order of bank4_weigh's operand
-    const int tiles = (int)(a.lse_stride / 32), KS = a.key_dim / 16;
+    const int tiles = (int)(a.row_stride / 32), KS = a.key_dim / 16;
     const int64_t g = (int64_t)(blockIdx.x - out_blocks) * 4 + wave;
     if (g >= (int64_t)a.batch * a.heads * tiles) return;
     const int bh = (int)(g / tiles), tile = (int)(g - (int64_t)bh * tiles), b = bh / a.heads, h = bh - b * a.heads, half = lane >> 5;
@@ -740,7 +747,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
     }
     return;
   }
-  __shared__ float lse[BLOCK_ROWS_MIN];
+  __shared__ float top[BLOCK_ROWS_MIN], inv[BLOCK_ROWS_MIN];
   __shared__ int lim[BLOCK_ROWS_MIN];
   const int per = (int)((a.slots + 1023) / 1024), g = blockIdx.x - out_blocks, bh = g / per, b = bh / a.heads;
   const int64_t slot = (int64_t)(g - bh * per) * 1024 + tid * 4;
@@ -749,7 +756,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
   const int cnt = read_count(a, b);
   for (int i = wave; i < a.rows; i += 4) {
     const RowJoin J(a, bh, i, lane);
-    if (lane == 0) { lse[i] = J.lse; lim[i] = (int)read_limit(a, len, cnt, i / a.group); }
+    if (lane == 0) { top[i] = J.top; inv[i] = J.inv_sum; lim[i] = (int)read_limit(a, len, cnt, i / a.group); }
   }
   __syncthreads();
   if (slot >= len) return;
@@ -759,7 +766,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
   for (int i = 0; i < a.rows; ++i) {
     const f32x4 x = *reinterpret_cast<const f32x4 *>(x0 + (int64_t)i * a.logit_stride);   // written up to the row's limit only
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] += slot + j < lim[i] ? __builtin_amdgcn_exp2f(x[j] - lse[i]) : 0.f;
+    for (int j = 0; j < 4; ++j) acc[j] += slot + j < lim[i] ? inv[i] * __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], a.scale_log2, -top[i])) : 0.f;
   }
   float *w = a.weight + (int64_t)bh * a.slots + slot;
 #pragma unroll
@@ -772,7 +779,7 @@ struct ReadPlan {
   int rows, tiles, nsplit, nvc, dvc;
   bool block;                        // 128 rows a workgroup (else 16)
   bool parts;                        // partial results go through the workspace
-  int64_t part_o, part_ml, logits, lse, q_pack, logit_stride, lse_stride;      // bytes; strides in elements
+  int64_t part_o, part_ml, logits, row_stat, q_pack, logit_stride, row_stride;      // bytes; strides in elements
 };
 
 
@@ -817,9 +824,9 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   p->part_ml = p->parts ? n * 16 : 0;
   p->logit_stride = (k->slots + 63) / 64 * 64;
   p->logits = weigh && !p->block ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
-  p->lse_stride = (rows + 31) / 32 * 32;
-  p->lse = weigh && p->block ? (int64_t)k->batch * k->heads * p->lse_stride * 4 : 0;
-  p->q_pack = p->lse / 4 * k->key_dim * 2 * (dtype == MIVOS_BF16 ? 1 : dtype == MIVOS_F16 ? 2 : 3);
+  p->row_stride = (rows + 31) / 32 * 32;
+  p->row_stat = weigh && p->block ? (int64_t)k->batch * k->heads * p->row_stride * 8 : 0;
+  p->q_pack = p->row_stat / 8 * k->key_dim * 2 * (dtype == MIVOS_BF16 ? 1 : dtype == MIVOS_F16 ? 2 : 3);
   return MIVOS_OK;
 }
 
@@ -899,7 +906,7 @@ extern "C" int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
-  return p.part_o + p.part_ml + p.logits + p.lse + p.q_pack;
+  return p.part_o + p.part_ml + p.logits + p.row_stat + p.q_pack;
 }
 
 extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t qb, int64_t qt, int64_t qh, int dtype, int q_heads, int tokens,
@@ -910,7 +917,7 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out)) || !(scale > -INFINITY && scale < INFINITY)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument");
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
   if (p.rows == 0) return MIVOS_OK;
-  const int64_t need = p.part_o + p.part_ml + p.logits + p.lse + p.q_pack;
+  const int64_t need = p.part_o + p.part_ml + p.logits + p.row_stat + p.q_pack;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: workspace of %lld bytes, 16-byte aligned", (long long)need);
   if (p.tiles > 65535 || (int64_t)bank->batch * bank->heads * p.nvc > 65535) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many row tiles");
@@ -921,8 +928,12 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   char *ws = (char *)workspace;
   if (p.parts) { a.part_o = (float *)ws; a.part_ml = (float *)(ws + p.part_o); }
   if (p.logits) a.logits = (float *)(ws + p.part_o + p.part_ml);
-  if (p.lse) { a.lse = (float *)(ws + p.part_o + p.part_ml); a.q_pack = (__bf16 *)(ws + p.part_o + p.part_ml + p.lse); }
-  a.slots = bank->slots; a.logit_stride = p.logit_stride; a.lse_stride = p.lse_stride;
+  if (p.row_stat) {
+    a.row_max = (float *)(ws + p.part_o + p.part_ml);
+    a.row_inv = a.row_max + p.row_stat / 8;
+    a.q_pack = (__bf16 *)(ws + p.part_o + p.part_ml + p.row_stat);
+  }
+  a.slots = bank->slots; a.logit_stride = p.logit_stride; a.row_stride = p.row_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
   a.key_dim = bank->key_dim; a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
   // logits are compared before they are scaled: a scale above 0, its sign with the queries (0 itself as 2^-126: every weight rounds to 1)
@@ -936,13 +947,13 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (!p.parts) return MIVOS_OK;
   const int64_t out_blocks = ((int64_t)a.batch * a.heads * a.rows + 3) / 4;
   int64_t blocks = out_blocks + (a.logits ? (int64_t)a.batch * a.heads * ((a.slots + 1023) / 1024) : 0);
-  if (a.q_pack) blocks += (a.batch * a.heads * (a.lse_stride / 32) + 3) / 4;
+  if (a.q_pack) blocks += (a.batch * a.heads * (a.row_stride / 32) + 3) / 4;
   if (blocks > 0x7fffffff) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many rows");
   if (dtype == MIVOS_BF16) join_launch<1>(a, (int)blocks, (int)out_blocks, s);
   else if (dtype == MIVOS_F16) join_launch<2>(a, (int)blocks, (int)out_blocks, s);
   else join_launch<3>(a, (int)blocks, (int)out_blocks, s);
   if (int rc = check_launch("bank4_read")) return rc;
-  if (!a.lse) return MIVOS_OK;
+  if (!a.row_max) return MIVOS_OK;
   if (int rc = bank->key_dim == 64 ? weigh_launch<64>(a, dtype, s) : bank->key_dim == 128 ? weigh_launch<128>(a, dtype, s) : weigh_launch<256>(a, dtype, s))
     return rc;
   return check_launch("bank4_read");
