@@ -137,11 +137,22 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 constexpr uint32_t KEY_STAYS = 0xffffffffu;
 
-constexpr int EVICT_THREADS = 1024, EVICT_WAVES = EVICT_THREADS / 64, EVICT_BINS = 2048, EVICT_COPIES = 4;
+constexpr int EVICT_THREADS = 1024, EVICT_WAVES = EVICT_THREADS / 64, EVICT_BINS = 2048;
 constexpr int EVICT_KEYS = 32;      // keys a lane holds: banks of up to 32 768 slots are read once
 
+__device__ __forceinline__ uint32_t waves_before(const uint32_t *v, int wave) {      // the sum over the waves before, all 16 read at once
+  uint32_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < EVICT_WAVES / 4; ++i) {
+    const u32x4 x = reinterpret_cast<const u32x4 *>(v)[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += 4 * i + j < wave ? x[j] : 0u;
+  }
+  return sum;
+}
+
 // Which slots of one (stream, head) stay: a radix select of the keep-th largest key (protected slots have the largest), 11 + 11 + 10 bits, the
-// counts in LDS (four copies: most weights of a bank share a few exponents, and a bin's increments are serial), then one ordered pass that
+// counts in LDS (copies of the counts against increments that meet in a bin gain nothing), then one ordered pass that
 // writes the kept slots ascending.  Equal weights: the lowest slots stay.  A wave owns a run of slots, so a slot's place follows from ballots
 // of its wave and one sum over the waves before: (larger keys before it) + min(equal ones before it, equal ones that stay).
 // One workgroup a (stream, head): bound by latency, 12 barriers and three passes of LDS counts (21 us at 21 060 slots; slots visited one
@@ -150,9 +161,8 @@ template <bool REGS>
 __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float *__restrict__ weight, const int32_t *__restrict__ lens, int heads, int64_t slots,
                                                                     int keep, int first, int recent, int32_t *__restrict__ slots_out,
                                                                     int32_t *__restrict__ lens_out) {
-  __shared__ uint32_t hist[EVICT_COPIES][EVICT_BINS];
-  __shared__ uint32_t sums[EVICT_WAVES], chosen[2];
-  __shared__ int larger[EVICT_WAVES], equal[EVICT_WAVES];
+  __shared__ uint32_t hist[EVICT_BINS], chosen[2];
+  __shared__ __align__(16) uint32_t sums[EVICT_WAVES], larger[EVICT_WAVES], equal[EVICT_WAVES];
   const int bh = blockIdx.x, b = bh / heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t n64 = lens[b];
   const int n = (int)(n64 < 0 ? 0 : n64 > slots ? slots : n64);
@@ -200,10 +210,10 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < EVICT_COPIES * EVICT_BINS; i += EVICT_THREADS) (&hist[0][0])[i] = 0;
+    for (int i = tid; i < EVICT_BINS; i += EVICT_THREADS) hist[i] = 0;
     __syncthreads();
     each([&](int i, uint32_t k) {
-      if ((k & mask) == prefix) atomicAdd(&hist[wave % EVICT_COPIES][(k >> shift) & (bins - 1)], 1u);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
     });
     __syncthreads();
     // thread t: bins 2 t, 2 t + 1 counted from the top
@@ -211,10 +221,7 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int bin = bins - 1 - (2 * tid + j);
-      c[j] = 0;
-      if (bin >= 0)
-#pragma unroll
-        for (int v = 0; v < EVICT_COPIES; ++v) c[j] += hist[v][bin];
+      c[j] = bin >= 0 ? hist[bin] : 0u;
       sum += c[j];
     }
     uint32_t before = sum;
@@ -224,8 +231,7 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
     }
     if (lane == 63) sums[wave] = before;
     __syncthreads();
-    before -= sum;
-    for (int v = 0; v < wave; ++v) before += sums[v];
+    before += waves_before(sums, wave) - sum;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       if (before < (uint32_t)want && (uint32_t)want <= before + c[j]) { chosen[0] = bins - 1 - (2 * tid + j); chosen[1] = before; }
@@ -244,8 +250,8 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
   });
   if (lane == 0) { larger[wave] = n_larger; equal[wave] = n_equal; }
   __syncthreads();
-  n_larger = n_equal = 0;
-  for (int v = 0; v < wave; ++v) { n_larger += larger[v]; n_equal += equal[v]; }
+  n_larger = (int)waves_before(larger, wave);
+  n_equal = (int)waves_before(equal, wave);
   each([&](int i, uint32_t k) {
     const uint64_t ba = __ballot(k > prefix), bt = __ballot(k == prefix);
     const int ties = n_equal + __builtin_amdgcn_mbcnt_hi((uint32_t)(bt >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bt, 0));
