@@ -34,7 +34,7 @@ struct ReadArgs {
   int64_t slots, logit_stride, row_stride;
   int batch, heads, group, tokens, rows, key_dim, value_dim, nsplit, causal, weigh, q_vec;
   float scale_log2;       // |scale| * log2(e): the softmax runs in powers of two; the sign of scale goes to the queries
-  float q_sign;
+  float q_sign;           // (0 where scale is: -inf * 0 of a masked logit is never formed)
 };
 
 __device__ __forceinline__ int64_t read_len(const ReadArgs &a, int b) {
@@ -374,15 +374,13 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   const int seen = row0 / a.group < cnt ? (int)read_limit(a, len, cnt, last_t) : 0;
   const int per = ((seen + 63) / 64 + a.nsplit - 1) / a.nsplit * 64;
   const int s0 = (int64_t)split * per < seen ? split * per : seen, s1 = seen - s0 < per ? seen : s0 + per;
-  int low = limit, high = live ? limit : 0;          // over the wave's rows
+  int low = limit;                                   // over the wave's rows
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int x = __shfl_xor(low, d), y = __shfl_xor(high, d);
+    const int x = __shfl_xor(low, d);
     low = x < low ? x : low;
-    high = y > high ? y : high;
   }
   low = __builtin_amdgcn_readfirstlane(low);
-  high = __builtin_amdgcn_readfirstlane(high);
 
   QueryCols<DK, PARTS> q;
   q.load((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign);
@@ -657,9 +655,8 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   }
 }
 
-// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum of the weights as the output uses them, 1 / their
-// exact sum, and the
-// factors of its slices' accumulators (-1: an empty slice).
+// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum of the weights as the output uses them,
+// 1 / their exact sum, and the factors of its slices' accumulators (-1: an empty slice).
 struct RowJoin {
   float f[2], inv, top, inv_sum;
   __device__ __forceinline__ RowJoin(const ReadArgs &a, int bh, int row, int lane) {
@@ -914,13 +911,18 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
                                 void *stream) {
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
-  if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out)) || !(scale > -INFINITY && scale < INFINITY)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument");
+  if (!dtype_ok(dtype) || (tokens > 0 && (!q || !out)) || !(scale >= -1e38f && scale <= 1e38f))
+    return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument (|scale| up to 1e38)");
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
   if (p.rows == 0) return MIVOS_OK;
   const int64_t need = p.part_o + p.part_ml + p.logits + p.row_stat + p.q_pack;
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: workspace of %lld bytes, 16-byte aligned", (long long)need);
   if (p.tiles > 65535 || (int64_t)bank->batch * bank->heads * p.nvc > 65535) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many row tiles");
+  // the join's workgroups: four rows each; then the weights of 1024 slots each, or four tiles of queries to pack
+  const int64_t heads = (int64_t)bank->batch * bank->heads, out_blocks = (heads * p.rows + 3) / 4;
+  const int64_t blocks = out_blocks + (p.logits ? heads * ((bank->slots + 1023) / 1024) : 0) + (p.q_pack ? (heads * (p.row_stride / 32) + 3) / 4 : 0);
+  if (p.parts && blocks >= 1 << 24) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many rows");
   hipStream_t s = (hipStream_t)stream;
   ReadArgs a{};
   a.kc = bank->key_codes; a.ks = bank->key_scales; a.vc = bank->value_codes; a.vs = bank->value_scales;
@@ -936,19 +938,14 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   a.slots = bank->slots; a.logit_stride = p.logit_stride; a.row_stride = p.row_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
   a.key_dim = bank->key_dim; a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
-  // logits are compared before they are scaled: a scale above 0, its sign with the queries (0 itself as 2^-126: every weight rounds to 1)
-  a.q_sign = scale < 0.f ? -1.f : 1.f;
-  a.scale_log2 *= a.q_sign;
-  if (a.scale_log2 < 0x1p-126f) a.scale_log2 = 0x1p-126f;
+  // logits are compared before they are scaled: a scale above 0, its sign (or the 0) with the queries
+  a.q_sign = scale < 0.f ? -1.f : scale > 0.f ? 1.f : 0.f;
+  a.scale_log2 = scale != 0.f ? a.scale_log2 * a.q_sign : 1.f;
   a.q_vec = (((qb | qt | qh) * dtype_bytes(dtype)) & 15) == 0 && ((uintptr_t)q & 15) == 0;
   if (int rc = bank->key_dim == 64 ? read_launch<64>(a, p, dtype, s) : bank->key_dim == 128 ? read_launch<128>(a, p, dtype, s) : read_launch<256>(a, p, dtype, s))
     return rc;
   if (int rc = check_launch("bank4_read")) return rc;
   if (!p.parts) return MIVOS_OK;
-  const int64_t out_blocks = ((int64_t)a.batch * a.heads * a.rows + 3) / 4;
-  int64_t blocks = out_blocks + (a.logits ? (int64_t)a.batch * a.heads * ((a.slots + 1023) / 1024) : 0);
-  if (a.q_pack) blocks += (a.batch * a.heads * (a.row_stride / 32) + 3) / 4;
-  if (blocks > 0x7fffffff) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many rows");
   if (dtype == MIVOS_BF16) join_launch<1>(a, (int)blocks, (int)out_blocks, s);
   else if (dtype == MIVOS_F16) join_launch<2>(a, (int)blocks, (int)out_blocks, s);
   else join_launch<3>(a, (int)blocks, (int)out_blocks, s);

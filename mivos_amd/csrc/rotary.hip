@@ -450,6 +450,6 @@ extern "C" int mivos_norm_rotary_grad(const mivos_rotary *d, float *dq_weight, f
     else if (d->dtype == MIVOS_F16) rotary_launch<_Float16, true>(a, p, s);
     else rotary_launch<__bf16, true>(a, p, s);
   }
-  rotary_weight_sum_kernel<<<dim3(cdiv(d->dim, 16), d->rows[1].heads ? 2 : 1), 256, 0, s>>>(a.partial, a.split, p.groups, d->dim, dq_weight, dk_weight);
+  rotary_weight_sum_kernel<<<dim3(cdiv(d->dim, 16), dk_weight ? 2 : 1), 256, 0, s>>>(a.partial, a.split, p.groups, d->dim, dq_weight, dk_weight);
   return check_launch("norm_rotary_grad");
 }

@@ -1262,7 +1262,7 @@ class Bank4:
                  "value_dim", "_desc", "_storages", "_ranges")
 
     def __setattr__(self, name, value):
-        if hasattr(self, name):      # the kernels hold the addresses
+        if hasattr(self, name) and getattr(self, name) is not value:      # the kernels hold the addresses; `bank.lens += n` writes into it
             raise MivosHipError(f"Bank4: the bank's {name} is fixed; write into it, or make another bank")
         object.__setattr__(self, name, value)
 
@@ -1361,7 +1361,7 @@ def bank4_read(bank, queries, scale=None, causal=False, count=None, weigh=False)
         raise MivosHipError(f"{hq} query heads over {bank.heads} bank heads")
     code = _dtype_code(queries)
     scale = d ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) <= 1e38:
         raise MivosHipError(f"bank4_read: scale {scale}")
     if count is not None:
         _int32_vector(count, b, "count")

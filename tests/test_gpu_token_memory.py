@@ -172,6 +172,19 @@ def test_rotary_empty_and_broadcast_positions():
     assert float((ops.rotary_axes(off, None, one.expand(3, 50, 3), plan)[0] - ref).abs().max()) <= 2.0 ** -19 * float(off.abs().max()) * 2
 
 
+def test_norm_rotary_gradient_without_key_heads():
+    """Keys of no heads: their weight's gradient is a sum over nothing, 0, whatever its memory held; both kernels."""
+    for dim in (64, 40):
+        plan, w = ops.RotaryAxes(dim, (8,), device=DEV), torch.ones(dim, device=DEV)
+        q, pos = torch.randn(2, 5, 2, dim, device=DEV), torch.zeros(2, 5, 1, dtype=torch.int32, device=DEV)
+        k = q[:, :, :0]
+        for t in [torch.full((dim,), float("nan"), device=DEV) for _ in range(8)]:      # (what the allocator hands out next)
+            del t
+        _, gk, gw, kw = ops.norm_rotary_grad(q, k, q, k, w, w, pos, plan)
+        assert gk.shape == k.shape and torch.equal(kw, torch.zeros_like(w))
+        assert torch.equal(gw, ops.norm_rotary_grad(q, None, q, None, w, None, pos, plan)[2])
+
+
 def test_norm_rotary_zero_rows():
     """A row of zeros: eps alone holds the norm; its gradient is w g / sqrt(eps)."""
     plan = ops.RotaryAxes(64, (32,), device=DEV)
@@ -386,6 +399,16 @@ def test_read_huge_logits_with_zero_scale_and_split_banks():
         q = 100 * torch.randn(1, rows, 1, 64, generator=torch.Generator().manual_seed(3))
         _check_read(bank, q, False, None, True, scale=0.0)
         _check_read(bank, q, True, None, True)
+
+
+@pytest.mark.parametrize("scale", (0.0, 2.0 ** -128, -2.0 ** -128))
+def test_read_scales_below_the_normal_numbers(scale):
+    """Logits of 2^122 ahead of the scale: a scale of 0 leaves equal weights, a subnormal one (exact in 32 bits) logits of 2^-6; both kernels."""
+    bank = _filled(1, 1, 300, 64, 64, (290,))
+    for rows in (3, 80):
+        q = 2.0 ** 118 * torch.randn(1, rows, 1, 64, generator=torch.Generator().manual_seed(3))
+        _check_read(bank, q, True, None, True, scale=scale)
+        _check_read(bank, q, False, None, True, scale=scale)
 
 
 def test_read_same_twice_and_tokens_zero():

@@ -130,11 +130,14 @@ def test_bank_refusals():
 def test_bank_buffers_are_fixed_and_may_come_from_one_allocation():
     b = _bank()
     _raises("fixed", setattr, b, "lens", torch.zeros(2, dtype=torch.int32))
+    lens = b.lens
+    b.lens += 3                                                      # writes into the buffer
+    assert b.lens is lens and lens.tolist() == [3, 3]
     whole = torch.zeros(2, 2, 2, 16, 32, dtype=torch.uint8)          # codes of keys and values side by side
     c = ops.Bank4(whole[0], b.key_scales, whole[1], b.value_scales, b.weight, b.lens)
     _raises("share memory", ops.bank4_evict, b, 8, c)
     _raises("share memory", ops.Bank4, whole[0], b.key_scales, whole[0], b.value_scales, b.weight, b.lens)
-    for scale in (math.inf, math.nan):
+    for scale in (math.inf, math.nan, 2e38, -2e38):
         _raises("scale", ops.bank4_read, b, torch.zeros(2, 1, 2, 64), scale=scale)
 
 
