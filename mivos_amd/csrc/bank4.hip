@@ -137,7 +137,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 constexpr uint32_t KEY_STAYS = 0xffffffffu;
 
-constexpr int EVICT_THREADS = 1024, EVICT_WAVES = EVICT_THREADS / 64, EVICT_BINS = 2048;
+constexpr int EVICT_THREADS = 1024, EVICT_WAVES = EVICT_THREADS / 64, EVICT_BINS = 2048, EVICT_COPIES = 4;
 constexpr int EVICT_KEYS = 32;      // keys a lane holds: banks of up to 32 768 slots are read once
 
 __device__ __forceinline__ uint32_t waves_before(const uint32_t *v, int wave) {      // the sum over the waves before, all 16 read at once
@@ -152,16 +152,17 @@ __device__ __forceinline__ uint32_t waves_before(const uint32_t *v, int wave) { 
 }
 
 // Which slots of one (stream, head) stay: a radix select of the keep-th largest key (protected slots have the largest), 11 + 11 + 10 bits, the
-// counts in LDS (copies of the counts against increments that meet in a bin gain nothing), then one ordered pass that
-// writes the kept slots ascending.  Equal weights: the lowest slots stay.  A wave owns a run of slots, so a slot's place follows from ballots
+// counts in LDS (four of each bin, by lane: most weights of a bank share a few exponents, and increments of one address are serial; one of each
+// takes 20 us instead of 18, the keys in LDS instead of registers no less), then one ordered pass that writes the kept slots ascending.  Equal weights: the lowest slots stay.  A wave owns a run of slots, so a slot's place follows from ballots
 // of its wave and one sum over the waves before: (larger keys before it) + min(equal ones before it, equal ones that stay).
-// One workgroup a (stream, head): bound by latency, 12 barriers and three passes of LDS counts (21 us at 21 060 slots; slots visited one
+// One workgroup a (stream, head): bound by latency, 12 barriers and three passes of LDS counts (18 us at 21 060 slots; slots visited one
 // 1024-wide row at a time with a scan each, and 8-bit digits, took 49 us).
 template <bool REGS>
 __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float *__restrict__ weight, const int32_t *__restrict__ lens, int heads, int64_t slots,
                                                                     int keep, int first, int recent, int32_t *__restrict__ slots_out,
                                                                     int32_t *__restrict__ lens_out) {
-  __shared__ uint32_t hist[EVICT_BINS], chosen[2];
+  __shared__ __align__(16) uint32_t hist[EVICT_BINS][EVICT_COPIES];
+  __shared__ uint32_t chosen[2];
   __shared__ __align__(16) uint32_t sums[EVICT_WAVES], larger[EVICT_WAVES], equal[EVICT_WAVES];
   const int bh = blockIdx.x, b = bh / heads, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t n64 = lens[b];
@@ -210,10 +211,10 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < EVICT_BINS; i += EVICT_THREADS) hist[i] = 0;
+    for (int i = tid; i < EVICT_BINS; i += EVICT_THREADS) *reinterpret_cast<u32x4 *>(hist[i]) = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
     each([&](int i, uint32_t k) {
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)][lane % EVICT_COPIES], 1u);
     });
     __syncthreads();
     // thread t: bins 2 t, 2 t + 1 counted from the top
@@ -221,7 +222,8 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int bin = bins - 1 - (2 * tid + j);
-      c[j] = bin >= 0 ? hist[bin] : 0u;
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(hist[bin >= 0 ? bin : 0]);
+      c[j] = bin >= 0 ? v[0] + v[1] + v[2] + v[3] : 0u;
       sum += c[j];
     }
     uint32_t before = sum;
