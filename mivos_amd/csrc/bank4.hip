@@ -84,7 +84,8 @@ __global__ __launch_bounds__(256) void bank4_append_kernel(mivos_bank4 bank, con
 }
 
 // ---------------------------------------------------------------------------------------------- values
-// Rows as in append, four in flight a thread: 104 us for 32 x 24 576 rows of 256 channels to bf16 (5.0 TB/s; one in flight: 113).
+// Rows as in append, four in flight a thread: 84 us for 32 x 24 576 rows of 256 channels to bf16 (6.1 TB/s,
+// nine tenths of it written; one in flight: 131).
 constexpr int VALUES_DEEP = 4;
 
 template <typename T>
@@ -265,7 +266,8 @@ __global__ __launch_bounds__(EVICT_THREADS) void bank4_select_kernel(const float
 }
 
 // Moves the kept rows: a thread a block of 32 channels, 16 bytes of codes; every fourth the scales of four blocks (WIDE: both rows have a
-// multiple of 128 channels; else each its own), the first the weight.  48 us for 32 x 24 576 rows of 256 channels (4.5 TB/s).
+// multiple of 128 channels; else each its own), the first the weight.  56 us for 32 x 24 576 of 32 768 rows of 256 channels
+// (3.9 TB/s of what is kept; stores among the loads: 67; a second row in flight a thread gains nothing).
 template <bool WIDE>
 __global__ __launch_bounds__(256) void bank4_move_kernel(mivos_bank4 from, mivos_bank4 to, int keep, const int32_t *__restrict__ slots) {
   const int bh = blockIdx.y;
@@ -282,17 +284,26 @@ __global__ __launch_bounds__(256) void bank4_move_kernel(mivos_bank4 from, mivos
   for (int64_t j = (int64_t)blockIdx.x * rows + r; j < keep; j += (int64_t)gridDim.x * rows) {
     const int64_t slot = from_slot[j];
     if (slot < 0) continue;
-    dc[j * nb] = sc[slot * nb];
-    if (!WIDE) ds[j * nb] = ss[slot * nb];
-    else if ((blk & 3) == 0) *reinterpret_cast<uint32_t *>(ds + j * nb) = *reinterpret_cast<const uint32_t *>(ss + slot * nb);
-    if (u == 0) to.weight[(int64_t)bh * to.slots + j] = from.weight[(int64_t)bh * from.slots + slot];
+    const u32x4 codes = sc[slot * nb];                 // (all loads ahead of the stores)
+    const bool scales = !WIDE || (blk & 3) == 0;
+    uint32_t scale = 0;
+    float w = 0.f;
+    if (scales) scale = WIDE ? *reinterpret_cast<const uint32_t *>(ss + slot * nb) : ss[slot * nb];
+    if (u == 0) w = from.weight[(int64_t)bh * from.slots + slot];
+    dc[j * nb] = codes;
+    if (WIDE && scales) *reinterpret_cast<uint32_t *>(ds + j * nb) = scale;
+    else if (!WIDE) ds[j * nb] = (uint8_t)scale;
+    if (u == 0) to.weight[(int64_t)bh * to.slots + j] = w;
   }
 }
 
-static int grid_x(int64_t rows, int at_once, int groups) {     // workgroups a (stream, head) of `at_once` rows each, up to 16 a CU over the launch
-  int64_t n = (rows + at_once - 1) / at_once, most = 256 * 16 / groups + 1;
+// Workgroups a stream (or a head of it) of `at_once` rows each, up to `most`.  Values and moves take one a row group (a launch that goes round
+// 16 a CU instead: 97 and 61 us instead of 84 and 56, at the sizes above), append up to 16 a CU, each of which reads the length and counts itself out.
+static int grid_x(int64_t rows, int at_once, int64_t most) {
+  const int64_t n = (rows + at_once - 1) / at_once;
   return (int)(n < 1 ? 1 : n > most ? most : n);
 }
+constexpr int64_t GRID_MOST = 1 << 20;
 
 }  // namespace mivos
 
@@ -306,7 +317,7 @@ extern "C" int mivos_bank4_append(const mivos_bank4 *bank, const void *keys, int
   const int units = (bank->key_dim + bank->value_dim) / 8, es = dtype_bytes(dtype);
   const int64_t all = kb | kt | kh | vb | vt | vh;
   const int vec = ((all * es) & 15) == 0 && (((uintptr_t)keys | (uintptr_t)values) & 15) == 0;
-  const dim3 grid(grid_x((int64_t)tokens * bank->heads, 256 / units, bank->batch), bank->batch);
+  const dim3 grid(grid_x((int64_t)tokens * bank->heads, 256 / units, 256 * 16 / bank->batch + 1), bank->batch);
   hipStream_t s = (hipStream_t)stream;
 #define GO(T) bank4_append_kernel<T><<<grid, 256, 0, s>>>(*bank, (const T *)keys, kb, kt, kh, (const T *)values, vb, vt, vh, vec, at, count, tokens, units)
   if (dtype == MIVOS_F32) GO(float);
@@ -322,7 +333,7 @@ extern "C" int mivos_bank4_values(const mivos_bank4 *bank, const int32_t *first,
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_values: bad argument");
   if (count == 0) return MIVOS_OK;
   const int rows = bank->batch * bank->heads, units = (bank->key_dim + bank->value_dim) / 8;
-  const dim3 grid(grid_x(count, VALUES_DEEP * (256 / units), rows), rows);
+  const dim3 grid(grid_x(count, VALUES_DEEP * (256 / units), GRID_MOST), rows);
   if (dtype == MIVOS_F32) bank4_values_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(*bank, first, (int)count, (float *)key_out, (float *)value_out);
   else bank4_values_kernel<__bf16><<<grid, 256, 0, (hipStream_t)stream>>>(*bank, first, (int)count, (__bf16 *)key_out, (__bf16 *)value_out);
   return check_launch("bank4_values");
@@ -346,7 +357,7 @@ extern "C" int mivos_bank4_evict(const mivos_bank4 *bank, const mivos_bank4 *out
   else
     bank4_select_kernel<false><<<rows, EVICT_THREADS, 0, s>>>(bank->weight, bank->lens, bank->heads, bank->slots, (int)keep, (int)first, (int)recent, slots_out, out->lens);
   if (int rc = check_launch("bank4_evict")) return rc;
-  const dim3 grid(grid_x(keep, a_row, rows), rows);
+  const dim3 grid(grid_x(keep, a_row, GRID_MOST), rows);
   if (bank->key_dim % 128 == 0 && bank->value_dim % 128 == 0) bank4_move_kernel<true><<<grid, 256, 0, s>>>(*bank, *out, (int)keep, slots_out);
   else bank4_move_kernel<false><<<grid, 256, 0, s>>>(*bank, *out, (int)keep, slots_out);
   return check_launch("bank4_evict");
