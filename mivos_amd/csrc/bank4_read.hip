@@ -11,6 +11,8 @@
 // mostly of one scale block, so K needs no staging; Q is kept in registers in the same channel order.  The result gives a lane one query
 // (column l % 16) and four keys a tile, which is the B operand of O^T = V^T P^T as it stands (the 8 keys of a lane in a pair of tiles are
 // the same 8 in both operands).  V rows are widened to bf16 in a wave's own LDS patch and read back transposed (ds_read_b64_tr_b16).
+#include <type_traits>
+
 #include "bank4.h"
 
 namespace mivos {
@@ -29,8 +31,10 @@ struct ReadArgs {
   const void *q;
   void *out;
   int64_t qb, qt, qh;
-  float *part_o, *part_ml, *logits, *row_max, *row_inv;
+  float *part_o, *part_ml, *logits, *row_max, *row_inv, *row_scale;
   __bf16 *q_pack;
+  _Float16 *q_pack_f16;
+  int32_t *redo;          // a flag a workgroup: fp16 products met a block that they do not hold, the bf16 ones do it again
   int64_t slots, logit_stride, row_stride;
   int batch, heads, group, tokens, rows, key_dim, value_dim, nsplit, causal, weigh, q_vec;
   float scale_log2;       // |scale| * log2(e): the softmax runs in powers of two; the sign of scale goes to the queries
@@ -58,16 +62,35 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-template <int PARTS>
-__device__ __forceinline__ void split8(f32x8 x, bf16x8 (&p)[PARTS]) {
+// x as a sum of PARTS bf16 or fp16 numbers
+template <typename E, int PARTS, typename V>
+__device__ __forceinline__ void split8_as(f32x8 x, V (&p)[PARTS]) {
 #pragma unroll
   for (int k = 0; k < PARTS; ++k)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[k][j] = (__bf16)x[j];
+      p[k][j] = (E)x[j];
       x[j] -= (float)p[k][j];
     }
 }
+template <int PARTS> __device__ __forceinline__ void split8(f32x8 x, bf16x8 (&p)[PARTS]) { split8_as<__bf16>(x, p); }
+template <int PARTS> __device__ __forceinline__ void split8(f32x8 x, f16x8 (&p)[PARTS]) { split8_as<_Float16>(x, p); }
+
+template <typename V> __device__ __forceinline__ V unpack8(uint32_t codes, float scale);
+template <> __device__ __forceinline__ bf16x8 unpack8<bf16x8>(uint32_t codes, float scale) { return bank4_unpack8(codes, scale); }
+template <> __device__ __forceinline__ f16x8 unpack8<f16x8>(uint32_t codes, float scale) { return bank4_unpack8_f16(codes, scale); }
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// Exponent of the power of two that brings a row of fp32 queries with the largest magnitude `top` to [2^13, 2^14) (rows below 2^-87: less far up)
+__device__ __forceinline__ int query_shift(float top) {
+  const int t = 13 + 127 - (int)(__float_as_uint(top) >> 23);
+  return t > 100 ? 100 : t < -114 ? -114 : t;
+}
+// what brings such a row's products to powers of two of a softmax weight; never 0 (a masked logit is -inf) nor infinite (a product may be 0):
+// where it is held back the products of fp16 blocks are far below 1 or far past every weight all the same
+__device__ __forceinline__ float row_scale(float scale_log2, float back) { return fminf(fmaxf(scale_log2 * back, 0x1p-126f), 0x1.fffffep127f); }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 .. 127
 
 template <int PARTS> struct ReadType;
 template <> struct ReadType<1> { typedef __bf16 T; };
@@ -84,8 +107,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t bank_rows(const uint8_t *p, in
 
 // The sum of a lane's softmax weights, as the second product uses them: bf16 queries round the weights, and the output is divided by the sum of
 // the rounded ones, so that what the rounding does to all of a row's weights alike drops out.
-template <int PARTS>
-__device__ __forceinline__ float weight_sum(float l, f32x8 p, const bf16x8 &pf) {
+template <int PARTS, typename V>
+__device__ __forceinline__ float weight_sum(float l, f32x8 p, const V &pf) {
   if constexpr (PARTS == 1) {
     const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
@@ -97,6 +120,8 @@ __device__ __forceinline__ float weight_sum(float l, f32x8 p, const bf16x8 &pf) 
   return l;
 }
 
+constexpr int block_occupancy(int dk, int dvc, int parts) { return parts == 1 && dk <= 128 && dvc <= 128 ? 2 : 1; }
+inline int query_parts(int dtype) { return dtype == MIVOS_BF16 ? 1 : dtype == MIVOS_F16 ? 2 : 3; }
 constexpr float MAX_LAG = 8.f;      // the running maximum follows a logit that passes it by more than this (powers of two): fewer rescales
 
 // ------------------------------------------------------------------------------------------ few rows: 16 a workgroup
@@ -315,24 +340,45 @@ struct KeyRow {
 #pragma unroll
       for (int i = 0; i < KI / 2; ++i) scales[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, col * (DK / 32), row * (DK / 32) + i * 4, 0) >> (8 * half);
   }
-  __device__ __forceinline__ float scale(int i) const { return bank4_scale((scales[i / 2] >> (16 * (i & 1))) & 255); }
+  __device__ __forceinline__ uint32_t byte(int i) const { return (scales[i / 2] >> (16 * (i & 1))) & 255; }
+  __device__ __forceinline__ float scale(int i) const { return bank4_scale(byte(i)); }
+  __device__ __forceinline__ bool fits_f16() const {
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) ok &= bank4_fits_f16(byte(i), codes[i]);
+    return ok;
+  }
 };
 
 // Queries of a lane (column l % 32), in the channel order of KeyRow.
-template <int DK, int PARTS>
+template <int DK, int PARTS, typename V>
 struct QueryCols {
-  bf16x8 f[DK / 16][PARTS];
-  template <typename T>
-  __device__ __forceinline__ void load(const T *row, int half, bool live, bool vec, float sign) {
+  V f[DK / 16][PARTS];
+  // SHIFT: the row times 2^t, t its query_shift -> 2^-t
+  template <bool SHIFT, typename T>
+  __device__ __forceinline__ float load(const T *row, int half, bool live, bool vec, float sign) {
+    auto channels = [&](int i) {
+      f32x8 x = load8(row + i / 4 * 64 + half * 32 + i % 4 * 8, vec);
 #pragma unroll
-    for (int i = 0; i < DK / 64; ++i)
+      for (int j = 0; j < 8; ++j) x[j] = live ? x[j] * sign : 0.f;
+      return x;
+    };
+    float up = 1.f, back = 1.f;
+    if constexpr (SHIFT) {
+      float top = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        f32x8 x = load8(row + i * 64 + half * 32 + u * 8, vec);
+      for (int i = 0; i < DK / 16; ++i) {
+        const f32x8 x = channels(i);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = live ? x[j] * sign : 0.f;
-        split8<PARTS>(x, f[i * 4 + u]);
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, __builtin_fabsf(x[j]));
       }
+      const int t = query_shift(fmaxf(top, __shfl_xor(top, 32)));
+      up = pow2(t);
+      back = pow2(-t);
+    }
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i) split8<PARTS>(SHIFT ? channels(i) * up : channels(i), f[i]);
+    return back;
   }
   __device__ __forceinline__ f32x16 dot(const KeyRow<DK> &k) const {       // [32 keys][32 queries]
     f32x16 c;
@@ -343,9 +389,9 @@ struct QueryCols {
       const float sc = k.scale(i);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const bf16x8 kf = bank4_unpack8(k.codes[i][u], sc);
+        const V kf = unpack8<V>(k.codes[i][u], sc);
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, f[i * 4 + u][p], c, 0, 0, 0);
+        for (int p = 0; p < PARTS; ++p) c = mfma32(kf, f[i * 4 + u][p], c);
       }
     }
     return c;
@@ -356,9 +402,18 @@ struct QueryCols {
 // codes straight into registers; the V rows are widened once for the workgroup into one of two LDS buffers while the matrix cores work on
 // the other.  S^T = K Q^T and O^T = V^T P^T on 32x32 products: a lane holds one query, 16 keys of each 32, and these are again the
 // operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^8.
-template <int DK, int DVC, int PARTS, bool WEIGH, bool CAUSAL>
-__global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1) void bank4_block_kernel(ReadArgs a) {
+// F16 (fp16 and fp32 queries): the products on fp16 numbers, which carry three bits more than bf16 ones - q in 1 / 2 of them (fp32 rows brought to
+// 2^14 first), the softmax weight times 2^12 in 2 (2^-22 of itself or 2^-37 of the row's largest; the maximum follows closer, by 2^3), where bf16 takes 2 / 3 and 2 / 3.  A 4-bit value
+// is exact in fp16 from 2^-24 to 6 * 2^13; a workgroup that meets a block outside raises its flag, and the bf16 kernel, launched behind, does that
+// workgroup's work again (the others leave at once).  2 x 1620 fp32 rows x 32 400 slots, 128 / 512: @F16@ us instead of 471.
+template <int DK, int DVC, int PARTS, bool F16, bool WEIGH, bool CAUSAL>
+__global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_block_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
+  typedef std::conditional_t<F16, f16x8, bf16x8> V8;
+  constexpr int QP = F16 ? PARTS - 1 : PARTS, PP = F16 ? 2 : PARTS;
+  constexpr bool SHIFT = F16 && PARTS == 3;
+  constexpr float LAG = F16 ? 3.f : MAX_LAG, P_UP = F16 ? 12.f : 0.f;        // weights are exp2(logit - (maximum - P_UP)), up to 2^(LAG + P_UP)
+  if (!F16 && a.redo && !a.redo[(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x]) return;
   constexpr int VS = DVC + 16, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB, VL = (VE + 255) / 256;
   extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
   __shared__ uint64_t nan_blocks[2][4][VL];            // causal: the value blocks of a buffer that stand for NaN, a bit a lane of the wave that stored it
@@ -382,8 +437,9 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   }
   low = __builtin_amdgcn_readfirstlane(low);
 
-  QueryCols<DK, PARTS> q;
-  q.load((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign);
+  QueryCols<DK, QP, V8> q;
+  const float back = q.template load<SHIFT>((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign);
+  const float scale = SHIFT ? row_scale(a.scale_log2, back) : a.scale_log2;
   f32x16 o[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -413,6 +469,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       vsn[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, tid / VB * vs_row + tid % VB, i * (256 / VB) * vs_row, 0);
     }
   };
+  bool outside = false;                                // F16: a block that fp16 does not hold
   auto store_values = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
@@ -422,12 +479,13 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
         break;
       }
       float sc = bank4_scale(vsn[i]);
+      if (F16) outside |= !bank4_fits_f16(vsn[i], vn[i]);
       if (CAUSAL) {
         nan_blocks[buf][wave][i] = __ballot(vsn[i] == kBank4NanScale);
         sc = vsn[i] == kBank4NanScale ? 1.f : sc;
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<bf16x8 *>(vt + (buf * 64 + vr) * VS + blk * 32 + j * 8) = bank4_unpack8(vn[i][j], sc);
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<V8 *>(vt + (buf * 64 + vr) * VS + blk * 32 + j * 8) = unpack8<V8>(vn[i][j], sc);
     }
   };
   // Causal: a value block that stands for NaN makes it NaN for the rows that see its slot and is finite for the others, whose weight there is 0.
@@ -457,7 +515,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
 #pragma unroll
     for (int j = 1; j < 16; ++j) t = fmaxf(fmaxf(t, x[0][j]), x[1][j]);
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
-    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * a.scale_log2;
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * scale;
   };
   auto settle = [&](f32x16 (&x)[2], int base) {      // masks the logits of a step that not all rows see, moves the maximum if it has to
     if (base + 64 > low || base + 64 > s1) {
@@ -468,7 +526,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
         for (int j = 0; j < 16; ++j) x[s][j] = base + s * 32 + mfma32_row(j, lane) < lim ? x[s][j] : -INFINITY;
       top = row_top(x);
     }
-    if (__any(top > m + MAX_LAG)) {
+    if (__any(top > m + LAG)) {
       const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
       l *= alpha;
@@ -481,16 +539,17 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
     if (CAUSAL) add_nans(buf, base);
     load_values(base + 64);                  // (behind the slice: nothing is read, zeros come back)
     load_keys(kn, base + 128);
-    const float mu = m == -INFINITY ? 0.f : m;
+    const float mu = m == -INFINITY ? 0.f : m - P_UP;
+    if (F16 && wave == 0) outside |= !k[0].fits_f16() || !k[1].fits_f16();      // (all waves hold the same keys)
     xn[0] = q.dot(k[0]);
     xn[1] = q.dot(k[1]);
-    bf16x8 pf[4][PARTS];
+    V8 pf[4][PP];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {           // 16 slots: keys 16 s + {0..3, 8..11} + 4 half
       f32x8 p;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], a.scale_log2, -mu));
-      split8<PARTS>(p, pf[s]);
+      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], scale, -mu));
+      split8<PP>(p, pf[s]);
       l_used = weight_sum<PARTS>(l_used, p, pf[s][0]);
       if (PARTS == 1 && WEIGH)
 #pragma unroll
@@ -503,9 +562,9 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
       for (int i = 0; i < NT; ++i) {
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32));
         const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32 + 8 * VS));
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        const V8 vf = __builtin_bit_cast(V8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int w = 0; w < PARTS; ++w) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s][w], o[i], 0, 0, 0);
+        for (int w = 0; w < PP; ++w) o[i] = mfma32(vf, pf[s][w], o[i]);
       }
     }
     top = row_top(xn);
@@ -517,6 +576,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   if (s0 < s1) {
     load_keys(ka, s0);
     load_values(s0);
+    if (F16 && wave == 0) outside |= !ka[0].fits_f16() || !ka[1].fits_f16();
     xa[0] = q.dot(ka[0]);
     xa[1] = q.dot(ka[1]);
     load_keys(ka, s0 + 64);
@@ -533,6 +593,11 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
   if (PARTS > 1) l = l_used;
   l += __shfl_xor(l, 32);
   l_used += __shfl_xor(l_used, 32);
+  m -= P_UP;
+  if constexpr (F16) {
+    const int any = __syncthreads_or(outside);
+    if (tid == 0) a.redo[(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = any;
+  }
   if (r >= a.rows) return;
   if (a.part_o) {
     const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + r;
@@ -564,8 +629,10 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 && DVC <= 128 ? 2 : 1)
 // runs over registers, the rows in order.  One workgroup: 128 * NS slots, NS x 32 a wave, their keys widened once into registers; 32 rows a
 // step go through LDS, copied as bank4_join has packed them in operand order.  (A wave that reads its rows as they lie in memory touches a
 // cache line a lane and load, and with 64 slots a workgroup the queries cross the L2 1.3 GB at 1620 x 32 400 x 2: 150 and 115 us.)
-template <int DK, int PARTS, int NS>
+// fp16 products (V8 = f16x8) and their flags as in bank4_block_kernel; SHIFT: fp32 rows were packed times a power of two of their own.
+template <int DK, int PARTS, int NS, typename V8, bool SHIFT>
 __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
+  constexpr bool F16 = std::is_same_v<V8, f16x8>;
   constexpr int KS = DK / 16, TILE = KS * PARTS * 64, TL = TILE / 256;       // 16-byte words a tile, a thread
   extern __shared__ __align__(16) u32x4 qs[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
@@ -573,24 +640,34 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   const int len = (int)read_len(a, b), cnt = read_count(a, b);
   const int rows = cnt * a.group;                       // (rows behind the count have no weight)
   if (first >= len || rows == 0) return;
+  int32_t *redo = a.redo + (a.redo ? blockIdx.y * gridDim.x + blockIdx.x : 0);
+  if (!F16 && a.redo && !*redo) return;
   const int64_t row_base = (int64_t)bh * a.slots;
   const auto rk = bank_rows(a.kc + (row_base + base) * (DK / 2), (int64_t)(len - base) * (DK / 2));
   const auto rs = bank_rows(a.ks + (row_base + base) * (DK / 32), (int64_t)(len - base) * (DK / 32));
-  bf16x8 kf[NS][KS];
+  V8 kf[NS][KS];
+  bool outside = false;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     KeyRow<DK> k;
     k.load(rk, rs, s * 32, col, half);
+    if (F16) outside |= !k.fits_f16();
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) kf[s][i * 4 + u] = bank4_unpack8(k.codes[i][u], k.scale(i));
+      for (int u = 0; u < 4; ++u) kf[s][i * 4 + u] = unpack8<V8>(k.codes[i][u], k.scale(i));
+  }
+  if constexpr (F16) {
+    const int any = __syncthreads_or(outside);
+    if (tid == 0) *redo = any;
+    if (any) return;
   }
   float acc[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) acc[s] = 0.f;
-  const u32x4 *q = reinterpret_cast<const u32x4 *>(a.q_pack) + (int64_t)bh * (a.row_stride / 32) * TILE + tid;
-  const float *row_max = a.row_max + (int64_t)bh * a.row_stride + half * 4, *row_inv = a.row_inv + (int64_t)bh * a.row_stride + half * 4;      // (rows behind the last hold anything: not added)
+  const u32x4 *q = (F16 ? reinterpret_cast<const u32x4 *>(a.q_pack_f16) : reinterpret_cast<const u32x4 *>(a.q_pack)) + (int64_t)bh * (a.row_stride / 32) * TILE + tid;
+  const int64_t row_at = (int64_t)bh * a.row_stride + half * 4;
+  const float *row_max = a.row_max + row_at, *row_inv = a.row_inv + row_at, *row_factor = a.row_scale + row_at;      // (rows behind the last hold anything: not added)
   const int tiles = (rows + 31) / 32;
   int tile0 = 0;                                        // causal: the first rows that see the workgroup's first slot
   if (a.causal) {
@@ -606,25 +683,27 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
 #pragma unroll
     for (int i = 0; i < TL; ++i) next[i] = q[(int64_t)more * TILE + i * 256];
     const int r0 = tile * 32;
-    f32x4 shift[4], inv[4];
+    f32x4 shift[4], inv[4], scale[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       shift[g] = *reinterpret_cast<const f32x4 *>(row_max + r0 + g * 8);
       inv[g] = *reinterpret_cast<const f32x4 *>(row_inv + r0 + g * 8);
+      scale[g] = f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+      if constexpr (SHIFT) scale[g] = *reinterpret_cast<const f32x4 *>(row_factor + r0 + g * 8);
     }
     f32x16 x[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[s][j] = 0.f;
-    const bf16x8 *qt = reinterpret_cast<const bf16x8 *>(qs) + buf * TILE + lane;
+    const V8 *qt = reinterpret_cast<const V8 *>(qs) + buf * TILE + lane;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) {
-        const bf16x8 qf = qt[(i * PARTS + p) * 64];
+        const V8 qf = qt[(i * PARTS + p) * 64];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) x[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[s][i], x[s], 0, 0, 0);
+        for (int s = 0; s < NS; ++s) x[s] = mfma32(qf, kf[s][i], x[s]);
       }
     if (r0 + 32 > rows || (a.causal && read_limit(a, len, cnt, r0 / a.group) < base + 32 * NS)) {
 #pragma unroll
@@ -632,7 +711,7 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
         const int row = r0 + mfma32_row(j, lane), lim = row < rows ? (int)read_limit(a, len, cnt, row / a.group) : 0;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          const float p = inv[j / 4][j % 4] * __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4]));
+          const float p = inv[j / 4][j % 4] * __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], scale[j / 4][j % 4], -shift[j / 4][j % 4]));
           acc[s] += base + s * 32 + col < lim ? p : 0.f;
         }
       }
@@ -641,7 +720,7 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
       for (int j = 0; j < 16; ++j)
 #pragma unroll
         for (int s = 0; s < NS; ++s)
-          acc[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], a.scale_log2, -shift[j / 4][j % 4])), inv[j / 4][j % 4], acc[s]);
+          acc[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x[s][j], scale[j / 4][j % 4], -shift[j / 4][j % 4])), inv[j / 4][j % 4], acc[s]);
     }
 #pragma unroll
     for (int i = 0; i < TL; ++i) qs[(buf ^ 1) * TILE + i * 256 + tid] = next[i];
@@ -733,14 +812,36 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
     const bool live = r < a.rows && t < read_count(a, b);
     const T *row = (const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh;
     bf16x8 *to = reinterpret_cast<bf16x8 *>(a.q_pack) + g * (KS * PARTS * 64) + lane;
-    for (int i = 0; i < KS; ++i) {
+    auto channels = [&](int i) {
       f32x8 y = load8(row + (i / 4) * 64 + half * 32 + (i & 3) * 8, a.q_vec);
 #pragma unroll
       for (int c = 0; c < 8; ++c) y[c] = live ? y[c] * a.q_sign : 0.f;
+      return y;
+    };
+    float up = 1.f;
+    if constexpr (PARTS == 3) {
+      float top = 0.f;
+      for (int i = 0; i < KS; ++i) {
+        const f32x8 y = channels(i);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) top = fmaxf(top, __builtin_fabsf(y[c]));
+      }
+      const int t = query_shift(fmaxf(top, __shfl_xor(top, 32)));
+      up = pow2(t);
+      if (half == 0) a.row_scale[(int64_t)bh * a.row_stride + r] = row_scale(a.scale_log2, pow2(-t));
+    }
+    for (int i = 0; i < KS; ++i) {
+      const f32x8 y = channels(i);
       bf16x8 qf[PARTS];
       split8<PARTS>(y, qf);
 #pragma unroll
       for (int p = 0; p < PARTS; ++p) to[(i * PARTS + p) * 64] = qf[p];
+      if constexpr (PARTS > 1) {
+        f16x8 hf[PARTS - 1];
+        split8<PARTS - 1>(y * up, hf);
+#pragma unroll
+        for (int p = 0; p < PARTS - 1; ++p) (reinterpret_cast<f16x8 *>(a.q_pack_f16) + g * (KS * (PARTS - 1) * 64) + lane)[(i * (PARTS - 1) + p) * 64] = hf[p];
+      }
     }
     return;
   }
@@ -776,17 +877,15 @@ struct ReadPlan {
   int rows, tiles, nsplit, nvc, dvc;
   bool block;                        // 128 rows a workgroup (else 16)
   bool parts;                        // partial results go through the workspace
-  int64_t part_o, part_ml, logits, row_stat, q_pack, logit_stride, row_stride;      // bytes; strides in elements
+  int64_t part_o, part_ml, logits, row_stat, q_pack, q_pack_f16, redo, logit_stride, row_stride;      // bytes; strides in elements
+  int64_t bytes() const { return part_o + part_ml + logits + row_stat + q_pack + q_pack_f16 + redo; }
 };
-
 
 // Value channels a workgroup accumulates: every chunk computes the logits again, so as many as the registers hold.
 static int read_dvc(int dk, int dv, bool block) {
   if (block && dk <= 128 && dv % 256 == 0) return 256;
   return dv % 128 ? 64 : 128;
 }
-
-constexpr int block_occupancy(int dk, int dvc, int dtype) { return dtype == MIVOS_BF16 && dk <= 128 && dvc <= 128 ? 2 : 1; }
 
 static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, int dtype, ReadPlan *p) {
   if (q_heads < 1 || q_heads % k->heads || tokens < 0) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: %d query heads over %d bank heads, %d tokens", q_heads, k->heads, tokens);
@@ -803,7 +902,7 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   if (p->block) {
     // Slices of a row tile's slots: the fewest rounds of the workgroups that run at once (two a CU where their registers allow it), a slice
     // costing its join (its accumulators are written and read once more) and its start.
-    const int at_once = 256 * block_occupancy(k->key_dim, p->dvc, dtype);
+    const int at_once = 256 * block_occupancy(k->key_dim, p->dvc, query_parts(dtype));
     const int most = (int)(k->slots / 512 < 1 ? 1 : k->slots / 512 > 128 ? 128 : k->slots / 512);     // (8 steps a slice pay for its start)
     double best = 1e30;
     for (int n = 1; n <= most; ++n) {
@@ -822,28 +921,35 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   p->logit_stride = (k->slots + 63) / 64 * 64;
   p->logits = weigh && !p->block ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
   p->row_stride = (rows + 31) / 32 * 32;
-  p->row_stat = weigh && p->block ? (int64_t)k->batch * k->heads * p->row_stride * 8 : 0;
-  p->q_pack = p->row_stat / 8 * k->key_dim * 2 * (dtype == MIVOS_BF16 ? 1 : dtype == MIVOS_F16 ? 2 : 3);
+  const int64_t packed = weigh && p->block ? (int64_t)k->batch * k->heads * p->row_stride : 0, f16 = query_parts(dtype) - 1;
+  p->row_stat = packed * 12;
+  p->q_pack = packed * k->key_dim * 2 * (f16 + 1);
+  p->q_pack_f16 = packed * k->key_dim * 2 * f16;
+  const int64_t flags = groups * p->nsplit, flags_weigh = weigh ? (int64_t)k->batch * k->heads * ((k->slots + 127) / 128) : 0;
+  p->redo = p->block && f16 ? ((flags > flags_weigh ? flags : flags_weigh) * 4 + 15) / 16 * 16 : 0;
   return MIVOS_OK;
 }
 
-template <int DK, int DVC, int PARTS, bool WEIGH, bool CAUSAL>
+template <int DK, int DVC, int PARTS, bool F16, bool WEIGH, bool CAUSAL>
 static int block_launch_one(const ReadArgs &a, const dim3 grid, hipStream_t s) {
   constexpr size_t lds = 2 * 64 * (DVC + 16) * 2;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
-    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, WEIGH, CAUSAL>, lds, raised, "bank4_read")) return rc;
+    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, F16, WEIGH, CAUSAL>, lds, raised, "bank4_read")) return rc;
   }
-  bank4_block_kernel<DK, DVC, PARTS, WEIGH, CAUSAL><<<grid, 256, lds, s>>>(a);
+  bank4_block_kernel<DK, DVC, PARTS, F16, WEIGH, CAUSAL><<<grid, 256, lds, s>>>(a);
   return MIVOS_OK;
 }
 
 // (only rounded weights need a second sum: with 2 or 3 parts the one in use is exact)
 template <int DK, int DVC, int PARTS>
 static int block_launch(const ReadArgs &a, const dim3 grid, hipStream_t s) {
-  if constexpr (PARTS == 1)
-    if (a.weigh) return a.causal ? block_launch_one<DK, DVC, 1, true, true>(a, grid, s) : block_launch_one<DK, DVC, 1, true, false>(a, grid, s);
-  return a.causal ? block_launch_one<DK, DVC, PARTS, false, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, false, false>(a, grid, s);
+  if constexpr (PARTS == 1) {
+    if (a.weigh) return a.causal ? block_launch_one<DK, DVC, 1, false, true, true>(a, grid, s) : block_launch_one<DK, DVC, 1, false, true, false>(a, grid, s);
+  } else {
+    if (int rc = a.causal ? block_launch_one<DK, DVC, PARTS, true, false, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, true, false, false>(a, grid, s)) return rc;
+  }
+  return a.causal ? block_launch_one<DK, DVC, PARTS, false, false, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, false, false, false>(a, grid, s);
 }
 
 template <int DK, int PARTS>
@@ -872,22 +978,29 @@ static void join_launch(const ReadArgs &a, int blocks, int out_blocks, hipStream
   else bank4_join_kernel<PARTS, 64><<<blocks, 256, 0, s>>>(a, out_blocks);
 }
 
-template <int DK, int PARTS, int NS>
+template <int DK, int PARTS, int NS, typename V8, bool SHIFT>
 static int weigh_launch_one(const ReadArgs &a, hipStream_t s) {
   constexpr size_t lds = 2 * (DK / 16) * PARTS * 64 * 16;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
-    if (int rc = ensure_dynamic_lds((const void *)bank4_weigh_kernel<DK, PARTS, NS>, lds, raised, "bank4_read")) return rc;
+    if (int rc = ensure_dynamic_lds((const void *)bank4_weigh_kernel<DK, PARTS, NS, V8, SHIFT>, lds, raised, "bank4_read")) return rc;
   }
-  bank4_weigh_kernel<DK, PARTS, NS><<<dim3(cdiv(a.slots, 128 * NS), a.batch * a.heads), 256, lds, s>>>(a);
+  bank4_weigh_kernel<DK, PARTS, NS, V8, SHIFT><<<dim3(cdiv(a.slots, 128 * NS), a.batch * a.heads), 256, lds, s>>>(a);
   return MIVOS_OK;
+}
+
+template <int DK, int PARTS, int NS>
+static int weigh_launch_two(const ReadArgs &a, hipStream_t s) {
+  if constexpr (PARTS > 1)
+    if (int rc = weigh_launch_one<DK, PARTS - 1, NS, f16x8, PARTS == 3>(a, s)) return rc;
+  return weigh_launch_one<DK, PARTS, NS, bf16x8, false>(a, s);
 }
 
 // 256 slots a workgroup where that still gives every CU one; else 128
 template <int DK, int PARTS>
 static int weigh_launch(const ReadArgs &a, hipStream_t s) {
-  if (a.batch * a.heads * (a.slots / 256) >= 240) return weigh_launch_one<DK, PARTS, 2>(a, s);
-  return weigh_launch_one<DK, PARTS, 1>(a, s);
+  if (a.batch * a.heads * (a.slots / 256) >= 240) return weigh_launch_two<DK, PARTS, 2>(a, s);
+  return weigh_launch_two<DK, PARTS, 1>(a, s);
 }
 
 template <int DK>
@@ -903,7 +1016,7 @@ extern "C" int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int
   ReadPlan p;
   if (int rc = bank4_check(bank, "bank4_read")) return rc;
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
-  return p.part_o + p.part_ml + p.logits + p.row_stat + p.q_pack;
+  return p.bytes();
 }
 
 extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t qb, int64_t qt, int64_t qh, int dtype, int q_heads, int tokens,
@@ -915,7 +1028,7 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: bad argument (|scale| up to 1e38)");
   if (int rc = read_plan(bank, q_heads, tokens, weigh, dtype, &p)) return rc;
   if (p.rows == 0) return MIVOS_OK;
-  const int64_t need = p.part_o + p.part_ml + p.logits + p.row_stat + p.q_pack;
+  const int64_t need = p.bytes();
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: workspace of %lld bytes, 16-byte aligned", (long long)need);
   if (p.tiles > 65535 || (int64_t)bank->batch * bank->heads * p.nvc > 65535) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many row tiles");
@@ -932,9 +1045,12 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (p.logits) a.logits = (float *)(ws + p.part_o + p.part_ml);
   if (p.row_stat) {
     a.row_max = (float *)(ws + p.part_o + p.part_ml);
-    a.row_inv = a.row_max + p.row_stat / 8;
+    a.row_inv = a.row_max + p.row_stat / 12;
+    a.row_scale = a.row_inv + p.row_stat / 12;
     a.q_pack = (__bf16 *)(ws + p.part_o + p.part_ml + p.row_stat);
+    a.q_pack_f16 = (_Float16 *)((char *)a.q_pack + p.q_pack);
   }
+  if (p.redo) a.redo = (int32_t *)(ws + need - p.redo);
   a.slots = bank->slots; a.logit_stride = p.logit_stride; a.row_stride = p.row_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
   a.key_dim = bank->key_dim; a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;

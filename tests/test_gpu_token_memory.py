@@ -27,10 +27,10 @@ DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _within(got, ref, tol):
-    got = got.double().cpu()
+    most, got = torch.finfo(got.dtype).max, got.double().cpu()
     assert got.shape == ref.shape
     assert torch.equal(got.isnan(), ref.isnan())
-    ok = ref.isnan() | ((got - ref).abs() <= tol + 1e-300)
+    ok = ref.isnan() | ((got - ref).abs() <= tol + 1e-300) | (got.isinf() & (got.sign() == ref.sign()) & (ref.abs() + tol >= most))      # (beyond the type: infinity)
     assert bool(ok.all()), f"{int((~ok).sum())} of {ok.numel()} off, worst ratio {float(((got - ref).abs() / (tol + 1e-300)).nan_to_num(0).max()):.3g}"
 
 
@@ -310,7 +310,14 @@ def _check_read(bank, q, causal, count, weigh, scale=None, dev_q=None):
     assert got.dtype == q.dtype
     P, parts = PART[q.dtype]
     dlt = (d * parts + 16) * U * big[..., None]
-    _within(got, ref, (HALF[q.dtype] + P) * ref.abs() + (P + 2 * dlt + 2.0 ** -20) * mag + FLOOR[q.dtype] + bank.slots * 2.0 ** -126 * 6 * 2.0 ** 8)
+    floor = FLOOR[q.dtype] + bank.slots * 2.0 ** -126 * 6 * 2.0 ** 8
+    if q.dtype != torch.bfloat16:
+        # Softmax weights as two fp16 numbers after a factor of 2^12, the row's largest at least 2^12: a weight's error is at most 2^-22 of it (inside
+        # 2^-20 * mag) or half of fp16's smallest step, 2^-25 / 2^12 = 2^-37 of the row's largest, which the sum of weights is not below; a slot times
+        # its value, of at most 6 * 2^13 (beyond it the products are bf16 ones), the channel's largest by bank head.
+        top = values.nan_to_num(0).abs().amax(2).clamp(max=6 * 2.0 ** 13)
+        floor = floor + (bank.slots * 2.0 ** -37 * top).repeat_interleave(hq // bank.heads, 1)[:, None]
+    _within(got, ref, (HALF[q.dtype] + P) * ref.abs() + (P + 2 * dlt + 2.0 ** -20) * mag + floor)
     if weigh:
         rows = t * hq // bank.heads
         total = base + received
@@ -399,6 +406,44 @@ def test_read_huge_logits_with_zero_scale_and_split_banks():
         q = 100 * torch.randn(1, rows, 1, 64, generator=torch.Generator().manual_seed(3))
         _check_read(bank, q, False, None, True, scale=0.0)
         _check_read(bank, q, True, None, True)
+
+
+@pytest.mark.parametrize("weigh", (False, True))
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("which", ("one key block", "one value block", "all keys", "all values", "small values", "zero blocks"))
+def test_read_blocks_of_every_size(which, dtype, weigh):
+    """Blocks whose numbers lie far outside fp16 beside ordinary ones, in some slices of the bank and not in others; queries that make their
+    logits ordinary again."""
+    bank = _filled(2, 1, 2500, 64, 128, (2500, 2049))
+    scales, codes, up = {"key": (bank.key_scales, bank.key_codes, 30), "val": (bank.value_scales, bank.value_codes, 90)}["key" if "key" in which else "val"]
+    if which.startswith("one"):
+        scales[0, 0, 2077, 1] += up
+    elif which.startswith("all"):
+        scales[:, :, :2049, 1] += up
+    elif which.startswith("small"):
+        scales[:, :, :2049] -= 80
+    else:
+        codes[:, :, 100:2000, :16] &= 0x88
+        scales[:, :, 100:2000, 0] = 7
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn(2, 70, 2, 64, generator=g)
+    if up == 30:
+        q[..., 32:] *= 2.0 ** -13                       # (fp16 holds them: the block's logits are of 2^17 + 3)
+        q[:, ::2, :, 32:] *= 2.0 ** -10
+    _check_read(bank, q.to(dtype), False, None, weigh)
+    _check_read(bank, q.to(dtype), True, None, weigh)
+
+
+@pytest.mark.parametrize("up", (-100, -30, 40, 110))
+def test_read_queries_of_every_size(up):
+    """fp32 queries far outside fp16, the scale undoing it; rows of zeros among them."""
+    bank = _filled(1, 2, 700, 128, 64, (690,))
+    q = torch.randn(1, 40, 4, 128, generator=torch.Generator().manual_seed(5)) * 2.0 ** (up + torch.arange(40).remainder(11).float()).view(1, 40, 1, 1)
+    q[:, 7] = 0
+    q[..., 5] *= 2.0 ** -12
+    for weigh in (False, True):
+        _check_read(bank, q, True, None, weigh, scale=2.0 ** -(up + 8))
+        _check_read(bank, q, False, None, weigh, scale=2.0 ** -(up + 8))
 
 
 @pytest.mark.parametrize("scale", (0.0, 2.0 ** -128, -2.0 ** -128))
