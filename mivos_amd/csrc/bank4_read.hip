@@ -74,7 +74,15 @@ __device__ __forceinline__ void split8_as(f32x8 x, V (&p)[PARTS]) {
     }
 }
 template <int PARTS> __device__ __forceinline__ void split8(f32x8 x, bf16x8 (&p)[PARTS]) { split8_as<__bf16>(x, p); }
-template <int PARTS> __device__ __forceinline__ void split8(f32x8 x, f16x8 (&p)[PARTS]) { split8_as<_Float16>(x, p); }
+template <int PARTS> __device__ __forceinline__ void split8(f32x8 x, f16x8 (&p)[PARTS]) {
+  p[0] = __builtin_convertvector(x, f16x8);
+  if constexpr (PARTS == 2) {
+    float one = 1.f;
+    asm("" : "+s"(one));               // (a factor that the compiler cannot drop: x * one - p and its rounding are one instruction, else three)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[1][j] = (_Float16)__builtin_fmaf(x[j], one, -(float)p[0][j]);
+  }
+}
 
 template <typename V> __device__ __forceinline__ V unpack8(uint32_t codes, float scale);
 template <> __device__ __forceinline__ bf16x8 unpack8<bf16x8>(uint32_t codes, float scale) { return bank4_unpack8(codes, scale); }
