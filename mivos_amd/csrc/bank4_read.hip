@@ -4,7 +4,8 @@
 //
 // Arithmetic.  A bank value has at most two significant bits and is exact in bf16, so both products run on the bf16 matrix cores with
 // exact bank operands: q (and the softmax weight p) is written as a sum of PARTS bf16 numbers - 1 for bf16 inputs (q exact, p rounded once,
-// 2^-8 of each term, the size of the output's own rounding), 2 for fp16 (11 bits of q exactly, 16 bits of p), 3 for fp32 (24 bits of both).
+// 2^-8 of each term, the size of the output's own rounding), 2 for fp16 (11 bits of q exactly, 16 bits of p), 3 for fp32 (24 bits of both).  Where many
+// rows make the products the cost, fp16 and fp32 queries take fp16 numbers instead, one part fewer (bank4_block_kernel).
 // Running maximum, sum and accumulators are fp32.
 //
 // Layout.  S^T = K Q^T on 16x16x32: lane l holds bank row l % 16 and channels (l / 16) * DK / 4 .. + DK / 4 of it - contiguous codes in memory,
@@ -411,9 +412,10 @@ struct QueryCols {
 // the other.  S^T = K Q^T and O^T = V^T P^T on 32x32 products: a lane holds one query, 16 keys of each 32, and these are again the
 // operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^8.
 // F16 (fp16 and fp32 queries): the products on fp16 numbers, which carry three bits more than bf16 ones - q in 1 / 2 of them (fp32 rows brought to
-// 2^14 first), the softmax weight times 2^12 in 2 (2^-22 of itself or 2^-37 of the row's largest; the maximum follows closer, by 2^3), where bf16 takes 2 / 3 and 2 / 3.  A 4-bit value
-// is exact in fp16 from 2^-24 to 6 * 2^13; a workgroup that meets a block outside raises its flag, and the bf16 kernel, launched behind, does that
-// workgroup's work again (the others leave at once).  2 x 1620 fp32 rows x 32 400 slots, 128 / 512: @F16@ us instead of 471.
+// 2^14 first), the softmax weight times 2^12 in 2 (2^-22 of itself or 2^-37 of the row's largest; the maximum is followed closer, by 2^3), where bf16
+// takes 2 / 3 and 2 / 3.  A 4-bit value is exact in fp16 from 2^-24 to 6 * 2^13; a workgroup that meets a block outside raises its flag, and the bf16
+// kernel, launched behind, does that workgroup's work again (the others leave at once, 5 us in all).  2 x 1620 fp32 rows x 32 400 slots, 128 / 512:
+// 400 us instead of 471, 0.81 PFLOP/s issued; all 512 value channels in one workgroup would need registers it does not have.
 template <int DK, int DVC, int PARTS, bool F16, bool WEIGH, bool CAUSAL>
 __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_block_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
@@ -515,8 +517,8 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
 
   // The logits run one step ahead: their products are issued among the exponentials of the step before, their maximum among its second
   // products.  The order inside a step is the compiler's: written out by hand, one product and at most four vector instructions behind it, the
-  // step takes a tenth fewer cycles and the chip holds a tenth less clock (fp32: 57 % of the cycles matrix work at 1.78 GHz, against 46 % at
-  // 2.05): power is what bounds this kernel, as it bounds a large library product (1.2 of the 2.5 PFLOP/s).
+  // step takes a tenth fewer cycles and the chip holds a tenth less clock (fp32 on bf16 numbers: 57 % of the cycles matrix work at 1.78 GHz,
+  // against 46 % at 2.05; fp16 numbers: 43 % at 1.77): power is what bounds this kernel, as it bounds a large library product (1.2 of the 2.5 PFLOP/s).
   float top;
   auto row_top = [&](const f32x16 (&x)[2]) {
     float t = fmaxf(x[0][0], x[1][0]);
