@@ -141,10 +141,11 @@ constexpr float MAX_LAG = 8.f;      // the running maximum follows a logit that 
 template <int DK, int DVC, int PARTS>
 __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_rows_kernel(ReadArgs a) {
   typedef typename ReadType<PARTS>::T T;
+  constexpr int PP = PARTS == 3 ? 3 : 2;
   constexpr int CPL = DK / 4, KSTEPS = DK / 32, VPAD = DVC + 16, OPAD = DVC + 4, NT = DVC / 16, VB = DVC / 32;
   constexpr int LDS_V = 4 * 32 * VPAD * 2, LDS_O = 4 * 16 * OPAD * 4;
   __shared__ __align__(16) char lds[LDS_V > LDS_O ? LDS_V : LDS_O];
-  __shared__ float stat[4][16][3];
+  __shared__ float stat[4][16][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
   const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
   const int split = blockIdx.x, row0 = blockIdx.y * 16;
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
   f32x4 o[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f, l_used = 0.f;
+  float m = -INFINITY, l = 0.f;
   __bf16 *vt = reinterpret_cast<__bf16 *>(lds) + wave * 32 * VPAD;
   const int v_row = a.value_dim / 2, vs_row = a.value_dim / 32;
   const uint8_t *kc = a.kc + (int64_t)bh * a.slots * (DK / 2), *ks = a.ks + (int64_t)bh * a.slots * (DK / 32);
@@ -246,7 +247,6 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
       const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
       l *= alpha;
-      l_used *= alpha;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
@@ -271,12 +271,10 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
       f32x8 p;
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[half * 2 + j / 4][j % 4], a.scale_log2, -mu));
-      bf16x8 pf[PARTS];
-      split8<PARTS>(p, pf);
-      l_used = weight_sum<PARTS>(l_used, p, pf[0]);
-      if (PARTS == 1 && a.logits)
+      bf16x8 pf[PP];
+      split8<PP>(p, pf);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) l += p[j];
+      for (int j = 0; j < 8; ++j) l += p[j];
       wave_lds_fence();
 #pragma unroll
       for (int i = 0; i < VB / 2; ++i) {
@@ -293,42 +291,38 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
         const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 16 * VPAD));
         const bf16x8 vf = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[q], o[i], 0, 0, 0);
+        for (int q = 0; q < PP; ++q) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[q], o[i], 0, 0, 0);
       }
     }
   }
-  if (PARTS > 1) l = l_used;
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
-  l_used += __shfl_xor(l_used, 16);
-  l_used += __shfl_xor(l_used, 32);
   // ---- the four waves meet
   __syncthreads();
   float *om = reinterpret_cast<float *>(lds);
 #pragma unroll
   for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4 *>(om + (wave * 16 + col) * OPAD + i * 16 + grp * 4) = o[i];
-  if (grp == 0) { stat[wave][col][0] = m; stat[wave][col][1] = l_used; stat[wave][col][2] = l; }
+  if (grp == 0) { stat[wave][col][0] = m; stat[wave][col][1] = l; }
   __syncthreads();
   for (int e = tid; e < 16 * DVC; e += 256) {
     const int rr = e / DVC, dv = e % DVC, row = row0 + rr;
     if (row >= a.rows) break;
     const float mm = fmaxf(fmaxf(stat[0][rr][0], stat[1][rr][0]), fmaxf(stat[2][rr][0], stat[3][rr][0]));
     const float mu = mm == -INFINITY ? 0.f : mm;
-    float acc = 0.f, used = 0.f, sum = 0.f;
+    float acc = 0.f, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float f = __builtin_amdgcn_exp2f(stat[w][rr][0] - mu);
       acc += f * om[(w * 16 + rr) * OPAD + dv];
-      used += f * stat[w][rr][1];
-      sum += f * stat[w][rr][2];
+      sum += f * stat[w][rr][1];
     }
     if (a.part_o) {
       const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + row;
       a.part_o[at * a.value_dim + chunk * DVC + dv] = acc;
-      if (dv == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = f32x4{mm, used, sum, 0.f};
+      if (dv == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = f32x4{mm, sum, sum, 0.f};
     } else {
       const int tt = row / a.group, j = h * a.group + row - tt * a.group;
-      ((T *)a.out)[(((int64_t)b * a.tokens + tt) * a.heads * a.group + j) * a.value_dim + chunk * DVC + dv] = (T)(used != 0.f ? acc / used : 0.f);
+      ((T *)a.out)[(((int64_t)b * a.tokens + tt) * a.heads * a.group + j) * a.value_dim + chunk * DVC + dv] = (T)(sum != 0.f ? acc / sum : 0.f);
     }
   }
 }
