@@ -20,9 +20,11 @@ namespace mivos {
 
 constexpr float LOG2E = 1.4426950408889634f;
 // Rows a bank head from which the 128-row kernel runs.  Both kernels, us without / with the weights gathered (bf16; 16-row tiles | 128 rows):
-//   4 heads x 16 384 slots, 2 streams   32 rows 35 / 44 | 28 / 34     64 rows 45 / 69 | 30 / 36     200 rows 57 / 169 | 41 / 52
-//   2 heads x 65 536 slots              32 rows 41 / 46 | 45 / 50     64 rows 46 / 64 | 44 / 50     200 rows 66 / 188 | 57 / 68
-//   8 heads x 4096 slots x 64, 4        32 rows 15 / 39 | 17 / 22     64 rows 23 / 64 | 19 / 24     200 rows 35 / 157 | 30 / 40
+//   4 heads x 16 384 slots, 2 streams   32 rows 28 / 41 | 25 / 30     64 rows 38 / 65 | 28 / 33     200 rows 60 / 155 | 41 / 53
+//   2 heads x 65 536 slots              32 rows 30 / 38 | 33 / 38     64 rows 37 / 59 | 33 / 40     200 rows 63 / 171 | 46 / 58
+//   8 heads x 4096 slots x 64, 4        32 rows 16 / 36 | 18 / 22     64 rows 24 / 58 | 19 / 24     200 rows 39 / 142 | 30 / 41
+//   1 head x 8192 slots, values of 512  32 rows 15 / 29 | 25 / 30     64 rows 17 / 49 | 26 / 31     200 rows 33 / 127 | 30 / 40
+// (fp32: 32 rows 32 | 32, 32 | 41, 18 | 24, 16 | 36; 64 rows 47 | 36, 42 | 43, 27 | 25, 19 | 38, weights 74 | 47, 65 | 52, 61 | 36, 51 | 47)
 constexpr int BLOCK_ROWS_MIN = 33;
 
 struct ReadArgs {
@@ -768,7 +770,7 @@ struct RowJoin {
   }
 };
 
-// Joins the slices of a row (first `out_blocks` workgroups, one wave a row; QL lanes cover the value channels, 64 / QL slices at a time)
+// Joins the slices of a row (first `out_blocks` workgroups, a wave a row and 4 * QL value channels, 64 / QL slices at a time)
 // and adds the rows' weights to the slots (the others, 1024 slots each, the rows in order: the sum does not depend on timing) or, ahead of
 // bank4_weigh, packs its queries.
 template <int PARTS, int QL>
@@ -777,33 +779,38 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if ((int)blockIdx.x < out_blocks) {
     const int64_t g = (int64_t)blockIdx.x * 4 + wave;
-    if (g >= (int64_t)a.batch * a.heads * a.rows) return;
-    const int bh = (int)(g / a.rows), row = (int)(g - (int64_t)bh * a.rows), b = bh / a.heads, h = bh - b * a.heads;
+    const int chunks = (a.value_dim + QL * 4 - 1) / (QL * 4);
+    const int64_t gr = g / chunks;
+    const int chunk = (int)(g - gr * chunks);
+    if (gr >= (int64_t)a.batch * a.heads * a.rows) return;
+    const int bh = (int)(gr / a.rows), row = (int)(gr - (int64_t)bh * a.rows), b = bh / a.heads, h = bh - b * a.heads;
     const RowJoin J(a, bh, row, lane);
-    if (a.row_max && lane == 0) { a.row_max[(int64_t)bh * a.row_stride + row] = J.top; a.row_inv[(int64_t)bh * a.row_stride + row] = J.inv_sum; }
+    if (a.row_max && chunk == 0 && lane == 0) { a.row_max[(int64_t)bh * a.row_stride + row] = J.top; a.row_inv[(int64_t)bh * a.row_stride + row] = J.inv_sum; }
     const int t = row / a.group, j = h * a.group + row - t * a.group;
     T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + j) * a.value_dim;
     const float *part = a.part_o + ((int64_t)bh * a.nsplit * a.rows + row) * a.value_dim;
     const int64_t stride = (int64_t)a.rows * a.value_dim;
-    for (int dv = lane % QL * 4; dv < a.value_dim; dv += QL * 4) {
-      f32x4 acc{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int s0 = 0; s0 < a.nsplit; s0 += 64 / QL) {
-        const int s = s0 + lane / QL;
-        const float f0 = __shfl(J.f[0], s & 63), f1 = __shfl(J.f[1], s & 63), f = s < 64 ? f0 : f1;
-        if (s < a.nsplit && f >= 0.f) acc += f * *reinterpret_cast<const f32x4 *>(part + s * stride + dv);
-      }
+    const int dv = chunk * QL * 4 + lane % QL * 4;
+    const float *from = part + (dv < a.value_dim ? dv : 0);
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s0 = 0; s0 < a.nsplit; s0 += 64 / QL) {
+      const int s = s0 + lane / QL;
+      const float f0 = __shfl(J.f[0], s & 63), f1 = __shfl(J.f[1], s & 63), f = s < 64 ? f0 : f1;
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (s < a.nsplit ? s : 0) * stride);      // (no branch: all loads go out together)
 #pragma unroll
-      for (int d = QL; d < 64; d <<= 1)
+      for (int c = 0; c < 4; ++c) acc[c] += s < a.nsplit && f >= 0.f ? f * x[c] : 0.f;
+    }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], d);
-      if (lane < QL) {
-        typedef T Tx4 __attribute__((ext_vector_type(4)));
-        Tx4 y;
+    for (int d = QL; d < 64; d <<= 1)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = (T)(J.inv == 0.f ? 0.f : acc[c] * J.inv);
-        *reinterpret_cast<Tx4 *>(out + dv) = y;
-      }
+      for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], d);
+    if (lane < QL && dv < a.value_dim) {
+      typedef T Tx4 __attribute__((ext_vector_type(4)));
+      Tx4 y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) y[c] = (T)(J.inv == 0.f ? 0.f : acc[c] * J.inv);
+      *reinterpret_cast<Tx4 *>(out + dv) = y;
     }
     return;
   }
@@ -975,10 +982,14 @@ static int read_launch(const ReadArgs &a, const ReadPlan &p, int dtype, hipStrea
   return dtype == MIVOS_F16 ? read_launch<DK, 2>(a, p, s) : read_launch<DK, 3>(a, p, s);
 }
 
+// Lanes over the value channels of a joined row: few rows are bound by the chain of their slices (one token over 8192 slots, values of 512: 13 us a
+// call instead of 28; 65 536 slots: 22 instead of 32), many by bytes.
+static int join_lanes(int64_t rows, int value_dim) { return value_dim <= 64 || rows <= 512 ? 16 : value_dim <= 128 ? 32 : 64; }
+
 template <int PARTS>
-static void join_launch(const ReadArgs &a, int blocks, int out_blocks, hipStream_t s) {
-  if (a.value_dim <= 64) bank4_join_kernel<PARTS, 16><<<blocks, 256, 0, s>>>(a, out_blocks);
-  else if (a.value_dim <= 128) bank4_join_kernel<PARTS, 32><<<blocks, 256, 0, s>>>(a, out_blocks);
+static void join_launch(const ReadArgs &a, int lanes, int blocks, int out_blocks, hipStream_t s) {
+  if (lanes == 16) bank4_join_kernel<PARTS, 16><<<blocks, 256, 0, s>>>(a, out_blocks);
+  else if (lanes == 32) bank4_join_kernel<PARTS, 32><<<blocks, 256, 0, s>>>(a, out_blocks);
   else bank4_join_kernel<PARTS, 64><<<blocks, 256, 0, s>>>(a, out_blocks);
 }
 
@@ -1036,8 +1047,9 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: workspace of %lld bytes, 16-byte aligned", (long long)need);
   if (p.tiles > 65535 || (int64_t)bank->batch * bank->heads * p.nvc > 65535) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many row tiles");
-  // the join's workgroups: four rows each; then the weights of 1024 slots each, or four tiles of queries to pack
-  const int64_t heads = (int64_t)bank->batch * bank->heads, out_blocks = (heads * p.rows + 3) / 4;
+  // the join's workgroups: four rows (or shares of their channels) each; then the weights of 1024 slots each, or four tiles of queries to pack
+  const int64_t heads = (int64_t)bank->batch * bank->heads, lanes = join_lanes(heads * p.rows, bank->value_dim);
+  const int64_t out_blocks = (heads * p.rows * cdiv(bank->value_dim, 4 * lanes) + 3) / 4;
   const int64_t blocks = out_blocks + (p.logits ? heads * ((bank->slots + 1023) / 1024) : 0) + (p.q_pack ? (heads * (p.row_stride / 32) + 3) / 4 : 0);
   if (p.parts && blocks >= 1 << 24) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_read: too many rows");
   hipStream_t s = (hipStream_t)stream;
@@ -1066,9 +1078,9 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
     return rc;
   if (int rc = check_launch("bank4_read")) return rc;
   if (!p.parts) return MIVOS_OK;
-  if (dtype == MIVOS_BF16) join_launch<1>(a, (int)blocks, (int)out_blocks, s);
-  else if (dtype == MIVOS_F16) join_launch<2>(a, (int)blocks, (int)out_blocks, s);
-  else join_launch<3>(a, (int)blocks, (int)out_blocks, s);
+  if (dtype == MIVOS_BF16) join_launch<1>(a, (int)lanes, (int)blocks, (int)out_blocks, s);
+  else if (dtype == MIVOS_F16) join_launch<2>(a, (int)lanes, (int)blocks, (int)out_blocks, s);
+  else join_launch<3>(a, (int)lanes, (int)blocks, (int)out_blocks, s);
   if (int rc = check_launch("bank4_read")) return rc;
   if (!a.row_max) return MIVOS_OK;
   if (int rc = bank->key_dim == 64 ? weigh_launch<64>(a, dtype, s) : bank->key_dim == 128 ? weigh_launch<128>(a, dtype, s) : weigh_launch<256>(a, dtype, s))
