@@ -4,8 +4,9 @@
 //
 // Arithmetic.  A bank value has at most two significant bits and is exact in bf16, so both products run on the bf16 matrix cores with
 // exact bank operands: q (and the softmax weight p) is written as a sum of PARTS bf16 numbers - 1 for bf16 inputs (q exact, p rounded once,
-// 2^-8 of each term, the size of the output's own rounding), 2 for fp16 (11 bits of q exactly, 16 bits of p), 3 for fp32 (24 bits of both).  Where many
-// rows make the products the cost, fp16 and fp32 queries take fp16 numbers instead, one part fewer (bank4_block_kernel).
+// 2^-8 of each term, the size of the output's own rounding), 2 for fp16 (11 bits of q exactly, 16 bits of p), 3 for fp32 (24 bits of both).  With few
+// rows, where bytes are the cost, p of bf16 inputs takes 2 as well; where many rows make the products the cost, fp16 and fp32 queries take fp16 numbers
+// instead, one part fewer (bank4_block_kernel).
 // Running maximum, sum and accumulators are fp32.
 //
 // Layout.  S^T = K Q^T on 16x16x32: lane l holds bank row l % 16 and channels (l / 16) * DK / 4 .. + DK / 4 of it - contiguous codes in memory,
