@@ -310,6 +310,8 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
   for (int e = tid; e < 16 * DVC; e += 256) {
     const int rr = e / DVC, dv = e % DVC, row = row0 + rr;
     if (row >= a.rows) break;
+    const int tt = row / a.group;
+    const bool valid = tt < cnt;      // (a padded token's queries are zeros, its logits only masked where a valid row's are)
     const float mm = fmaxf(fmaxf(stat[0][rr][0], stat[1][rr][0]), fmaxf(stat[2][rr][0], stat[3][rr][0]));
     const float mu = mm == -INFINITY ? 0.f : mm;
     float acc = 0.f, sum = 0.f;
@@ -322,10 +324,10 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
     if (a.part_o) {
       const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + row;
       a.part_o[at * a.value_dim + chunk * DVC + dv] = acc;
-      if (dv == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = f32x4{mm, sum, sum, 0.f};
+      if (dv == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = valid ? f32x4{mm, sum, sum, 0.f} : f32x4{-INFINITY, 0.f, 0.f, 0.f};
     } else {
-      const int tt = row / a.group, j = h * a.group + row - tt * a.group;
-      ((T *)a.out)[(((int64_t)b * a.tokens + tt) * a.heads * a.group + j) * a.value_dim + chunk * DVC + dv] = (T)(sum != 0.f ? acc / sum : 0.f);
+      const int j = h * a.group + row - tt * a.group;
+      ((T *)a.out)[(((int64_t)b * a.tokens + tt) * a.heads * a.group + j) * a.value_dim + chunk * DVC + dv] = (T)(valid && sum != 0.f ? acc / sum : 0.f);
     }
   }
 }

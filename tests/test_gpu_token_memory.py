@@ -651,3 +651,28 @@ def test_two_streams_at_once():
     for a, b in zip(alone, both):
         for u, v in zip(a, b):
             assert torch.equal(u[0], v[0]) and torch.equal(u[1], v[1])
+
+
+# ------------------------------------------------------------------------------------------------ padded tokens
+# tokens, query heads a bank head, valid tokens of the two streams: rows of one 16-row tile, of two, and of the 128-row kernel
+PADDED = [(5, 1, (3, 5)), (2, 3, (1, 0)), (4, 8, (2, 3)), (40, 2, (33, 1))]
+
+
+@pytest.mark.parametrize("weigh", (False, True))
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("slots", (100, 1000, 5000))
+@pytest.mark.parametrize("case", PADDED, ids=lambda c: f"{c[0]}x{c[1]}")
+def test_read_padded_tokens_are_zero(case, slots, dtype, weigh):
+    """Tokens behind a stream's count beside valid ones, over one slice of the bank and several: exactly 0, whatever the bank holds."""
+    tokens, group, counts = case
+    bank = _filled(2, 2, slots, 64, 128, (slots - 3, slots * 2 // 3), seed=tokens)
+    q = 2 * torch.randn(2, tokens, 2 * group, 64, generator=torch.Generator().manual_seed(slots))
+    count = torch.tensor(counts, dtype=torch.int32)
+    for nan in (False, True):
+        if nan:                                                    # a key block that only the valid rows of the first stream meet
+            bank.key_scales[0, :, 7, 1] = 255
+        for causal in (False, True):
+            got = _check_read(bank, q.to(dtype), causal, count, weigh and not nan)
+            for b in range(2):
+                assert not bool(got[b, counts[b]:].view(torch.uint8).any())
+                assert bool(got[b, :counts[b]].isnan().all()) == (nan and b == 0) or not counts[b]
