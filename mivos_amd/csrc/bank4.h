@@ -40,9 +40,10 @@ __device__ __forceinline__ f16x8 bank4_unpack8_f16(uint32_t codes, float scale) 
   const f16x4 lo = __builtin_shufflevector(a, b, 0, 1, 2, 3), hi = __builtin_shufflevector(c, d, 0, 1, 2, 3);
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// 0.5 * 2^(byte - 127) >= 2^-24 and 6 * 2^(byte - 127) <= 6 * 2^13, or a block of zeros
+// 0.5 * 2^(byte - 127) >= 2^-24 and 6 * 2^(byte - 127) <= 6 * 2^13, or a block of zeros (under kBank4NanScale too: the conversion answers NaN)
+constexpr uint32_t kBank4F16Least = 104, kBank4F16Most = 140;
 __device__ __forceinline__ bool bank4_fits_f16(uint32_t byte, u32x4 codes) {
-  return byte - 104u <= 36u || ((codes[0] | codes[1] | codes[2] | codes[3]) & 0x77777777u) == 0;
+  return byte - kBank4F16Least <= kBank4F16Most - kBank4F16Least || ((codes[0] | codes[1] | codes[2] | codes[3]) & 0x77777777u) == 0;
 }
 
 // 8 consecutive elements of a row as fp32; `vec`: the address is a multiple of 16 bytes

@@ -3,10 +3,9 @@
 // and, when asked, weight[s] += sum over the rows (tokens x G) of their softmax weight on slot s.
 //
 // Arithmetic.  A bank value has at most two significant bits and is exact in bf16, so both products run on the bf16 matrix cores with
-// exact bank operands: q (and the softmax weight p) is written as a sum of PARTS bf16 numbers - 1 for bf16 inputs (q exact, p rounded once,
-// 2^-8 of each term, the size of the output's own rounding), 2 for fp16 (11 bits of q exactly, 16 bits of p), 3 for fp32 (24 bits of both).  With few
-// rows, where bytes are the cost, p of bf16 inputs takes 2 as well; where many rows make the products the cost, fp16 and fp32 queries take fp16 numbers
-// instead, one part fewer (bank4_block_kernel).
+// exact bank operands: q and the softmax weight p are written as sums of bf16 numbers - q in 1 for bf16 inputs (exact), 2 for fp16 (exact), 3 for
+// fp32 (24 bits), p in 2, 2 and 3 (16, 16 and 24 bits).  That is what few rows take, where bytes are the cost.  Where many rows make the products the
+// cost they run on fp16 numbers, one part fewer (bank4_block_kernel).
 // Running maximum, sum and accumulators are fp32.
 //
 // Layout.  S^T = K Q^T on 16x16x32: lane l holds bank row l % 16 and channels (l / 16) * DK / 4 .. + DK / 4 of it - contiguous codes in memory,
@@ -38,9 +37,9 @@ struct ReadArgs {
   float *part_o, *part_ml, *logits, *row_max, *row_inv, *row_scale;
   __bf16 *q_pack;
   _Float16 *q_pack_f16;
-  int32_t *redo;          // a flag a workgroup: fp16 products met a block that they do not hold, the bf16 ones do it again
+  int32_t *redo;          // bank4_weigh: a flag a workgroup, fp16 products met a block that they do not hold and the bf16 ones do it again
   int64_t slots, logit_stride, row_stride;
-  int batch, heads, group, tokens, rows, key_dim, value_dim, nsplit, causal, weigh, q_vec;
+  int batch, heads, group, tokens, rows, key_dim, value_dim, nsplit, causal, q_vec;
   float scale_log2;       // |scale| * log2(e): the softmax runs in powers of two; the sign of scale goes to the queries
   float q_sign;           // (0 where scale is: -inf * 0 of a masked logit is never formed)
 };
@@ -110,26 +109,12 @@ template <> struct ReadType<2> { typedef _Float16 T; };
 template <> struct ReadType<3> { typedef float T; };
 
 typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // Rows [0, n) of a bank array behind a wave-uniform address: loads take one per-lane offset and answer 0 behind the last row (codes 0, scale
 // byte 0: the value 0), so that what lies behind a stream's length is neither addressed nor looked at.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t bank_rows(const uint8_t *p, int64_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes), 0x00020000);
-}
-
-// The sum of a lane's softmax weights, as the second product uses them: bf16 queries round the weights, and the output is divided by the sum of
-// the rounded ones, so that what the rounding does to all of a row's weights alike drops out.
-template <int PARTS, typename V>
-__device__ __forceinline__ float weight_sum(float l, f32x8 p, const V &pf) {
-  if constexpr (PARTS == 1) {
-    const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pf[2 * j], pf[2 * j + 1]}, one, l, false);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) l += p[j];
-  }
-  return l;
 }
 
 constexpr int block_occupancy(int dk, int dvc, int parts) { return parts == 1 && dk <= 128 && dvc <= 128 ? 2 : 1; }
@@ -324,7 +309,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
     if (a.part_o) {
       const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + row;
       a.part_o[at * a.value_dim + chunk * DVC + dv] = acc;
-      if (dv == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = valid ? f32x4{mm, sum, sum, 0.f} : f32x4{-INFINITY, 0.f, 0.f, 0.f};
+      if (dv == 0 && chunk == 0) *reinterpret_cast<f32x2 *>(a.part_ml + at * 2) = valid ? f32x2{mm, sum} : f32x2{-INFINITY, 0.f};
     } else {
       const int j = h * a.group + row - tt * a.group;
       ((T *)a.out)[(((int64_t)b * a.tokens + tt) * a.heads * a.group + j) * a.value_dim + chunk * DVC + dv] = (T)(valid && sum != 0.f ? acc / sum : 0.f);
@@ -350,6 +335,10 @@ struct KeyRow {
   }
   __device__ __forceinline__ uint32_t byte(int i) const { return (scales[i / 2] >> (16 * (i & 1))) & 255; }
   __device__ __forceinline__ float scale(int i) const { return bank4_scale(byte(i)); }
+  __device__ __forceinline__ void most(u16x2 &m) const {      // the largest scale bytes of words' halves
+#pragma unroll
+    for (int i = 0; i < (KI + 1) / 2; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, scales[i] & 0x00ff00ffu));
+  }
   __device__ __forceinline__ bool fits_f16() const {
     bool ok = true;
 #pragma unroll
@@ -409,23 +398,24 @@ struct QueryCols {
 // One workgroup: 128 rows (32 a wave) x one slice of the slots x DVC value channels, 64 slots a step.  Every wave reads the step's K
 // codes straight into registers; the V rows are widened once for the workgroup into one of two LDS buffers while the matrix cores work on
 // the other.  S^T = K Q^T and O^T = V^T P^T on 32x32 products: a lane holds one query, 16 keys of each 32, and these are again the
-// operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^8.
-// F16 (fp16 and fp32 queries): the products on fp16 numbers, which carry three bits more than bf16 ones - q in 1 / 2 of them (fp32 rows brought to
-// 2^14 first), the softmax weight times 2^12 in 2 (2^-22 of itself or 2^-37 of the row's largest; the maximum is followed closer, by 2^3), where bf16
-// takes 2 / 3 and 2 / 3.  A 4-bit value is exact in fp16 from 2^-24 to 6 * 2^13; a workgroup that meets a block outside raises its flag, and the bf16
-// kernel, launched behind, does that workgroup's work again (the others leave at once, 5 us in all).  2 x 1620 fp32 rows x 32 400 slots, 128 / 512:
-// 400 us instead of 471, 0.81 PFLOP/s issued; all 512 value channels in one workgroup would need registers it does not have.
-template <int DK, int DVC, int PARTS, bool F16, bool WEIGH, bool CAUSAL>
-__global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_block_kernel(ReadArgs a) {
+// operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^LAG.
+// F16: the products on fp16 numbers, which carry three bits more than bf16 ones.  fp16 and fp32 queries: q in 1 / 2 of them (fp32 rows brought to
+// 2^14 first), the softmax weight times 2^12 in 2 (2^-22 of itself or 2^-37 of the row's largest; the maximum is followed closer, by 2^3).  bf16
+// queries: keys and q as bf16, the weight times 2^8 in 1 (2^-11 of itself or 2^-33 of the row's largest; one bf16 number, 2^-8 of it, put the error of
+// 3 x 1021 causal tokens over 16 300 slots at 1.3 times that of fp32 weights, two take 489 us there: 359, 372 and 489).
+// A 4-bit value is exact in fp16 from 2^-24 to 6 * 2^13; a workgroup that has met a block outside, or keys above it, whose logits lie so far apart that
+// such weights lose channels, does its work again on bf16 numbers (twice the time and more, for that workgroup).  2 x 1620 fp32 rows x 32 400 slots,
+// 128 / 512: 400 us instead of 471, 0.81 PFLOP/s issued; all 512 value channels in one workgroup would need registers it does not have.
+// -> true: F16, and the workgroup has met such a block (nothing is written)
+template <int DK, int DVC, int PARTS, bool F16, bool CAUSAL, int VL = (DVC * 2 + 255) / 256>
+__device__ __forceinline__ bool block_rows(const ReadArgs &a, __bf16 *vt, uint64_t (&nan_blocks)[2][4][VL]) {
   typedef typename ReadType<PARTS>::T T;
+  constexpr bool KEYS_F16 = F16 && PARTS > 1, SHIFT = F16 && PARTS == 3;
+  typedef std::conditional_t<KEYS_F16, f16x8, bf16x8> K8;
   typedef std::conditional_t<F16, f16x8, bf16x8> V8;
-  constexpr int QP = F16 ? PARTS - 1 : PARTS, PP = F16 ? 2 : PARTS;
-  constexpr bool SHIFT = F16 && PARTS == 3;
-  constexpr float LAG = F16 ? 3.f : MAX_LAG, P_UP = F16 ? 12.f : 0.f;        // weights are exp2(logit - (maximum - P_UP)), up to 2^(LAG + P_UP)
-  if (!F16 && a.redo && !a.redo[(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x]) return;
-  constexpr int VS = DVC + 16, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB, VL = (VE + 255) / 256;
-  extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
-  __shared__ uint64_t nan_blocks[2][4][VL];            // causal: the value blocks of a buffer that stand for NaN, a bit a lane of the wave that stored it
+  constexpr int QP = KEYS_F16 ? PARTS - 1 : PARTS, PP = F16 && PARTS == 1 ? 1 : PARTS == 3 && !F16 ? 3 : 2;
+  constexpr float LAG = F16 ? PARTS == 1 ? 7.f : 3.f : MAX_LAG, P_UP = F16 ? PARTS == 1 ? 8.f : 12.f : 0.f;        // weights are exp2(logit - (maximum - P_UP)), up to 2^(LAG + P_UP)
+  constexpr int VS = DVC + 16, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
   const int split = blockIdx.x, row0 = blockIdx.y * 128, r = row0 + wave * 32 + col;
@@ -446,7 +436,7 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
   }
   low = __builtin_amdgcn_readfirstlane(low);
 
-  QueryCols<DK, QP, V8> q;
+  QueryCols<DK, QP, K8> q;
   const float back = q.template load<SHIFT>((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign);
   const float scale = SHIFT ? row_scale(a.scale_log2, back) : a.scale_log2;
   f32x16 o[NT];
@@ -454,7 +444,7 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-  float m = -INFINITY, l = 0.f, l_used = 0.f;
+  float m = -INFINITY, l = 0.f;
   const int v_row = a.value_dim / 2, vs_row = a.value_dim / 32;
   const uint8_t *kc = a.kc + (int64_t)bh * a.slots * (DK / 2), *ks = a.ks + (int64_t)bh * a.slots * (DK / 32);
   const uint8_t *vc = a.vc + (int64_t)bh * a.slots * v_row + chunk * (DVC / 2), *vs = a.vs + (int64_t)bh * a.slots * vs_row + chunk * VB;
@@ -479,6 +469,7 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
     }
   };
   bool outside = false;                                // F16: a block that fp16 does not hold
+  u16x2 k_most = {0, 0};                               // and, of keys that stay bf16, their largest scale bytes
   auto store_values = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
@@ -539,7 +530,6 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
       const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
       l *= alpha;
-      l_used *= alpha;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i] *= alpha;
     }
@@ -549,7 +539,8 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
     load_values(base + 64);                  // (behind the slice: nothing is read, zeros come back)
     load_keys(kn, base + 128);
     const float mu = m == -INFINITY ? 0.f : m - P_UP;
-    if (F16 && wave == 0) outside |= !k[0].fits_f16() || !k[1].fits_f16();      // (all waves hold the same keys)
+    if (KEYS_F16 && wave == 0) outside |= !k[0].fits_f16() || !k[1].fits_f16();      // (all waves hold the same keys)
+    if (F16 && !KEYS_F16) { k[0].most(k_most); k[1].most(k_most); }
     xn[0] = q.dot(k[0]);
     xn[1] = q.dot(k[1]);
     V8 pf[4][PP];
@@ -559,10 +550,8 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
 #pragma unroll
       for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], scale, -mu));
       split8<PP>(p, pf[s]);
-      l_used = weight_sum<PARTS>(l_used, p, pf[s][0]);
-      if (PARTS == 1 && WEIGH)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) l += p[j];
+      for (int j = 0; j < 8; ++j) l += p[j];
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -585,7 +574,8 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
   if (s0 < s1) {
     load_keys(ka, s0);
     load_values(s0);
-    if (F16 && wave == 0) outside |= !ka[0].fits_f16() || !ka[1].fits_f16();
+    if (KEYS_F16 && wave == 0) outside |= !ka[0].fits_f16() || !ka[1].fits_f16();
+    if (F16 && !KEYS_F16) { ka[0].most(k_most); ka[1].most(k_most); }
     xa[0] = q.dot(ka[0]);
     xa[1] = q.dot(ka[1]);
     load_keys(ka, s0 + 64);
@@ -599,15 +589,13 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
     if (base + 64 >= s1) break;
     step(xb, xa, kb, ka, base + 64, 1);
   }
-  if (PARTS > 1) l = l_used;
   l += __shfl_xor(l, 32);
-  l_used += __shfl_xor(l_used, 32);
   m -= P_UP;
   if constexpr (F16) {
-    const int any = __syncthreads_or(outside);
-    if (tid == 0) a.redo[(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = any;
+    if (!KEYS_F16) outside |= k_most[0] > kBank4F16Most || k_most[1] > kBank4F16Most;
+    if (__syncthreads_or(outside)) return true;
   }
-  if (r >= a.rows) return;
+  if (r >= a.rows) return false;
   if (a.part_o) {
     const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + r;
 #pragma unroll
@@ -616,9 +604,9 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<f32x4 *>(a.part_o + at * a.value_dim + chunk * DVC + i * 32 + j * 8 + half * 4) =
             f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
-    if (half == 0 && chunk == 0) *reinterpret_cast<f32x4 *>(a.part_ml + at * 4) = live ? f32x4{m, l_used, l, 0.f} : f32x4{-INFINITY, 0.f, 0.f, 0.f};
+    if (half == 0 && chunk == 0) *reinterpret_cast<f32x2 *>(a.part_ml + at * 2) = live ? f32x2{m, l} : f32x2{-INFINITY, 0.f};
   } else {
-    const float inv = live && l_used != 0.f ? 1.f / l_used : 0.f;
+    const float inv = live && l != 0.f ? 1.f / l : 0.f;
     T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + h * a.group + r - t * a.group) * a.value_dim + chunk * DVC;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -631,6 +619,14 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
         *reinterpret_cast<Tx4 *>(out + i * 32 + j * 8 + half * 4) = y;
       }
   }
+  return false;
+}
+
+template <int DK, int DVC, int PARTS, bool CAUSAL>
+__global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_block_kernel(ReadArgs a) {
+  extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
+  __shared__ uint64_t nan_blocks[2][4][(DVC * 2 + 255) / 256];            // causal: the value blocks of a buffer that stand for NaN, a bit a lane of the wave that stored it
+  if (block_rows<DK, DVC, PARTS, true, CAUSAL>(a, vt, nan_blocks)) block_rows<DK, DVC, PARTS, false, CAUSAL>(a, vt, nan_blocks);
 }
 
 // weight[s] += sum over the rows of exp2(logit - maximum) / sum, each row's maximum and 1 / sum from bank4_join (one number, their logarithm
@@ -638,7 +634,8 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
 // runs over registers, the rows in order.  One workgroup: 128 * NS slots, NS x 32 a wave, their keys widened once into registers; 32 rows a
 // step go through LDS, copied as bank4_join has packed them in operand order.  (A wave that reads its rows as they lie in memory touches a
 // cache line a lane and load, and with 64 slots a workgroup the queries cross the L2 1.3 GB at 1620 x 32 400 x 2: 150 and 115 us.)
-// fp16 products (V8 = f16x8) and their flags as in bank4_block_kernel; SHIFT: fp32 rows were packed times a power of two of their own.
+// fp16 products (V8 = f16x8) as in bank4_block_kernel, but for a flag and a second launch (4.6 us where no flag is up); SHIFT: fp32 rows were packed
+// times a power of two of their own.
 template <int DK, int PARTS, int NS, typename V8, bool SHIFT>
 __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   constexpr bool F16 = std::is_same_v<V8, f16x8>;
@@ -649,8 +646,8 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   const int len = (int)read_len(a, b), cnt = read_count(a, b);
   const int rows = cnt * a.group;                       // (rows behind the count have no weight)
   if (first >= len || rows == 0) return;
-  int32_t *redo = a.redo + (a.redo ? blockIdx.y * gridDim.x + blockIdx.x : 0);
-  if (!F16 && a.redo && !*redo) return;
+  int32_t *redo = a.redo + blockIdx.y * gridDim.x + blockIdx.x;
+  if (!F16 && PARTS > 1 && !*redo) return;            // (bf16 queries: these products alone)
   const int64_t row_base = (int64_t)bh * a.slots;
   const auto rk = bank_rows(a.kc + (row_base + base) * (DK / 2), (int64_t)(len - base) * (DK / 2));
   const auto rs = bank_rows(a.ks + (row_base + base) * (DK / 32), (int64_t)(len - base) * (DK / 32));
@@ -743,33 +740,31 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   }
 }
 
-// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum of the weights as the output uses them,
-// 1 / their exact sum, and the factors of its slices' accumulators (-1: an empty slice).
+// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum of the weights, and the factors of its slices'
+// accumulators (-1: an empty slice).
 struct RowJoin {
-  float f[2], inv, top, inv_sum;
+  float f[2], inv, top;
   __device__ __forceinline__ RowJoin(const ReadArgs &a, int bh, int row, int lane) {
-    const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + row) * 4;
-    float m[2], u[2], l[2];
+    const float *ml = a.part_ml + ((int64_t)bh * a.nsplit * a.rows + row) * 2;
+    float m[2], l[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int s = lane + 64 * k;
-      const f32x4 v = s < a.nsplit ? *reinterpret_cast<const f32x4 *>(ml + (int64_t)s * a.rows * 4) : f32x4{-INFINITY, 0.f, 0.f, 0.f};
+      const f32x2 v = s < a.nsplit ? *reinterpret_cast<const f32x2 *>(ml + (int64_t)s * a.rows * 2) : f32x2{-INFINITY, 0.f};
       m[k] = v.x;
-      u[k] = v.y;
-      l[k] = v.z;
+      l[k] = v.y;
     }
     float mm = fmaxf(m[0], m[1]);
     for (int d = 1; d < 64; d <<= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     const float mu = mm == -INFINITY ? 0.f : mm;
     f[0] = __builtin_amdgcn_exp2f(m[0] - mu);
     f[1] = __builtin_amdgcn_exp2f(m[1] - mu);
-    float used = f[0] * u[0] + f[1] * u[1], sum = f[0] * l[0] + f[1] * l[1];
-    for (int d = 1; d < 64; d <<= 1) { used += __shfl_xor(used, d); sum += __shfl_xor(sum, d); }
-    inv = used != 0.f ? 1.f / used : 0.f;
+    float sum = f[0] * l[0] + f[1] * l[1];
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    inv = sum != 0.f ? 1.f / sum : 0.f;
     top = mu;
-    inv_sum = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) f[k] = m[k] == -INFINITY && u[k] == 0.f ? -1.f : f[k];       // an empty slice: its accumulators may be anything
+    for (int k = 0; k < 2; ++k) f[k] = m[k] == -INFINITY && l[k] == 0.f ? -1.f : f[k];       // an empty slice: its accumulators may be anything
   }
 };
 
@@ -788,7 +783,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
     if (gr >= (int64_t)a.batch * a.heads * a.rows) return;
     const int bh = (int)(gr / a.rows), row = (int)(gr - (int64_t)bh * a.rows), b = bh / a.heads, h = bh - b * a.heads;
     const RowJoin J(a, bh, row, lane);
-    if (a.row_max && chunk == 0 && lane == 0) { a.row_max[(int64_t)bh * a.row_stride + row] = J.top; a.row_inv[(int64_t)bh * a.row_stride + row] = J.inv_sum; }
+    if (a.row_max && chunk == 0 && lane == 0) { a.row_max[(int64_t)bh * a.row_stride + row] = J.top; a.row_inv[(int64_t)bh * a.row_stride + row] = J.inv; }
     const int t = row / a.group, j = h * a.group + row - t * a.group;
     T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + j) * a.value_dim;
     const float *part = a.part_o + ((int64_t)bh * a.nsplit * a.rows + row) * a.value_dim;
@@ -868,7 +863,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
   const int cnt = read_count(a, b);
   for (int i = wave; i < a.rows; i += 4) {
     const RowJoin J(a, bh, i, lane);
-    if (lane == 0) { top[i] = J.top; inv[i] = J.inv_sum; lim[i] = (int)read_limit(a, len, cnt, i / a.group); }
+    if (lane == 0) { top[i] = J.top; inv[i] = J.inv; lim[i] = (int)read_limit(a, len, cnt, i / a.group); }
   }
   __syncthreads();
   if (slot >= len) return;
@@ -931,7 +926,7 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   p->parts = p->nsplit > 1 || weigh;
   const int64_t n = (int64_t)k->batch * k->heads * p->nsplit * rows;
   p->part_o = p->parts ? n * k->value_dim * 4 : 0;
-  p->part_ml = p->parts ? n * 16 : 0;
+  p->part_ml = p->parts ? (n * 8 + 15) / 16 * 16 : 0;
   p->logit_stride = (k->slots + 63) / 64 * 64;
   p->logits = weigh && !p->block ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
   p->row_stride = (rows + 31) / 32 * 32;
@@ -939,31 +934,24 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   p->row_stat = packed * 12;
   p->q_pack = packed * k->key_dim * 2 * (f16 + 1);
   p->q_pack_f16 = packed * k->key_dim * 2 * f16;
-  const int64_t flags = groups * p->nsplit, flags_weigh = weigh ? (int64_t)k->batch * k->heads * ((k->slots + 127) / 128) : 0;
-  p->redo = p->block && f16 ? ((flags > flags_weigh ? flags : flags_weigh) * 4 + 15) / 16 * 16 : 0;
+  p->redo = weigh && p->block && f16 ? ((int64_t)k->batch * k->heads * ((k->slots + 127) / 128) * 4 + 15) / 16 * 16 : 0;
   return MIVOS_OK;
 }
 
-template <int DK, int DVC, int PARTS, bool F16, bool WEIGH, bool CAUSAL>
+template <int DK, int DVC, int PARTS, bool CAUSAL>
 static int block_launch_one(const ReadArgs &a, const dim3 grid, hipStream_t s) {
   constexpr size_t lds = 2 * 64 * (DVC + 16) * 2;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
-    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, F16, WEIGH, CAUSAL>, lds, raised, "bank4_read")) return rc;
+    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, CAUSAL>, lds, raised, "bank4_read")) return rc;
   }
-  bank4_block_kernel<DK, DVC, PARTS, F16, WEIGH, CAUSAL><<<grid, 256, lds, s>>>(a);
+  bank4_block_kernel<DK, DVC, PARTS, CAUSAL><<<grid, 256, lds, s>>>(a);
   return MIVOS_OK;
 }
 
-// (only rounded weights need a second sum: with 2 or 3 parts the one in use is exact)
 template <int DK, int DVC, int PARTS>
 static int block_launch(const ReadArgs &a, const dim3 grid, hipStream_t s) {
-  if constexpr (PARTS == 1) {
-    if (a.weigh) return a.causal ? block_launch_one<DK, DVC, 1, false, true, true>(a, grid, s) : block_launch_one<DK, DVC, 1, false, true, false>(a, grid, s);
-  } else {
-    if (int rc = a.causal ? block_launch_one<DK, DVC, PARTS, true, false, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, true, false, false>(a, grid, s)) return rc;
-  }
-  return a.causal ? block_launch_one<DK, DVC, PARTS, false, false, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, false, false, false>(a, grid, s);
+  return a.causal ? block_launch_one<DK, DVC, PARTS, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, false>(a, grid, s);
 }
 
 template <int DK, int PARTS>
@@ -1072,7 +1060,7 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (p.redo) a.redo = (int32_t *)(ws + need - p.redo);
   a.slots = bank->slots; a.logit_stride = p.logit_stride; a.row_stride = p.row_stride;
   a.batch = bank->batch; a.heads = bank->heads; a.group = q_heads / bank->heads; a.tokens = tokens; a.rows = p.rows;
-  a.key_dim = bank->key_dim; a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.weigh = weigh; a.scale_log2 = scale * LOG2E;
+  a.key_dim = bank->key_dim; a.value_dim = bank->value_dim; a.nsplit = p.nsplit; a.causal = causal; a.scale_log2 = scale * LOG2E;
   // logits are compared before they are scaled: a scale above 0, its sign (or the 0) with the queries
   a.q_sign = scale < 0.f ? -1.f : scale > 0.f ? 1.f : 0.f;
   a.scale_log2 = scale != 0.f ? a.scale_log2 * a.q_sign : 1.f;

@@ -676,3 +676,19 @@ def test_read_padded_tokens_are_zero(case, slots, dtype, weigh):
             for b in range(2):
                 assert not bool(got[b, counts[b]:].view(torch.uint8).any())
                 assert bool(got[b, :counts[b]].isnan().all()) == (nan and b == 0) or not counts[b]
+
+
+# ------------------------------------------------------------------------------------------------ precision of the products
+@pytest.mark.parametrize("tokens,p,floor", [(8, 2.0 ** -16, 0.0), (33, 2.0 ** -11, 2.0 ** -33), (150, 2.0 ** -11, 2.0 ** -33)])
+@pytest.mark.parametrize("lens", ((2, 3), (5, 70)))
+def test_read_bf16_queries_keep_their_weights(lens, tokens, p, floor):
+    """Few slots of near weights and values of either sign, so that an output is far below its terms and shows how its weights were rounded: two
+    bf16 numbers (2^-16 of each) with up to 32 rows, one fp16 number (half a step: 2^-11 of each, or 2^-25 / 2^8 of the row's largest) with more."""
+    bank = _filled(2, 1, 80, 64, 128, lens, seed=tokens)
+    keys, values = _rows(bank)
+    q = (0.4 * torch.randn(2, tokens, 1, 64, generator=torch.Generator().manual_seed(6))).bfloat16()
+    for causal in (False, True):
+        ref, _, mag, big = O.read(keys, values, bank.lens.cpu(), q.double(), torch.full((2,), tokens), 64 ** -0.5, causal)
+        got = ops.bank4_read(bank, q.to(DEV), causal=causal)
+        tol = (2.0 ** -8 + p) * ref.abs() + (p + 2 * (64 + 16) * U * big[..., None] + 2.0 ** -20) * mag
+        _within(got, ref, tol + 80 * (floor * values.nan_to_num(0).abs().amax((1, 2))[:, None, None] + 2.0 ** -126 * 6 * 2.0 ** 8))
