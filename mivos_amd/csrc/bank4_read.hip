@@ -37,7 +37,7 @@ struct ReadArgs {
   float *part_o, *part_ml, *logits, *row_max, *row_inv, *row_scale;
   __bf16 *q_pack;
   _Float16 *q_pack_f16;
-  int32_t *redo;          // bank4_weigh: a flag a workgroup, fp16 products met a block that they do not hold and the bf16 ones do it again
+  int32_t *redo;          // fp16 and fp32 queries: a flag a workgroup, fp16 products met a block that they do not hold, the bf16 ones do it again
   int64_t slots, logit_stride, row_stride;
   int batch, heads, group, tokens, rows, key_dim, value_dim, nsplit, causal, q_vec;
   float scale_log2;       // |scale| * log2(e): the softmax runs in powers of two; the sign of scale goes to the queries
@@ -404,229 +404,32 @@ struct QueryCols {
 // queries: keys and q as bf16, the weight times 2^8 in 1 (2^-11 of itself or 2^-33 of the row's largest; one bf16 number, 2^-8 of it, put the error of
 // 3 x 1021 causal tokens over 16 300 slots at 1.3 times that of fp32 weights, two take 489 us there: 359, 372 and 489).
 // A 4-bit value is exact in fp16 from 2^-24 to 6 * 2^13; a workgroup that has met a block outside, or keys above it, whose logits lie so far apart that
-// such weights lose channels, does its work again on bf16 numbers (twice the time and more, for that workgroup).  2 x 1620 fp32 rows x 32 400 slots,
+// such weights lose channels, does its work again on bf16 numbers (twice the time and more, for that workgroup; 5 us for the launch where no flag is up).  2 x 1620 fp32 rows x 32 400 slots,
 // 128 / 512: 400 us instead of 471, 0.81 PFLOP/s issued; all 512 value channels in one workgroup would need registers it does not have.
-// -> true: F16, and the workgroup has met such a block (nothing is written)
-template <int DK, int DVC, int PARTS, bool F16, bool CAUSAL, int VL = (DVC * 2 + 255) / 256>
-__device__ __forceinline__ bool block_rows(const ReadArgs &a, __bf16 *vt, uint64_t (&nan_blocks)[2][4][VL]) {
-  typedef typename ReadType<PARTS>::T T;
-  constexpr bool KEYS_F16 = F16 && PARTS > 1, SHIFT = F16 && PARTS == 3;
-  typedef std::conditional_t<KEYS_F16, f16x8, bf16x8> K8;
-  typedef std::conditional_t<F16, f16x8, bf16x8> V8;
-  constexpr int QP = KEYS_F16 ? PARTS - 1 : PARTS, PP = F16 && PARTS == 1 ? 1 : PARTS == 3 && !F16 ? 3 : 2;
-  constexpr float LAG = F16 ? PARTS == 1 ? 7.f : 3.f : MAX_LAG, P_UP = F16 ? PARTS == 1 ? 8.f : 12.f : 0.f;        // weights are exp2(logit - (maximum - P_UP)), up to 2^(LAG + P_UP)
-  constexpr int VS = DVC + 16, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
-  const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
-  const int split = blockIdx.x, row0 = blockIdx.y * 128, r = row0 + wave * 32 + col;
-  const int64_t len = read_len(a, b);
-  const int cnt = read_count(a, b), t = r / a.group;
-  const bool live = r < a.rows && t < cnt;
-  const int limit = live && CAUSAL ? (int)read_limit(a, len, cnt, t) : (int)len;
-  int last_t = (row0 + 127 < a.rows ? row0 + 127 : a.rows - 1) / a.group;
-  last_t = last_t < cnt ? last_t : cnt - 1;
-  const int seen = row0 / a.group < cnt ? (int)read_limit(a, len, cnt, last_t) : 0;
-  const int per = ((seen + 63) / 64 + a.nsplit - 1) / a.nsplit * 64;
-  const int s0 = (int64_t)split * per < seen ? split * per : seen, s1 = seen - s0 < per ? seen : s0 + per;
-  int low = limit;                                   // over the wave's rows
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int x = __shfl_xor(low, d);
-    low = x < low ? x : low;
-  }
-  low = __builtin_amdgcn_readfirstlane(low);
-
-  QueryCols<DK, QP, K8> q;
-  const float back = q.template load<SHIFT>((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign);
-  const float scale = SHIFT ? row_scale(a.scale_log2, back) : a.scale_log2;
-  f32x16 o[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  const int v_row = a.value_dim / 2, vs_row = a.value_dim / 32;
-  const uint8_t *kc = a.kc + (int64_t)bh * a.slots * (DK / 2), *ks = a.ks + (int64_t)bh * a.slots * (DK / 32);
-  const uint8_t *vc = a.vc + (int64_t)bh * a.slots * v_row + chunk * (DVC / 2), *vs = a.vs + (int64_t)bh * a.slots * vs_row + chunk * VB;
-  KeyRow<DK> ka[2], kb[2];
-  u32x4 vn[VL];
-  uint32_t vsn[VL];
-
-  auto load_keys = [&](KeyRow<DK> *to, int base) {
-    const int64_t n = s1 - base, at = base;
-    const auto rk = bank_rows(kc + at * (DK / 2), n * (DK / 2)), rs = bank_rows(ks + at * (DK / 32), n * (DK / 32));
-    to[0].load(rk, rs, 0, col, half);
-    to[1].load(rk, rs, 32, col, half);
-  };
-  auto load_values = [&](int base) {
-    const int64_t n = s1 - base, at = base;
-    const auto rv = bank_rows(vc + at * v_row, n * v_row - chunk * (DVC / 2)), rw = bank_rows(vs + at * vs_row, n * vs_row - chunk * VB);
-#pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      if (VE < 256 && tid >= VE) break;
-      vn[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, tid / VB * v_row + tid % VB * 16, i * (256 / VB) * v_row, 0);
-      vsn[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, tid / VB * vs_row + tid % VB, i * (256 / VB) * vs_row, 0);
-    }
-  };
-  bool outside = false;                                // F16: a block that fp16 does not hold
-  u16x2 k_most = {0, 0};                               // and, of keys that stay bf16, their largest scale bytes
-  auto store_values = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int e = i * 256 + tid, vr = e / VB, blk = e % VB;
-      if (VE < 256 && e >= VE) {
-        if (CAUSAL) nan_blocks[buf][wave][i] = 0;
-        break;
-      }
-      float sc = bank4_scale(vsn[i]);
-      if (F16) outside |= !bank4_fits_f16(vsn[i], vn[i]);
-      if (CAUSAL) {
-        nan_blocks[buf][wave][i] = __ballot(vsn[i] == kBank4NanScale);
-        sc = vsn[i] == kBank4NanScale ? 1.f : sc;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<V8 *>(vt + (buf * 64 + vr) * VS + blk * 32 + j * 8) = unpack8<V8>(vn[i][j], sc);
-    }
-  };
-  // Causal: a value block that stands for NaN makes it NaN for the rows that see its slot and is finite for the others, whose weight there is 0.
-  auto add_nans = [&](int buf, int base) {
-    uint64_t any = 0;
-#pragma unroll
-    for (int i = 0; i < 4 * VL; ++i) any |= nan_blocks[buf][i / VL][i % VL];
-    if (!any) return;
-    for (int i = 0; i < 4 * VL; ++i) {
-      for (uint64_t bad = nan_blocks[buf][i / VL][i % VL]; bad; bad &= bad - 1) {
-        const int e = i % VL * 256 + i / VL * 64 + __builtin_ctzll(bad);
-        const float add = base + e / VB < limit ? NAN : 0.f;
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-          if (c == e % VB) o[c] += add;
-      }
-    }
-  };
-
-  // The logits run one step ahead: their products are issued among the exponentials of the step before, their maximum among its second
-  // products.  The order inside a step is the compiler's: written out by hand, one product and at most four vector instructions behind it, the
-  // step takes a tenth fewer cycles and the chip holds a tenth less clock (fp32 on bf16 numbers: 57 % of the cycles matrix work at 1.78 GHz,
-  // against 46 % at 2.05; fp16 numbers: 43 % at 1.77): power is what bounds this kernel, as it bounds a large library product (1.2 of the 2.5 PFLOP/s).
-  float top;
-  auto row_top = [&](const f32x16 (&x)[2]) {
-    float t = fmaxf(x[0][0], x[1][0]);
-#pragma unroll
-    for (int j = 1; j < 16; ++j) t = fmaxf(fmaxf(t, x[0][j]), x[1][j]);
-    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
-    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * scale;
-  };
-  auto settle = [&](f32x16 (&x)[2], int base) {      // masks the logits of a step that not all rows see, moves the maximum if it has to
-    if (base + 64 > low || base + 64 > s1) {
-      const int lim = limit < s1 ? limit : s1;
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[s][j] = base + s * 32 + mfma32_row(j, lane) < lim ? x[s][j] : -INFINITY;
-      top = row_top(x);
-    }
-    if (__any(top > m + LAG)) {
-      const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) o[i] *= alpha;
-    }
-  };
-  auto step = [&](f32x16 (&x)[2], f32x16 (&xn)[2], const KeyRow<DK> (&k)[2], KeyRow<DK> (&kn)[2], int base, int buf) {
-    if (CAUSAL) add_nans(buf, base);
-    load_values(base + 64);                  // (behind the slice: nothing is read, zeros come back)
-    load_keys(kn, base + 128);
-    const float mu = m == -INFINITY ? 0.f : m - P_UP;
-    if (KEYS_F16 && wave == 0) outside |= !k[0].fits_f16() || !k[1].fits_f16();      // (all waves hold the same keys)
-    if (F16 && !KEYS_F16) { k[0].most(k_most); k[1].most(k_most); }
-    xn[0] = q.dot(k[0]);
-    xn[1] = q.dot(k[1]);
-    V8 pf[4][PP];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {           // 16 slots: keys 16 s + {0..3, 8..11} + 4 half
-      f32x8 p;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s / 2][(s & 1) * 8 + j], scale, -mu));
-      split8<PP>(p, pf[s]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) l += p[j];
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const __bf16 *at = vt + (buf * 64 + s * 16 + half * 4 + (lane & 15) / 4) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32));
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + i * 32 + 8 * VS));
-        const V8 vf = __builtin_bit_cast(V8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int w = 0; w < PP; ++w) o[i] = mfma32(vf, pf[s][w], o[i]);
-      }
-    }
-    top = row_top(xn);
-    store_values(buf ^ 1);
-    __syncthreads();
-    settle(xn, base + 64);
-  };
-  f32x16 xa[2], xb[2];
-  if (s0 < s1) {
-    load_keys(ka, s0);
-    load_values(s0);
-    if (KEYS_F16 && wave == 0) outside |= !ka[0].fits_f16() || !ka[1].fits_f16();
-    if (F16 && !KEYS_F16) { ka[0].most(k_most); ka[1].most(k_most); }
-    xa[0] = q.dot(ka[0]);
-    xa[1] = q.dot(ka[1]);
-    load_keys(ka, s0 + 64);
-    store_values(0);
-    top = row_top(xa);
-    settle(xa, s0);
-  }
-  __syncthreads();
-  for (int base = s0; base < s1; base += 128) {
-    step(xa, xb, ka, kb, base, 0);
-    if (base + 64 >= s1) break;
-    step(xb, xa, kb, ka, base + 64, 1);
-  }
-  l += __shfl_xor(l, 32);
-  m -= P_UP;
-  if constexpr (F16) {
-    if (!KEYS_F16) outside |= k_most[0] > kBank4F16Most || k_most[1] > kBank4F16Most;
-    if (__syncthreads_or(outside)) return true;
-  }
-  if (r >= a.rows) return false;
-  if (a.part_o) {
-    const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + r;
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<f32x4 *>(a.part_o + at * a.value_dim + chunk * DVC + i * 32 + j * 8 + half * 4) =
-            f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
-    if (half == 0 && chunk == 0) *reinterpret_cast<f32x2 *>(a.part_ml + at * 2) = live ? f32x2{m, l} : f32x2{-INFINITY, 0.f};
-  } else {
-    const float inv = live && l != 0.f ? 1.f / l : 0.f;
-    T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + h * a.group + r - t * a.group) * a.value_dim + chunk * DVC;
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        typedef T Tx4 __attribute__((ext_vector_type(4)));
-        Tx4 y;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = (T)(inv == 0.f ? 0.f : o[i][4 * j + c] * inv);
-        *reinterpret_cast<Tx4 *>(out + i * 32 + j * 8 + half * 4) = y;
-      }
-  }
-  return false;
+// F16: `again` says that the workgroup has met such a block; then it has written nothing.
+// (The body is in bank4_block.h, once as a kernel's own text and once as a function's: in a function that a kernel calls, the compiler orders a step
+// otherwise, and 3 x 1021 causal fp32 tokens over 16 300 slots take 860 us instead of 800.)
+// fp16 and fp32 queries: F16 raises the workgroup's flag, and the bf16 kernel is launched behind.
+template <int DK, int DVC, int PARTS, bool F16, bool CAUSAL>
+__global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_block_kernel(ReadArgs a) {
+  int32_t *redo = a.redo + (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+  if (!F16 && !*redo) return;
+  bool again = false;
+#include "bank4_block.h"
+  if (F16 && threadIdx.x == 0) *redo = again;
 }
 
-template <int DK, int DVC, int PARTS, bool CAUSAL>
-__global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_block_kernel(ReadArgs a) {
-  extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
-  __shared__ uint64_t nan_blocks[2][4][(DVC * 2 + 255) / 256];            // causal: the value blocks of a buffer that stand for NaN, a bit a lane of the wave that stored it
-  if (block_rows<DK, DVC, PARTS, true, CAUSAL>(a, vt, nan_blocks)) block_rows<DK, DVC, PARTS, false, CAUSAL>(a, vt, nan_blocks);
+// bf16 queries: both in one launch (a second one is 2 us of a call over few slots).
+template <int DK, int DVC, bool F16, bool CAUSAL>
+__device__ __forceinline__ bool block_rows_bf16(const ReadArgs &a) {
+  constexpr int PARTS = 1;
+  bool again = false;
+#include "bank4_block.h"
+  return again;
+}
+template <int DK, int DVC, bool CAUSAL>
+__global__ __launch_bounds__(256, block_occupancy(DK, DVC, 1)) void bank4_block_bf16_kernel(ReadArgs a) {
+  if (block_rows_bf16<DK, DVC, true, CAUSAL>(a)) block_rows_bf16<DK, DVC, false, CAUSAL>(a);
 }
 
 // weight[s] += sum over the rows of exp2(logit - maximum) / sum, each row's maximum and 1 / sum from bank4_join (one number, their logarithm
@@ -634,8 +437,7 @@ __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_bl
 // runs over registers, the rows in order.  One workgroup: 128 * NS slots, NS x 32 a wave, their keys widened once into registers; 32 rows a
 // step go through LDS, copied as bank4_join has packed them in operand order.  (A wave that reads its rows as they lie in memory touches a
 // cache line a lane and load, and with 64 slots a workgroup the queries cross the L2 1.3 GB at 1620 x 32 400 x 2: 150 and 115 us.)
-// fp16 products (V8 = f16x8) as in bank4_block_kernel, but for a flag and a second launch (4.6 us where no flag is up); SHIFT: fp32 rows were packed
-// times a power of two of their own.
+// fp16 products (V8 = f16x8) and their flags as in bank4_block_kernel; SHIFT: fp32 rows were packed times a power of two of their own.
 template <int DK, int PARTS, int NS, typename V8, bool SHIFT>
 __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   constexpr bool F16 = std::is_same_v<V8, f16x8>;
@@ -934,24 +736,30 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   p->row_stat = packed * 12;
   p->q_pack = packed * k->key_dim * 2 * (f16 + 1);
   p->q_pack_f16 = packed * k->key_dim * 2 * f16;
-  p->redo = weigh && p->block && f16 ? ((int64_t)k->batch * k->heads * ((k->slots + 127) / 128) * 4 + 15) / 16 * 16 : 0;
+  const int64_t flags = groups * p->nsplit, flags_weigh = weigh ? (int64_t)k->batch * k->heads * ((k->slots + 127) / 128) : 0;
+  p->redo = p->block && f16 ? ((flags > flags_weigh ? flags : flags_weigh) * 4 + 15) / 16 * 16 : 0;
   return MIVOS_OK;
 }
 
-template <int DK, int DVC, int PARTS, bool CAUSAL>
+template <int DK, int DVC, int PARTS, bool F16, bool CAUSAL>
 static int block_launch_one(const ReadArgs &a, const dim3 grid, hipStream_t s) {
   constexpr size_t lds = 2 * 64 * (DVC + 16) * 2;
+  void (*kernel)(ReadArgs);
+  if constexpr (PARTS == 1) kernel = bank4_block_bf16_kernel<DK, DVC, CAUSAL>;
+  else kernel = bank4_block_kernel<DK, DVC, PARTS, F16, CAUSAL>;
   if constexpr (lds > 65536) {
     static std::atomic<uint64_t> raised{0};
-    if (int rc = ensure_dynamic_lds((const void *)bank4_block_kernel<DK, DVC, PARTS, CAUSAL>, lds, raised, "bank4_read")) return rc;
+    if (int rc = ensure_dynamic_lds((const void *)kernel, lds, raised, "bank4_read")) return rc;
   }
-  bank4_block_kernel<DK, DVC, PARTS, CAUSAL><<<grid, 256, lds, s>>>(a);
+  kernel<<<grid, 256, lds, s>>>(a);
   return MIVOS_OK;
 }
 
 template <int DK, int DVC, int PARTS>
 static int block_launch(const ReadArgs &a, const dim3 grid, hipStream_t s) {
-  return a.causal ? block_launch_one<DK, DVC, PARTS, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, false>(a, grid, s);
+  if (int rc = a.causal ? block_launch_one<DK, DVC, PARTS, true, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, true, false>(a, grid, s)) return rc;
+  if constexpr (PARTS > 1) return a.causal ? block_launch_one<DK, DVC, PARTS, false, true>(a, grid, s) : block_launch_one<DK, DVC, PARTS, false, false>(a, grid, s);
+  return MIVOS_OK;
 }
 
 template <int DK, int PARTS>
