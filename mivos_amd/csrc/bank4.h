@@ -42,8 +42,10 @@ __device__ __forceinline__ f16x8 bank4_unpack8_f16(uint32_t codes, float scale) 
 }
 // 0.5 * 2^(byte - 127) >= 2^-24 and 6 * 2^(byte - 127) <= 6 * 2^13, or a block of zeros (under kBank4NanScale too: the conversion answers NaN)
 constexpr uint32_t kBank4F16Least = 104, kBank4F16Most = 140;
-__device__ __forceinline__ bool bank4_fits_f16(uint32_t byte, u32x4 codes) {
-  return byte - kBank4F16Least <= kBank4F16Most - kBank4F16Least || ((codes[0] | codes[1] | codes[2] | codes[3]) & 0x77777777u) == 0;
+__device__ __forceinline__ bool bank4_zeros(u32x4 codes) { return ((codes[0] | codes[1] | codes[2] | codes[3]) & 0x77777777u) == 0; }
+// (most: a smaller limit of the caller's)
+__device__ __forceinline__ bool bank4_fits_f16(uint32_t byte, u32x4 codes, uint32_t most = kBank4F16Most) {
+  return (byte >= kBank4F16Least && byte <= most) || bank4_zeros(codes);
 }
 
 // 8 consecutive elements of a row as fp32; `vec`: the address is a multiple of 16 bytes

@@ -8,6 +8,7 @@
   constexpr int VS = DVC + 16, NT = DVC / 32, VB = DVC / 32, VE = 64 * VB, VL = (VE + 255) / 256;
   extern __shared__ __align__(16) __bf16 vt[];         // two buffers of 64 rows
   __shared__ uint64_t nan_blocks[2][4][VL];            // causal: the value blocks of a buffer that stand for NaN, a bit a lane of the wave that stored it
+  __shared__ uint32_t key_limit;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
   const int nvc = a.value_dim / DVC, chunk = blockIdx.z % nvc, bh = blockIdx.z / nvc, b = bh / a.heads, h = bh - b * a.heads;
   const int split = blockIdx.x, row0 = blockIdx.y * 128, r = row0 + wave * 32 + col;
@@ -29,8 +30,17 @@
   low = __builtin_amdgcn_readfirstlane(low);
 
   QueryCols<DK, QP, K8> q;
-  const float back = q.template load<SHIFT>((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign);
+  float lost = 0.f;
+  const float back = q.template load<SHIFT>((const T *)a.q + b * a.qb + (int64_t)(live ? t : 0) * a.qt + (int64_t)(h * a.group + (live ? r - t * a.group : 0)) * a.qh, half, live, a.q_vec, a.q_sign, lost);
   const float scale = SHIFT ? row_scale(a.scale_log2, back) : a.scale_log2;
+  uint32_t key_most = kBank4F16Most;
+  if constexpr (SHIFT) {                                // over the workgroup's rows
+    if (tid == 0) key_limit = kBank4F16Most;
+    __syncthreads();
+    if (lost != 0.f) atomicMin(&key_limit, key_byte_limit(lost, scale));
+    __syncthreads();
+    key_most = __builtin_amdgcn_readfirstlane(key_limit);
+  }
   f32x16 o[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -131,7 +141,7 @@
     load_values(base + 64);                  // (behind the slice: nothing is read, zeros come back)
     load_keys(kn, base + 128);
     const float mu = m == -INFINITY ? 0.f : m - P_UP;
-    if (KEYS_F16 && wave == 0) outside |= !k[0].fits_f16() || !k[1].fits_f16();      // (all waves hold the same keys)
+    if (KEYS_F16 && wave == 0) outside |= !k[0].fits_f16(key_most) || !k[1].fits_f16(key_most);      // (all waves hold the same keys)
     if (F16 && !KEYS_F16) { k[0].most(k_most); k[1].most(k_most); }
     xn[0] = q.dot(k[0]);
     xn[1] = q.dot(k[1]);
@@ -166,7 +176,7 @@
   if (s0 < s1) {
     load_keys(ka, s0);
     load_values(s0);
-    if (KEYS_F16 && wave == 0) outside |= !ka[0].fits_f16() || !ka[1].fits_f16();
+    if (KEYS_F16 && wave == 0) outside |= !ka[0].fits_f16(key_most) || !ka[1].fits_f16(key_most);
     if (F16 && !KEYS_F16) { ka[0].most(k_most); ka[1].most(k_most); }
     xa[0] = q.dot(ka[0]);
     xa[1] = q.dot(ka[1]);

@@ -35,6 +35,7 @@ struct ReadArgs {
   void *out;
   int64_t qb, qt, qh;
   float *part_o, *part_ml, *logits, *row_max, *row_inv, *row_scale;
+  uint32_t *row_limit;    // bank4_weigh: the key_byte_limit of 32 rows, at the first of them
   __bf16 *q_pack;
   _Float16 *q_pack_f16;
   int32_t *redo;          // fp16 and fp32 queries: a flag a workgroup, fp16 products met a block that they do not hold, the bf16 ones do it again
@@ -102,6 +103,23 @@ __device__ __forceinline__ int query_shift(float top) {
 // where it is held back the products of fp16 blocks are far below 1 or far past every weight all the same
 __device__ __forceinline__ float row_scale(float scale_log2, float back) { return fminf(fmaxf(scale_log2 * back, 0x1p-126f), 0x1.fffffep127f); }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 .. 127
+
+// A row's channels as two fp16 numbers each: 2^-22 of the channel, but below 2^-3 (2^-16 of the row's largest) half of 2^-24.  What that leaves out
+// beyond 2^-22 of a channel, summed over the row, bounds the error of its logits by the keys they meet; keys that could take it past 2^-22 are for
+// bf16 numbers: the largest scale byte that may stay (normal rows against normal keys of 128 channels reach that at 2^16 times their size).
+__device__ __forceinline__ float left_out(f32x8 x, const f16x8 (&p)[2]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float r = __builtin_fabsf((x[j] - (float)p[0][j]) - (float)p[1][j]);
+    sum += r > 0x1p-22f * __builtin_fabsf(x[j]) ? r : 0.f;
+  }
+  return sum;
+}
+__device__ __forceinline__ uint32_t key_byte_limit(float lost, float scale) {
+  const uint32_t byte = __float_as_uint(0x1p-22f / 6.f / (lost * scale)) >> 23;       // 6 * 2^(byte - 127) * lost * scale <= 2^-22; nothing lost: 255
+  return byte < kBank4F16Most ? byte : kBank4F16Most;
+}
 
 template <int PARTS> struct ReadType;
 template <> struct ReadType<1> { typedef __bf16 T; };
@@ -339,10 +357,10 @@ struct KeyRow {
 #pragma unroll
     for (int i = 0; i < (KI + 1) / 2; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, scales[i] & 0x00ff00ffu));
   }
-  __device__ __forceinline__ bool fits_f16() const {
+  __device__ __forceinline__ bool fits_f16(uint32_t most = kBank4F16Most) const {
     bool ok = true;
 #pragma unroll
-    for (int i = 0; i < KI; ++i) ok &= bank4_fits_f16(byte(i), codes[i]);
+    for (int i = 0; i < KI; ++i) ok &= bank4_fits_f16(byte(i), codes[i], most);
     return ok;
   }
 };
@@ -351,9 +369,9 @@ struct KeyRow {
 template <int DK, int PARTS, typename V>
 struct QueryCols {
   V f[DK / 16][PARTS];
-  // SHIFT: the row times 2^t, t its query_shift -> 2^-t
+  // SHIFT: the row times 2^t, t its query_shift -> 2^-t; lost: left_out of it
   template <bool SHIFT, typename T>
-  __device__ __forceinline__ float load(const T *row, int half, bool live, bool vec, float sign) {
+  __device__ __forceinline__ float load(const T *row, int half, bool live, bool vec, float sign, float &lost) {
     auto channels = [&](int i) {
       f32x8 x = load8(row + i / 4 * 64 + half * 32 + i % 4 * 8, vec);
 #pragma unroll
@@ -374,7 +392,12 @@ struct QueryCols {
       back = pow2(-t);
     }
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i) split8<PARTS>(SHIFT ? channels(i) * up : channels(i), f[i]);
+    for (int i = 0; i < DK / 16; ++i) {
+      const f32x8 x = SHIFT ? channels(i) * up : channels(i);
+      split8<PARTS>(x, f[i]);
+      if constexpr (SHIFT) lost += left_out(x, f[i]);
+    }
+    if (SHIFT) lost += __shfl_xor(lost, 32);
     return back;
   }
   __device__ __forceinline__ f32x16 dot(const KeyRow<DK> &k) const {       // [32 keys][32 queries]
@@ -455,15 +478,31 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   const auto rs = bank_rows(a.ks + (row_base + base) * (DK / 32), (int64_t)(len - base) * (DK / 32));
   V8 kf[NS][KS];
   bool outside = false;
+  uint32_t key_byte = 0;                                // SHIFT: the largest scale byte of the lane's blocks that are not zeros
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     KeyRow<DK> k;
     k.load(rk, rs, s * 32, col, half);
     if (F16) outside |= !k.fits_f16();
+    if (SHIFT)
+#pragma unroll
+      for (int i = 0; i < DK / 64; ++i)
+        if (!bank4_zeros(k.codes[i]) && k.byte(i) > key_byte) key_byte = k.byte(i);
 #pragma unroll
     for (int i = 0; i < DK / 64; ++i)
 #pragma unroll
       for (int u = 0; u < 4; ++u) kf[s][i * 4 + u] = unpack8<V8>(k.codes[i][u], k.scale(i));
+  }
+  if constexpr (SHIFT) {
+    __shared__ uint32_t key_limit;
+    if (tid == 0) key_limit = kBank4F16Most;
+    __syncthreads();
+    for (int i = tid * 32; i < rows; i += 256 * 32) {
+      const uint32_t limit = a.row_limit[(int64_t)bh * a.row_stride + i];
+      if (limit < kBank4F16Most) atomicMin(&key_limit, limit);
+    }
+    __syncthreads();
+    outside |= key_byte > key_limit;
   }
   if constexpr (F16) {
     const int any = __syncthreads_or(outside);
@@ -629,7 +668,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
       for (int c = 0; c < 8; ++c) y[c] = live ? y[c] * a.q_sign : 0.f;
       return y;
     };
-    float up = 1.f;
+    float up = 1.f, scale = 1.f, lost = 0.f;
     if constexpr (PARTS == 3) {
       float top = 0.f;
       for (int i = 0; i < KS; ++i) {
@@ -639,7 +678,8 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
       }
       const int t = query_shift(fmaxf(top, __shfl_xor(top, 32)));
       up = pow2(t);
-      if (half == 0) a.row_scale[(int64_t)bh * a.row_stride + r] = row_scale(a.scale_log2, pow2(-t));
+      scale = row_scale(a.scale_log2, pow2(-t));
+      if (half == 0) a.row_scale[(int64_t)bh * a.row_stride + r] = scale;
     }
     for (int i = 0; i < KS; ++i) {
       const f32x8 y = channels(i);
@@ -650,9 +690,18 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
       if constexpr (PARTS > 1) {
         f16x8 hf[PARTS - 1];
         split8<PARTS - 1>(y * up, hf);
+        if constexpr (PARTS == 3) lost += left_out(y * up, hf);
 #pragma unroll
         for (int p = 0; p < PARTS - 1; ++p) (reinterpret_cast<f16x8 *>(a.q_pack_f16) + g * (KS * (PARTS - 1) * 64) + lane)[(i * (PARTS - 1) + p) * 64] = hf[p];
       }
+    }
+    if constexpr (PARTS == 3) {
+      uint32_t limit = key_byte_limit(lost + __shfl_xor(lost, 32), scale);
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t x = __shfl_xor(limit, d);
+        limit = x < limit ? x : limit;
+      }
+      if (lane == 0) a.row_limit[(int64_t)bh * a.row_stride + tile * 32] = limit;
     }
     return;
   }
@@ -733,7 +782,7 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   p->logits = weigh && !p->block ? (int64_t)k->batch * k->heads * rows * p->logit_stride * 4 : 0;
   p->row_stride = (rows + 31) / 32 * 32;
   const int64_t packed = weigh && p->block ? (int64_t)k->batch * k->heads * p->row_stride : 0, f16 = query_parts(dtype) - 1;
-  p->row_stat = packed * 12;
+  p->row_stat = packed * 16;
   p->q_pack = packed * k->key_dim * 2 * (f16 + 1);
   p->q_pack_f16 = packed * k->key_dim * 2 * f16;
   const int64_t flags = groups * p->nsplit, flags_weigh = weigh ? (int64_t)k->batch * k->heads * ((k->slots + 127) / 128) : 0;
@@ -860,8 +909,9 @@ extern "C" int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t 
   if (p.logits) a.logits = (float *)(ws + p.part_o + p.part_ml);
   if (p.row_stat) {
     a.row_max = (float *)(ws + p.part_o + p.part_ml);
-    a.row_inv = a.row_max + p.row_stat / 12;
-    a.row_scale = a.row_inv + p.row_stat / 12;
+    a.row_inv = a.row_max + p.row_stat / 16;
+    a.row_scale = a.row_inv + p.row_stat / 16;
+    a.row_limit = (uint32_t *)(a.row_scale + p.row_stat / 16);
     a.q_pack = (__bf16 *)(ws + p.part_o + p.part_ml + p.row_stat);
     a.q_pack_f16 = (_Float16 *)((char *)a.q_pack + p.q_pack);
   }

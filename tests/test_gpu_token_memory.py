@@ -692,3 +692,21 @@ def test_read_bf16_queries_keep_their_weights(lens, tokens, p, floor):
         got = ops.bank4_read(bank, q.to(DEV), causal=causal)
         tol = (2.0 ** -8 + p) * ref.abs() + (p + 2 * (64 + 16) * U * big[..., None] + 2.0 ** -20) * mag
         _within(got, ref, tol + 80 * (floor * values.nan_to_num(0).abs().amax((1, 2))[:, None, None] + 2.0 ** -126 * 6 * 2.0 ** 8))
+
+
+@pytest.mark.parametrize("weigh", (False, True))
+@pytest.mark.parametrize("which", ("blocks", "silent channel"))
+def test_read_fp32_queries_of_far_apart_channels(which, weigh):
+    """fp32 rows whose largest channels meet the smallest keys, or keys of 0, and whose logits come from channels 2^30 below: held to 24 bits all the same."""
+    bank = _filled(2, 1, 700, 64, 64, (700, 333))
+    q = torch.randn(2, 70, 2, 64, generator=torch.Generator().manual_seed(8))
+    if which == "blocks":
+        bank.key_scales[..., 0], bank.key_scales[..., 1] = 104, 140
+        q[..., 32:] *= 2.0 ** -30
+        scale = 2.0 ** 15
+    else:
+        bank.key_codes[..., 2] &= 0x0f                             # channel 5
+        q[..., 5] = 2.0 ** 32
+        scale = None
+    for causal in (False, True):
+        _check_read(bank, q, causal, None, weigh, scale=scale)
