@@ -710,3 +710,61 @@ def test_read_fp32_queries_of_far_apart_channels(which, weigh):
         scale = None
     for causal in (False, True):
         _check_read(bank, q, causal, None, weigh, scale=scale)
+
+
+def _check_many(bank, q, causal, weigh, scale):
+    """_check_read for 33 rows and more, with what these hold of a bf16 row's softmax weights: an fp16 number after a factor of 2^8, the row's largest at
+    least 2^8, so 2^-11 of each, or half of fp16's smallest step, 2^-25 / 2^8 = 2^-33 of the row's largest (a slot, times the channel's largest value)."""
+    if q.dtype != torch.bfloat16:
+        return _check_read(bank, q, causal, None, weigh, scale=scale)
+    keys, values = _rows(bank)
+    d, t = q.shape[3], q.shape[1]
+    ref, received, mag, big = O.read(keys, values, bank.lens.cpu(), q.double(), torch.full((q.shape[0],), t), scale or d ** -0.5, causal)
+    base = bank.weight.double().cpu()
+    got = ops.bank4_read(bank, q.to(DEV), scale=scale, causal=causal, weigh=weigh)
+    top = values.nan_to_num(0).abs().amax(2).clamp(max=6 * 2.0 ** 13).repeat_interleave(q.shape[2] // bank.heads, 1)[:, None]
+    dlt = (d + 16) * U * big[..., None]
+    _within(got, ref, (HALF[q.dtype] + 2.0 ** -11) * ref.abs() + (2.0 ** -11 + 2 * dlt + 2.0 ** -20) * mag + bank.slots * (2.0 ** -33 * top + 2.0 ** -126 * 6 * 2.0 ** 8))
+    rows = t * q.shape[2] // bank.heads
+    total = base + received if weigh else base
+    _within(bank.weight, total, (2 * (d + 16) * U * big.amax() + 2.0 ** -20 + rows * U) * received + 2 * U * total.abs() + rows * 2.0 ** -126)
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("tokens", (10, 90))
+def test_read_blocks_that_append_marked(tokens, dtype):
+    """Keys and values with infinities and NaN as append writes them (codes 0 under the scale byte 255): NaN for the rows that see them, and no others."""
+    bank = _filled(2, 1, 300, 64, 128, (300, 250))
+    g = torch.Generator().manual_seed(tokens)
+    k, v = torch.randn(2, 1, 1, 64, generator=g), torch.randn(2, 1, 1, 128, generator=g)
+    v[0, 0, 0, 40], k[1, 0, 0, 3] = float("inf"), float("nan")
+    lens = bank.lens.clone()
+    ops.bank4_append(bank, k.to(DEV), v.to(DEV), at=lens - 5)
+    bank.lens.copy_(lens)
+    assert int(bank.value_scales[0, 0, 295, 1]) == 255 and not bool(bank.value_codes[0, 0, 295, 16:32].any()) and int(bank.key_scales[1, 0, 245, 0]) == 255
+    q = torch.randn(2, tokens, 2, 64, generator=g).to(dtype)
+    for causal, seeing in ((True, 5), (False, tokens)):
+        got = _check_read(bank, q, causal, None, False).isnan()
+        assert bool(got[0, -seeing:, :, 32:64].all()) and int(got[0].sum()) == seeing * 2 * 32
+        assert bool(got[1, -seeing:].all()) and int(got[1].sum()) == seeing * 2 * 128
+    ops.bank4_read(bank, q.to(DEV), causal=True, weigh=True)       # the first stream's keys are numbers, so its weights are; the other's are NaN
+    keys, values = _rows(bank)
+    _, ref, _, big = O.read(keys, values, bank.lens.cpu(), q.double(), torch.full((2,), tokens), 64 ** -0.5, True)
+    d = (64 * PART[dtype][1] + 16) * U * big[0].max()
+    _within(bank.weight[0], ref[0], (2 * d + 2.0 ** -20 + 2 * tokens * U) * ref[0] + 2 * tokens * 2.0 ** -126)
+    assert torch.equal(bank.weight[1].isnan().cpu(), ref[1].isnan())
+
+
+@pytest.mark.parametrize("weigh", (False, True))
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("which", ("keys", "values"))
+def test_read_smallest_blocks_that_fp16_holds(which, dtype, weigh):
+    """Scale bytes 104 .. 112 and their neighbours below: codes of 2^-24 and up, subnormal in fp16."""
+    bank = _filled(2, 1, 700, 64, 128, (700, 333))
+    scales = bank.key_scales if which == "keys" else bank.value_scales
+    for lowest in (104, 102):
+        scales.copy_((lowest + torch.arange(scales.numel()) % 9).view(scales.shape))
+        q = 2 * torch.randn(2, 70, 2, 64, generator=torch.Generator().manual_seed(8))
+        for causal in (False, True):
+            _check_many(bank, q.to(dtype), causal, weigh, 2.0 ** 15 if which == "keys" else None)
