@@ -6,9 +6,9 @@
 //   dx = r (w g - x r^2 mean(w g x)),  r = (mean(x^2) + eps)^(-1/2),      dw = sum over the rows of g x r.
 //
 // The angle.  A position times a frequency is needed modulo a turn only, so the frequency is kept as a 64-bit fraction of a turn and the
-// product taken modulo 2^64: exact to 2^-33 turns for every 32-bit position (an fp32 product is off by 0.004 radian at position 70 000).
-// Sine and cosine are Taylor polynomials on an eighth of a turn to either side (error < 2^-24), once a token and pair: a workgroup puts them in LDS
-// and all heads of its tokens read them there.
+// product taken modulo 2^64 and rounded to 2^-32 turns: off by 2^-33 turns, and 2^-34 for the frequency, at every 32-bit position (an fp32
+// product is off by 0.004 radian at position 70 000).  Sine and cosine are Taylor polynomials on an eighth of a turn to either side
+// (error < 2^-24), once a token and pair: a workgroup puts them in LDS and all heads of its tokens read them there.
 //
 // Bound: bytes.  Every row is read once and written once (backward: x and dy once, dx once); a row of 16 * U channels is held by
 // 2^ceil(log2 U) neighbouring lanes, 16 channels a lane, so the mean is log2 lane exchanges and nothing is staged.
@@ -39,7 +39,7 @@ struct RotaryArgs {
 
 // sine and cosine of pos * freq turns (freq in 2^-64 turns)
 __device__ __forceinline__ void turn_sincos(int32_t pos, uint64_t freq, float sign, float &s, float &c) {
-  const uint32_t turn = (uint32_t)(((uint64_t)(int64_t)pos * freq) >> 32);
+  const uint32_t turn = (uint32_t)(((uint64_t)(int64_t)pos * freq + 0x80000000u) >> 32);      // (rounded to 2^-32 turns)
   const uint32_t quarter = (turn + 0x20000000u) >> 30;
   const float x = (float)(int32_t)(turn - (quarter << 30)) * 1.4629180792671596e-9f;      // 2 pi / 2^32: [-pi/4, pi/4)
   const float z = x * x;

@@ -1110,7 +1110,7 @@ class RotaryAxes:
     """Plan of a rotary position with several axes: `sections[a]` channel pairs turn with axis a (time, height, width, ...), the channels
     behind the pairs are not turned.  Pair j of a section of n has the frequency base^(-j / n); shared=True: one ladder over all pairs,
     base^(-i / sum(sections)).  interleaved=True pairs neighbouring channels, else channel i goes with i + sum(sections).  The device
-    table keeps every frequency as a 64-bit fraction of a turn, so angles are exact for every int32 position."""
+    table keeps every frequency as a 64-bit fraction of a turn, so angles are right to 2^-32 turns for every int32 position."""
     __slots__ = ("head_dim", "sections", "pairs", "interleaved", "freq", "axis", "tables")
 
     def __init__(self, head_dim, sections, base=10000.0, shared=False, interleaved=False, device="cuda"):

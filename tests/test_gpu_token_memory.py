@@ -9,6 +9,8 @@ of 2^-24):
              d = (Dk parts + 16) u A, the error of a logit with A = max sum |q| |k| scale (x log2 e folded: the factor 2).
   weight     (2 d + 2^-20 + rows u) of the value, and 2^-126 a row: the exponential gives 0 below the smallest normal fp32 number, so each
              row's share is off by less than that number (1.18e-38); for the same reason a read's elements by slots 2^-126 max |v|, below 6 * 2^8 here."""
+import math
+
 import pytest
 import torch
 
@@ -768,3 +770,21 @@ def test_read_smallest_blocks_that_fp16_holds(which, dtype, weigh):
         q = 2 * torch.randn(2, 70, 2, 64, generator=torch.Generator().manual_seed(8))
         for causal in (False, True):
             _check_many(bank, q.to(dtype), causal, weigh, 2.0 ** 15 if which == "keys" else None)
+
+
+# ------------------------------------------------------------------------------------------------ angles
+def test_rotary_angles_are_rounded_not_cut():
+    """Angles next to whole multiples of 2^-32 turns: off by half of that (and 2^-34 for the frequency), so the sine of a small one is off by
+    2 pi (2^-33 + 2^-34) and 2^-21 of itself (sine 4u, product u, frequency's double precision none)."""
+    for dim in (4, 16):                                            # a wave a row; 16 channels a lane
+        pairs, r = dim // 2, 0.8
+        base = (2 * math.pi * r * 2.0 ** -32) ** -pairs            # the second pair turns by r 2^-32 turns a position
+        plan = ops.RotaryAxes(dim, (pairs,), base=base, device=DEV)
+        pos = torch.arange(-9, 10, dtype=torch.int32)
+        x = torch.zeros(1, 19, 1, dim)
+        x[..., 1] = 1
+        for sign, call in ((1, ops.rotary_axes), (-1, ops.rotary_axes_grad)):
+            y = call(x.to(DEV), None, pos.to(DEV).view(1, 19, 1), plan)[0]
+            ref = sign * torch.sin(pos.double() * 2 * math.pi * r * 2.0 ** -32)
+            got = y[0, :, 0, 1 + pairs].double().cpu()
+            assert bool(((got - ref).abs() <= 2 * math.pi * (2.0 ** -33 + 2.0 ** -34) + 2.0 ** -21 * ref.abs()).all()), (dim, sign, got, ref)
