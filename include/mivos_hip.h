@@ -506,8 +506,8 @@ typedef struct {
   int32_t batch, heads, key_dim, value_dim;                       /* dims: multiples of 32 up to 1024     */
 } mivos_bank4;
 /* keys [batch][tokens][heads][key_dim], values [...][value_dim] (strides as above): token t < count[b] (NULL: all) of stream b goes to slot
- * at[b] + t, its weight becomes 0, lens[b] = at[b] + count[b].  at may be bank->lens itself (append behind what is there).  Tokens whose
- * slot is outside the bank are dropped and raise status bit 0. */
+ * at[b] + t, its weight becomes 0, lens[b] = at[b] + count[b].  at may be bank->lens itself (append behind what is there); otherwise neither at
+ * nor count may overlap it.  Tokens whose slot is outside the bank are dropped and raise status bit 0. */
 int mivos_bank4_append(const mivos_bank4 *bank, const void *keys, int64_t kb, int64_t kt, int64_t kh, const void *values, int64_t vb, int64_t vt,
                        int64_t vh, int dtype, const int32_t *at, const int32_t *count, int tokens, void *stream);
 /* What slots [first[b], first[b] + count) (first NULL: 0) stand for: dense [batch][heads][count][key_dim] / [value_dim], fp32 or bf16 (both
@@ -522,7 +522,7 @@ int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int q_heads, i
 int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t qb, int64_t qt, int64_t qh, int dtype, int q_heads, int tokens, const int32_t *count,
                      float scale, int causal, int weigh, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 /* Keeps `keep` slots of every (stream, head): the first `first`, the last `recent` and, of the others, those with the largest weight (equal
- * weights: the lowest slots; NaN counts as the least), in their order, in bank `out` (other buffers, slots >= keep) with their weights;
+ * weights: the lowest slots; NaN counts as the least), in their order, in bank `out` (sharing no buffer, slots >= keep) with their weights;
  * out->lens[b] = min(lens[b], keep).  slots_out [batch][heads][keep]: the slots they came from, -1 behind them.  Rows of `out` behind its new
  * length are left as they were. */
 int mivos_bank4_evict(const mivos_bank4 *bank, const mivos_bank4 *out, int64_t keep, int64_t first, int64_t recent, int32_t *slots_out, void *stream);

@@ -94,7 +94,25 @@ inline int bank4_check(const mivos_bank4 *k, const char *what) {
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: bank of %d x %d heads x %lld slots", what, k->batch, k->heads, (long long)k->slots);
   if (k->key_dim < 32 || k->key_dim > 1024 || k->key_dim % 32 || k->value_dim < 32 || k->value_dim > 1024 || k->value_dim % 32)
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: key / value rows of %d / %d channels (multiples of 32 up to 1024)", what, k->key_dim, k->value_dim);
+  if (((uintptr_t)k->key_codes | (uintptr_t)k->key_scales | (uintptr_t)k->value_codes | (uintptr_t)k->value_scales) & 15)
+    return fail(MIVOS_ERR_INVALID_ARGUMENT, "%s: codes and scales must be 16-byte aligned", what);
   return MIVOS_OK;
+}
+
+struct Span {
+  uintptr_t first, end;
+  Span(const void *p, int64_t bytes) : first((uintptr_t)p), end((uintptr_t)p + bytes) {}
+  bool meets(const Span &o) const { return first < o.end && o.first < end; }
+};
+// whether a buffer of the one bank shares memory with a buffer of the other
+inline bool bank4_meet(const mivos_bank4 &x, const mivos_bank4 &y) {
+  auto spans = [](const mivos_bank4 &k, auto &&use) {
+    const int64_t rows = (int64_t)k.batch * k.heads * k.slots;
+    return use(Span(k.key_codes, rows * k.key_dim / 2)) || use(Span(k.key_scales, rows * k.key_dim / 32)) || use(Span(k.value_codes, rows * k.value_dim / 2)) ||
+           use(Span(k.value_scales, rows * k.value_dim / 32)) || use(Span(k.weight, rows * 4)) || use(Span(k.lens, (int64_t)k.batch * 4)) ||
+           use(Span(k.status, (int64_t)(1 + k.batch) * 4));
+  };
+  return spans(x, [&](const Span &a) { return spans(y, [&](const Span &b) { return a.meets(b); }); });
 }
 
 }  // namespace mivos

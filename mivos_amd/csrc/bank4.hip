@@ -313,6 +313,9 @@ extern "C" int mivos_bank4_append(const mivos_bank4 *bank, const void *keys, int
                                   int64_t vt, int64_t vh, int dtype, const int32_t *at, const int32_t *count, int tokens, void *stream) {
   if (int rc = bank4_check(bank, "bank4_append")) return rc;
   if (!dtype_ok(dtype) || tokens < 0 || !at || (tokens && (!keys || !values))) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_append: bad argument");
+  const Span lens(bank->lens, (int64_t)bank->batch * 4);
+  if ((at != bank->lens && lens.meets(Span(at, (int64_t)bank->batch * 4))) || (count && lens.meets(Span(count, (int64_t)bank->batch * 4))))
+    return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_append: at or count overlaps the bank's lengths");
   if ((int64_t)tokens * bank->heads > 0x7fffffff) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_append: %d tokens x %d heads", tokens, bank->heads);
   const int units = (bank->key_dim + bank->value_dim) / 8, es = dtype_bytes(dtype);
   const int64_t all = kb | kt | kh | vb | vt | vh;
@@ -345,8 +348,7 @@ extern "C" int mivos_bank4_evict(const mivos_bank4 *bank, const mivos_bank4 *out
   if (int rc = bank4_check(out, "bank4_evict")) return rc;
   if (out->batch != bank->batch || out->heads != bank->heads || out->key_dim != bank->key_dim || out->value_dim != bank->value_dim)
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_evict: the two banks differ in streams, heads or channels");
-  if (out->key_codes == bank->key_codes || out->value_codes == bank->value_codes || out->weight == bank->weight || out->lens == bank->lens)
-    return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_evict: the banks share memory");
+  if (bank4_meet(*bank, *out)) return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_evict: the banks share memory");
   if (keep < 1 || keep > out->slots || first < 0 || recent < 0 || first + recent > keep || !slots_out)
     return fail(MIVOS_ERR_INVALID_ARGUMENT, "bank4_evict: keep %lld of %lld slots, first %lld, recent %lld", (long long)keep, (long long)out->slots,
                 (long long)first, (long long)recent);

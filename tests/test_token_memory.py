@@ -167,3 +167,30 @@ def test_c_entries_check_their_arguments_without_a_gpu():
     assert lib.mivos_norm_rotary_grad(r, None, None, None) == -1
     assert C.sizeof(_lib.RotaryRows) == 88 and C.sizeof(_lib.Bank4Desc) == 80
     assert C.sizeof(_lib.RotaryDesc) == ops._ROTARY.size and _lib.RotaryDesc.eps.offset + 4 == ops._ROTARY.size
+
+
+def test_c_entries_refuse_overlapping_and_unaligned_buffers():
+    """What the Python wrappers refuse, the C entries refuse too: counts on top of the lengths that append writes, a bank that shares any of its
+    seven buffers with the one it is brought down from, codes and scales off 16 bytes."""
+    lib = _lib.load()
+    b, o = _bank(), _bank(slots=8)
+    d = b._desc
+    copy = lambda s: _lib.Bank4Desc(*(getattr(s, n) for n, _ in s._fields_))  # noqa: E731
+    append = lambda desc, at, count: lib.mivos_bank4_append(desc, 16, 0, 0, 0, 16, 0, 0, 0, 0, at, count, 3, None)  # noqa: E731
+    for at, count in ((d.lens + 4, None), (d.lens - 4, None), (64, d.lens), (64, d.lens + 4), (d.lens, d.lens - 4), (d.lens, d.lens)):
+        assert append(d, at, count) == -1 and b"overlap" in lib.mivos_last_error(), (at - d.lens, count)
+    last = {"key_codes": 2 * 2 * 16 * 32, "key_scales": 2 * 2 * 16 * 2, "value_codes": 2 * 2 * 16 * 32, "value_scales": 2 * 2 * 16 * 2, "weight": 2 * 2 * 16 * 4, "lens": 8,
+            "status": 12}
+    for name, size in last.items():
+        for at in (getattr(d, name), getattr(d, name) + (size - 16 if size > 16 else size - 4)):
+            c = copy(o._desc)
+            setattr(c, name, at)
+            assert lib.mivos_bank4_evict(d, c, 4, 0, 0, 64, None) == -1 and b"share memory" in lib.mivos_last_error(), name
+    c = copy(o._desc)
+    c.value_codes = d.weight                                       # one buffer of the one, another of the other
+    assert lib.mivos_bank4_evict(d, c, 4, 0, 0, 64, None) == -1 and b"share memory" in lib.mivos_last_error()
+    for name in ("key_codes", "key_scales", "value_codes", "value_scales"):
+        c = copy(d)
+        setattr(c, name, getattr(d, name) + 8)
+        assert append(c, d.lens, None) == -1 and b"aligned" in lib.mivos_last_error(), name
+        assert lib.mivos_bank4_values(c, None, 1, 16, 16, 0, None) == -1 and lib.mivos_bank4_read_workspace_bytes(c, 4, 5, 0, 1) == -1
