@@ -1118,8 +1118,8 @@ class RotaryAxes:
         pairs = sum(sections)
         if not sections or min(sections) < 0 or pairs < 1 or 2 * pairs > head_dim or head_dim > 512:
             raise MivosHipError(f"RotaryAxes: sections {sections} (channel pairs an axis) do not fit heads of {head_dim} channels (at most 512)")
-        if not 0 < base < float("inf"):
-            raise MivosHipError(f"RotaryAxes: base {base}")
+        if not 1e-30 <= base < float("inf"):      # (50 digits hold 2^64 / base to a unit)
+            raise MivosHipError(f"RotaryAxes: base {base} (from 1e-30 up)")
         self.head_dim, self.sections, self.pairs, self.interleaved = int(head_dim), sections, pairs, bool(interleaved)
         turns, axes = _rotary_table(sections, float(base), bool(shared))
         self.freq = torch.tensor(turns, dtype=torch.int64, device=device)

@@ -194,3 +194,16 @@ def test_c_entries_refuse_overlapping_and_unaligned_buffers():
         setattr(c, name, getattr(d, name) + 8)
         assert append(c, d.lens, None) == -1 and b"aligned" in lib.mivos_last_error(), name
         assert lib.mivos_bank4_values(c, None, 1, 16, 16, 0, None) == -1 and lib.mivos_bank4_read_workspace_bytes(c, 4, 5, 0, 1) == -1
+
+
+def test_rotary_plan_bases_at_the_limits():
+    """Frequencies of the smallest base against exact fractions, and the bases below it, whose fractions of a turn 50 digits do not hold."""
+    from fractions import Fraction
+    pi = Fraction(31415926535897932384626433832795028841971693993751058209749445923078164062862089986280348253421170679, 10 ** 100)
+    plan = ops.RotaryAxes(8, (2, 1, 1), base=2.0 ** -96, device="cpu")      # the second pair: 2^48
+    turn = Fraction(2 ** 64) / (2 * pi)
+    for i, f in ((0, 1), (1, 2 ** 48), (2, 1), (3, 1)):
+        away = (int(plan.freq[i]) - turn * f) % 2 ** 64
+        assert min(away, 2 ** 64 - away) <= 1
+    for base in (1e-31, 5e-324, 0.0, -1.0, math.inf, math.nan):
+        _raises("base", ops.RotaryAxes, 8, (4,), base=base, device="cpu")
