@@ -517,7 +517,8 @@ int mivos_bank4_values(const mivos_bank4 *bank, const int32_t *first, int64_t co
  * [batch][tokens][q_heads][value_dim] = softmax over the visible slots of scale * q . k, times v.  Visible: all filled slots; causal: token t
  * of count[b] (NULL: tokens) sees slots < lens[b] - count[b] + t + 1 (the tokens are the newest ones, already appended).  Tokens >= count[b]
  * and rows that see nothing give 0.  weigh: weight[b][h][s] += the softmax weights of the stream's rows on slot s.  key_dim 64, 128 or 256,
- * value_dim a multiple of 64, at most 2^20 rows (tokens x q_heads / heads) and |scale| up to 1e38. */
+ * value_dim a multiple of 64, at most 2^20 rows (tokens x q_heads / heads), |scale| up to 1e38; batch x heads x value_dim / 64
+ * up to 65 535 is always taken (beyond it the entry may refuse). */
 int64_t mivos_bank4_read_workspace_bytes(const mivos_bank4 *bank, int q_heads, int tokens, int dtype, int weigh);
 int mivos_bank4_read(const mivos_bank4 *bank, const void *q, int64_t qb, int64_t qt, int64_t qh, int dtype, int q_heads, int tokens, const int32_t *count,
                      float scale, int causal, int weigh, void *out, void *workspace, int64_t workspace_bytes, void *stream);

@@ -424,15 +424,17 @@ struct QueryCols {
 // operand of the second product.  The running maximum is moved (and the accumulators rescaled) only when a logit passes it by 2^LAG.
 // F16: the products on fp16 numbers, which carry three bits more than bf16 ones.  fp16 and fp32 queries: q in 1 / 2 of them (fp32 rows brought to
 // 2^14 first), the softmax weight times 2^12 in 2 (2^-22 of itself or 2^-37 of the row's largest; the maximum is followed closer, by 2^3).  bf16
-// queries: keys and q as bf16, the weight times 2^8 in 1 (2^-11 of itself or 2^-33 of the row's largest; one bf16 number, 2^-8 of it, put the error of
-// 3 x 1021 causal tokens over 16 300 slots at 1.3 times that of fp32 weights, two take 489 us there: 359, 372 and 489).
-// A 4-bit value is exact in fp16 from 2^-24 to 6 * 2^13; a workgroup that has met a block outside, or keys above it, whose logits lie so far apart that
-// such weights lose channels, does its work again on bf16 numbers (twice the time and more, for that workgroup; 5 us for the launch where no flag is up).  2 x 1620 fp32 rows x 32 400 slots,
-// 128 / 512: 400 us instead of 471, 0.81 PFLOP/s issued; all 512 value channels in one workgroup would need registers it does not have.
-// F16: `again` says that the workgroup has met such a block; then it has written nothing.
+// queries: keys and q as bf16, the weight times 2^8 in 1 (2^-11 of itself or 2^-33 of the row's largest).  One bf16 number, 2^-8 of the weight, put
+// the error of 3 x 1021 causal tokens over 16 300 slots at 1.3 times that of fp32 weights, two take 489 us there: 359, 372 and 489.
+// A 4-bit value is exact in fp16 from 2^-24 to 6 * 2^13.  A workgroup that has met a block outside (of keys under bf16 queries: above, where logits may
+// lie so far apart that such weights lose channels), or an fp32 row that loses channels to its keys (key_byte_limit), does its work again on
+// bf16 numbers: where all do, 1000 tokens, 4 over 2 heads, 16 384 slots take 99 us instead of 59 (bf16) and 165 instead of 85 (fp32).
+// 2 x 1620 fp32 rows x 32 400 slots, 128 / 512: 400 us instead of 471 on bf16 numbers alone, 0.81 PFLOP/s issued; all 512 value channels in one
+// workgroup would need registers it does not have.
+// F16: `again` says that the workgroup has met such a block or row; then it has written nothing.
 // (The body is in bank4_block.h, once as a kernel's own text and once as a function's: in a function that a kernel calls, the compiler orders a step
 // otherwise, and 3 x 1021 causal fp32 tokens over 16 300 slots take 860 us instead of 800.)
-// fp16 and fp32 queries: F16 raises the workgroup's flag, and the bf16 kernel is launched behind.
+// fp16 and fp32 queries: F16 raises the workgroup's flag, and the bf16 kernel is launched behind (5 us where no flag is up).
 template <int DK, int DVC, int PARTS, bool F16, bool CAUSAL>
 __global__ __launch_bounds__(256, block_occupancy(DK, DVC, PARTS)) void bank4_block_kernel(ReadArgs a) {
   int32_t *redo = a.redo + (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
@@ -772,7 +774,9 @@ static int read_plan(const mivos_bank4 *k, int q_heads, int tokens, int weigh, i
   } else {
     const int64_t want = groups ? (2048 + groups - 1) / groups : 1, most = (k->slots + 255) / 256;
     p->nsplit = (int)(want < most ? want : most);
-    p->nsplit = p->nsplit > 128 ? 128 : p->nsplit < 1 || k->slots <= 1024 ? 1 : p->nsplit;     // (a short bank: no second launch)
+    p->nsplit = p->nsplit > 128 ? 128 : p->nsplit < 1 || k->slots <= 1024 ? 1 : p->nsplit;
+    // (a short bank: no second launch; 1 token, 1 to 64 heads, values of 64 to 512: 8.3 - 10.5 us at 1024 slots, 11.7 - 11.8 in slices at 1025; with
+    // the weights gathered, which take that launch anyway, 15.7 and 11.9.  The plan knows the capacity only: 1000 slots filled of 65 536 take 19 us)
   }
   p->parts = p->nsplit > 1 || weigh;
   const int64_t n = (int64_t)k->batch * k->heads * p->nsplit * rows;

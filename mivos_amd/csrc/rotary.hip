@@ -53,7 +53,8 @@ __device__ __forceinline__ void turn_sincos(int32_t pos, uint64_t freq, float si
 }
 
 // ------------------------------------------------------------------------------------------ any width, any alignment: one wave a row
-// Lane l holds channels l, l + 64, ...; dim <= 512.
+// Lane l holds channels l, l + 64, ...; dim <= 512.  Every channel computes its own sine and cosine and loads are 2 or 4 bytes a lane: bound by
+// instructions, 638 us (norm) and 1340 (gradient) for 32 400 tokens x 20 heads of 128 channels, bf16, where the rows below take 68 and 135.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void rotary_any_kernel(RotaryArgs a) {
   __shared__ float dw[4][2][512];
