@@ -198,6 +198,7 @@
     again = __syncthreads_or(outside);
   }
   if (r < a.rows && !again) {
+    const float inv = live && l != 0.f ? 1.f / l : 0.f;
     if (a.part_o) {
       const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + r;
 #pragma unroll
@@ -205,10 +206,9 @@
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<f32x4 *>(a.part_o + at * a.value_dim + chunk * DVC + i * 32 + j * 8 + half * 4) =
-              f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+              inv == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv};
       if (half == 0 && chunk == 0) *reinterpret_cast<f32x2 *>(a.part_ml + at * 2) = live ? f32x2{m, l} : f32x2{-INFINITY, 0.f};
     } else {
-      const float inv = live && l != 0.f ? 1.f / l : 0.f;
       T *out = (T *)a.out + (((int64_t)b * a.tokens + t) * a.heads * a.group + h * a.group + r - t * a.group) * a.value_dim + chunk * DVC;
 #pragma unroll
       for (int i = 0; i < NT; ++i)

@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256, PARTS == 1 && DK <= 128 ? 3 : 2) void bank4_ro
     }
     if (a.part_o) {
       const int64_t at = ((int64_t)bh * a.nsplit + split) * a.rows + row;
-      a.part_o[at * a.value_dim + chunk * DVC + dv] = acc;
+      a.part_o[at * a.value_dim + chunk * DVC + dv] = valid && sum != 0.f ? acc / sum : 0.f;
       if (dv == 0 && chunk == 0) *reinterpret_cast<f32x2 *>(a.part_ml + at * 2) = valid ? f32x2{mm, sum} : f32x2{-INFINITY, 0.f};
     } else {
       const int j = h * a.group + row - tt * a.group;
@@ -583,8 +583,9 @@ __global__ __launch_bounds__(256) void bank4_weigh_kernel(ReadArgs a) {
   }
 }
 
-// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum of the weights, and the factors of its slices'
-// accumulators (-1: an empty slice).
+// A row's slices: lane s holds slice s (and s + 64).  Gives every lane the row's maximum, 1 / sum of the weights, and the shares of its slices in that
+// sum.  A slice's partial output is divided by its own sum already: the maximum that this sum is taken against differs between the
+// workgroups of a row's value channels where some run on fp16 numbers and some on bf16 ones, and only the first leaves its maximum and sum here.
 struct RowJoin {
   float f[2], inv, top;
   __device__ __forceinline__ RowJoin(const ReadArgs &a, int bh, int row, int lane) {
@@ -600,14 +601,12 @@ struct RowJoin {
     float mm = fmaxf(m[0], m[1]);
     for (int d = 1; d < 64; d <<= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     const float mu = mm == -INFINITY ? 0.f : mm;
-    f[0] = __builtin_amdgcn_exp2f(m[0] - mu);
-    f[1] = __builtin_amdgcn_exp2f(m[1] - mu);
-    float sum = f[0] * l[0] + f[1] * l[1];
+    f[0] = __builtin_amdgcn_exp2f(m[0] - mu) * l[0];
+    f[1] = __builtin_amdgcn_exp2f(m[1] - mu) * l[1];
+    float sum = f[0] + f[1];
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
     inv = sum != 0.f ? 1.f / sum : 0.f;
     top = mu;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) f[k] = m[k] == -INFINITY && l[k] == 0.f ? -1.f : f[k];       // an empty slice: its accumulators may be anything
   }
 };
 
@@ -640,7 +639,7 @@ __global__ __launch_bounds__(256) void bank4_join_kernel(ReadArgs a, int out_blo
       const float f0 = __shfl(J.f[0], s & 63), f1 = __shfl(J.f[1], s & 63), f = s < 64 ? f0 : f1;
       const f32x4 x = *reinterpret_cast<const f32x4 *>(from + (s < a.nsplit ? s : 0) * stride);      // (no branch: all loads go out together)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[c] += s < a.nsplit && f >= 0.f ? f * x[c] : 0.f;
+      for (int c = 0; c < 4; ++c) acc[c] += s < a.nsplit ? f * x[c] : 0.f;
     }
 #pragma unroll
     for (int d = QL; d < 64; d <<= 1)

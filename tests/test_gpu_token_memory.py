@@ -788,3 +788,17 @@ def test_rotary_angles_are_rounded_not_cut():
             ref = sign * torch.sin(pos.double() * 2 * math.pi * r * 2.0 ** -32)
             got = y[0, :, 0, 1 + pairs].double().cpu()
             assert bool(((got - ref).abs() <= 2 * math.pi * (2.0 ** -33 + 2.0 ** -34) + 2.0 ** -21 * ref.abs()).all()), (dim, sign, got, ref)
+
+
+@pytest.mark.parametrize("weigh", (False, True))
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("dk,dv,slots", [(128, 512, 2500), (64, 192, 90), (256, 256, 1300)])
+def test_read_blocks_outside_fp16_in_some_channels(dk, dv, slots, dtype, weigh):
+    """Value blocks outside fp16 in some of a row's channels: the workgroups of those channels run on other numbers than those of the rest, over one slice
+    or several, and the rows' slices are joined all the same."""
+    bank = _filled(2, 1, slots, dk, dv, (slots, slots - 20))
+    bank.value_scales[0, 0, 5, 0] = 150
+    bank.value_scales[1, 0, slots // 2, dv // 32 - 1] = 80
+    q = 2 * torch.randn(2, 50, 2, dk, generator=torch.Generator().manual_seed(8))
+    for causal in (False, True):
+        _check_many(bank, q.to(dtype), causal, weigh, None)
